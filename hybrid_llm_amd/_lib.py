@@ -39,6 +39,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                           _I, _F, _P]),
     "llmy_banded_attn_decode_parts_bf16": (_I, [_P, _I, _I64, _I64, _I, _I, _P, _P, _P, _P, _I,
                                                 _I, _I, _I, _F, _P]),
+    "llmy_qk_norm_rope_bf16": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I, _P, _P, _F, _I,
+                                    _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _I, _P]),
+    "llmy_paged_kv_append": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I, _F, _F, _P, _P, _P,
+                                  _P, _I, _P, _F, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _I,
+                                  _I, _I, _I, _I, _I, _I, _I, _P]),
+    "llmy_paged_attn_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
+    "llmy_paged_attn_decode": (_I, [_P, _I64, _I64, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P, _I64,
+                                    _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
     "llmy_gdn_prefill_workspace_bytes": (C.c_int64, [_I, _I, _I, _I, _I]),
     "llmy_gdn_prefill_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _P]),
     "llmy_gdn_prefill_bf16_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),

@@ -1,0 +1,605 @@
+// Attention of one new token per sequence over a paged key-value cache:
+//   z_j = scale q . k_j, capped: c tanh(z / c), less slope_h (len - 1 - j);
+//   o = sum_j softmax(z)_j v_j over the positions max(0, len - W) <= j < len,
+// query head h reading key-value head h / (Hq / Hkv).  Cache and page table as in
+// paged.hpp, bf16 or e4m3 times a scale.
+//
+// Bound by the read of K and V, whatever the grouping: a group's query heads (up to
+// 16) are the columns of one 16 x 16 x 32 MFMA, so a key row is read once for all of
+// them, and the matrix cores do with 16 columns what vector code would have to do once
+// per head.
+//   * S^T = K Q^T: lane l (g = l / 16) gets keys 4 g + r of a 16-key tile for head
+//     l % 16.  Two such tiles are, register by register, the B operand of a 32-key
+//     product O^T += V^T P^T under the key order 4 g + j, 16 + 4 g + j, so the
+//     weights never leave their registers; V^T comes from transposing LDS reads of
+//     row-major V rows in that order.
+//   * a wave is a workgroup and works alone: its 32-key steps arrive by DMA into 2 or
+//     3 LDS stages of its own and nothing ever waits for another wave.  Four to ten
+//     waves a CU keep 64 KiB and more in flight per CU, several times what the read
+//     rate needs to cover a load's latency.
+//   * the work is the flat list of all (sequence, key-value head, step), cut into
+//     equal runs: one run per wave, found from the lengths on the device.  A batch of
+//     any mixture of lengths is balanced, and the host never learns the lengths.  A
+//     run that starts or ends inside a head's steps leaves (m, l, O) partials in the
+//     workspace, at most two, and a second kernel joins them; a head that lies in
+//     one run is stored by that wave.  A cache too short to be cut takes one wave a
+//     head and no second launch.
+//   * the page ids come by scalar loads (a page holds whole 16-key tiles, so they are
+//     the same for every lane of a DMA), which leaves the vector counter to the DMAs.
+// Masked keys (past the length, before the window, in a page that the table does not
+// name) have their scores set to -inf and their V rows zeroed in LDS, so nothing
+// that such a place holds, NaN and infinities included, reaches a sum.
+//
+// Weights are rounded to bf16 for the product; their sum adds the rounded ones, so a
+// head that looks at one key returns that key's value exactly.  e4m3 converts to
+// bf16 without rounding; its scales go into the score scale and the final factor.
+#include "common.hpp"
+#include "abi_util.hpp"
+#include "attn_tile.hpp"
+#include "paged.hpp"
+
+namespace llmy {
+
+// Read-only words at wave-uniform addresses, by scalar loads.
+typedef const int32_t __attribute__((address_space(4)))* const_i32;
+
+__device__ __forceinline__ int32_t scalar_at(const int32_t* p, long long i) {
+  return reinterpret_cast<const_i32>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+constexpr int kStep = 32;      // keys a step
+constexpr int kMinSteps = 4;   // least steps of a run: 128 keys
+
+struct PagedArgs {
+  const uint16_t* q;
+  long long qb, qh;            // strides of q by sequence and head (elements)
+  const uint8_t *kc, *vc;
+  const int32_t *table, *lengths;
+  uint16_t* out;               // [B, Hq, HD]
+  float *po, *pml;             // partials: O [2 runs, GT, HD] and (m, l) [2 runs, GT, 2]
+  const float* slopes;
+  float scale_log2, cap_log2, cap_x2, v_scale;
+  int B, hq, hkv, G, HT, GT;   // G = Hq / Hkv in HT tiles of GT <= 16 heads
+  int width, shift, pages, window, cap_len;
+  int runs;                    // 0: one wave a (sequence, head tile), no join
+};
+
+struct Seq {
+  int len, lo, s0, s1;         // visible positions [lo, len), steps [s0, s1)
+};
+
+__device__ __forceinline__ Seq seq_of(int len, int cap_len, int window) {
+  Seq s;
+  s.len = min(max(len, 0), cap_len);
+  s.lo = window > 0 ? max(0, s.len - window) : 0;
+  s.s0 = s.lo / kStep;
+  s.s1 = static_cast<int>((static_cast<unsigned>(s.len) + kStep - 1) / kStep);
+  return s;
+}
+
+__device__ __forceinline__ long long shfl_up64(long long v, int d) {
+  const int lo = __shfl_up(static_cast<int>(v & 0xffffffffll), d, kWave);
+  const int hi = __shfl_up(static_cast<int>(v >> 32), d, kWave);
+  return (static_cast<long long>(hi) << 32) | static_cast<uint32_t>(lo);
+}
+
+__device__ __forceinline__ long long readlane64(long long v, int l) {
+  const int lo = __builtin_amdgcn_readlane(static_cast<int>(v & 0xffffffffll), l);
+  const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+  return (static_cast<long long>(hi) << 32) | static_cast<uint32_t>(lo);
+}
+
+// Steps of all sequences, as sums over 64 blocks of `per` sequences, one per lane.
+struct StepScan {
+  long long before, upto, total;  // this lane's block: exclusive and inclusive sums
+  int per;
+};
+
+__device__ __forceinline__ StepScan scan_steps(const PagedArgs& a, int lane) {
+  StepScan r;
+  r.per = (a.B + kWave - 1) / kWave;
+  long long n = 0;
+  const int b1 = min(a.B, (lane + 1) * r.per);
+  for (int b = lane * r.per; b < b1; ++b) {
+    const Seq s = seq_of(a.lengths[b], a.cap_len, a.window);
+    n += s.s1 - s.s0;
+  }
+  r.upto = n;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const long long o = shfl_up64(r.upto, d);
+    if (lane >= d) r.upto += o;
+  }
+  r.before = r.upto - n;
+  r.total = readlane64(r.upto, kWave - 1);
+  return r;
+}
+
+__device__ __forceinline__ int run_steps(long long total, int runs) {
+  const long long q = (total + runs - 1) / runs;
+  return static_cast<int>(q > kMinSteps ? q : kMinSteps);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void lds_settle2(u32x4* f) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1])::"memory");
+}
+
+__device__ __forceinline__ void lds_settle_v4(u32x2* f) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3])::"memory");
+}
+
+// 8 e4m3 codes as bf16 (exact).
+__device__ __forceinline__ bf16x8 e4m3_to_bf16(uint32_t lo, uint32_t hi) {
+  uint4 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  return as_bf16x8(r);
+}
+
+// Staged rows keep their 16-byte chunks XOR-swizzled so that the fragment reads below
+// spread over the banks: 8 lanes reading one chunk of 8 consecutive key rows, and a
+// 16-lane group reading 4 (bf16) or 8 (e4m3) key rows of one transposed V tile.
+template <int HD, bool F8>
+struct Tile {
+  static constexpr int RB = HD * (F8 ? 1 : 2);       // bytes a row
+  static constexpr int CH = RB / 16;                 // chunks a row
+  static constexpr int RPB = 64 / CH;                // rows of one 1 KiB DMA
+  static constexpr int NB = kStep / RPB;             // DMAs of a K or V tile
+  static constexpr int BYTES = kStep * RB;           // of a K or V tile
+  static constexpr int STAGES = BYTES >= 8192 ? 2 : 3;
+  static __device__ __forceinline__ int kswz(int row) {
+    return CH == 4 ? (row >> 1) & 3 : row & 7;
+  }
+  static __device__ __forceinline__ int vswz(int row) {
+    if (!F8) return 2 * (row & 3);
+    const int n = (row & 3) | ((row >> 2) & 4);  // its place among the group's 8 rows
+    return CH == 4 ? n >> 1 : n;
+  }
+};
+
+template <int HD, bool F8>
+__global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
+  using T = Tile<HD, F8>;
+  constexpr int RB = T::RB, NB = T::NB, ST = T::STAGES;
+  constexpr int NS = HD / 32;                 // 32-dim slices of the score product
+  constexpr int ND = HD / 16;                 // 16-dim output tiles
+  constexpr int NK = F8 ? HD / 64 : HD / 32;  // 16-byte K reads of a 16-key tile
+  __shared__ __align__(1024) uint8_t smem[ST * 2 * T::BYTES];
+
+  const int lane = threadIdx.x;
+  const int g = lane >> 4, col = lane & 15;
+  const int units = a.hkv * a.HT;
+
+  // this wave's run: `count` steps from step s of head tile u of sequence b on
+  int b, u, s, count, run_q = 0;
+  long long run_at = 0;
+  Seq cur;
+  if (a.runs == 0) {
+    b = blockIdx.x / units;
+    u = blockIdx.x - b * units;
+    cur = seq_of(scalar_at(a.lengths, b), a.cap_len, a.window);
+    s = cur.s0;
+    count = cur.s1 - cur.s0;
+    if (count == 0) {  // nothing visible: zeros
+      const int kvh = u / a.HT, ht = u - kvh * a.HT;
+      const int heads = min(16, a.G - 16 * ht);
+      uint16_t* o = a.out + (static_cast<long long>(b) * a.hq + kvh * a.G + 16 * ht) * HD;
+      for (int e = 8 * lane; e < heads * HD; e += 512)
+        *reinterpret_cast<uint4*>(o + e) = uint4{0u, 0u, 0u, 0u};
+      return;
+    }
+  } else {
+    const StepScan sc = scan_steps(a, lane);
+    const long long total = sc.total * units;
+    run_q = run_steps(total, a.runs);
+    run_at = static_cast<long long>(blockIdx.x) * run_q;
+    if (run_at >= total) return;
+    count = static_cast<int>(min(static_cast<long long>(run_q), total - run_at));
+    const int blk = __ffsll(static_cast<unsigned long long>(__ballot(sc.upto * units > run_at))) - 1;
+    long long at = readlane64(sc.before, blk);
+    b = blk * sc.per;
+    for (;; ++b) {  // ends: the block's sum passes run_at
+      cur = seq_of(scalar_at(a.lengths, b), a.cap_len, a.window);
+      if ((at + cur.s1 - cur.s0) * units > run_at) break;
+      at += cur.s1 - cur.s0;
+    }
+    const long long rem = run_at - at * units;
+    u = static_cast<int>(rem / (cur.s1 - cur.s0));
+    s = cur.s0 + static_cast<int>(rem - static_cast<long long>(u) * (cur.s1 - cur.s0));
+  }
+
+  // DMA lanes: lane p of block j fills row RPB j + p / CH, chunk slot p % CH
+  uint32_t kdo[NB], vdo[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int r = T::RPB * j + lane / T::CH, sl = lane % T::CH;
+    kdo[j] = (lane / T::CH) * RB + 16 * (sl ^ T::kswz(r));
+    vdo[j] = (lane / T::CH) * RB + 16 * (sl ^ T::vswz(r));
+  }
+  unsigned bad = 0;  // two bits a stage: its 16-key tiles whose page the table does not name
+  int ib = b, iu = u, is = s;
+  Seq icur = cur;
+  auto next = [&](int& nb, int& nu, int& ns, Seq& q) {  // the step after; the caller counts
+    if (++ns < q.s1) return;
+    if (++nu == units) {
+      nu = 0;
+      do {
+        q = seq_of(scalar_at(a.lengths, ++nb), a.cap_len, a.window);
+      } while (q.s0 == q.s1);
+    }
+    ns = q.s0;
+  };
+  auto issue = [&](int st) {
+    const int kvh = iu / a.HT;
+    const long long row = static_cast<long long>(ib) * a.width;
+    const int key0 = is * kStep;
+    const int last = (icur.len - 1) >> a.shift;  // keys past the length stay in its page
+    uint8_t* sk = smem + st * 2 * T::BYTES;
+    bad &= ~(3u << (2 * st));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = key0 + 16 * h;
+      const int page = scalar_at(a.table, row + min(key >> a.shift, last));
+      const bool ok = page >= 0 && page < a.pages;
+      if (!ok) bad |= 1u << (2 * st + h);
+      const long long at = (((static_cast<long long>(ok ? page : 0) * a.hkv + kvh) << a.shift) +
+                            (key & ((1 << a.shift) - 1))) * RB;
+      const uint8_t *kp = a.kc + at, *vp = a.vc + at;
+#pragma unroll
+      for (int j = 0; j < NB / 2; ++j) {
+        const int blk = h * (NB / 2) + j;
+        dma16(kp + j * 1024 + kdo[blk], sk + blk * 1024);
+        dma16(vp + j * 1024 + vdo[blk], sk + T::BYTES + blk * 1024);
+      }
+    }
+  };
+
+  // fragment offsets (bytes from a stage's K or V tile)
+  const uint32_t sbase = lds_addr(smem);
+  uint32_t koff[NK], voff[ND];
+#pragma unroll
+  for (int t = 0; t < NK; ++t) koff[t] = col * RB + 16 * ((4 * t + g) ^ T::kswz(col));
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    if (F8) {
+      const int n = col >> 1, row = (n < 4 ? 0 : 16) + 4 * g + (n & 3);
+      voff[d] = row * RB + 16 * (d ^ T::vswz(row)) + 8 * (col & 1);
+    } else {
+      const int row = 4 * g + (col >> 2), dim = 16 * d + 4 * (col & 3);
+      voff[d] = row * RB + 16 * ((dim >> 3) ^ T::vswz(row)) + 2 * (dim & 7);
+    }
+  }
+
+  int issued = 0;
+  for (; issued < ST && issued < count; ++issued) {
+    if (issued) next(ib, iu, is, icur);
+    issue(issued);
+  }
+
+  uint4 qf[NS];
+  f32x4 acc[ND];
+  float m_run = -INFINITY, l_run = 0.f, slope = 0.f;
+  bool fresh = true;
+  int st = 0;
+  for (int i = 0; i < count; ++i) {
+    const int kvh = u / a.HT, ht = u - kvh * a.HT;
+    const int heads = min(16, a.G - 16 * ht);
+    const int h0 = kvh * a.G + 16 * ht;
+    if (fresh) {
+      fresh = false;
+      const uint16_t* qp = a.q + b * a.qb + (h0 + min(col, heads - 1)) * a.qh;
+#pragma unroll
+      for (int t = 0; t < NS; ++t) {
+        const int d0 = F8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
+        qf[t] = *reinterpret_cast<const uint4*>(qp + d0);
+      }
+      if (a.slopes) slope = a.slopes[h0 + min(col, heads - 1)] * 1.4426950408889634f;
+      m_run = -INFINITY;
+      l_run = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // DMAs complete in order: this stage has landed once only later stages' are out
+    if (issued - i == ST) wait_vm<(ST - 1) * 2 * NB>();
+    else wait_vm<0>();
+    const uint32_t kst = sbase + st * 2 * T::BYTES, vst = kst + T::BYTES;
+    const int key0 = s * kStep;
+    const unsigned hole = (bad >> (2 * st)) & 3u;
+    const bool edge = key0 < cur.lo || key0 + kStep > cur.len || hole;
+
+    u32x4 kf[2 * NK];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int t = 0; t < NK; ++t) kf[k * NK + t] = lds_b128(kst + 16 * k * RB + koff[t]);
+    if (edge) {  // masked keys' V rows are zeroed
+      for (int e = lane; e < kStep * T::CH; e += 64) {
+        const int row = e / T::CH, key = key0 + row;
+        if (key < cur.lo || key >= cur.len || ((hole >> (row >> 4)) & 1u))
+          *reinterpret_cast<uint4*>(smem + st * 2 * T::BYTES + T::BYTES + 16 * e) =
+              uint4{0u, 0u, 0u, 0u};
+      }
+      wave_lds_order();
+    }
+    if constexpr (NK == 1) lds_settle2(kf);
+    else
+#pragma unroll
+      for (int t = 0; t < 2 * NK; t += 4) lds_settle4(kf + t);
+    constexpr int NV = F8 ? ND : 2 * ND;
+    u32x2 vf[NV];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      if (F8) {
+        vf[d] = lds_tr8(vst + voff[d]);
+      } else {
+        vf[2 * d] = lds_tr16(vst + voff[d]);
+        vf[2 * d + 1] = lds_tr16(vst + voff[d] + 16 * RB);
+      }
+    }
+    f32x4 sc[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      sc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < NS; ++t) {
+        bf16x8 kk;
+        if (F8) {
+          const u32x4 w = kf[k * NK + t / 2];
+          kk = (t & 1) ? e4m3_to_bf16(w.z, w.w) : e4m3_to_bf16(w.x, w.y);
+        } else {
+          kk = __builtin_bit_cast(bf16x8, kf[k * NK + t]);
+        }
+        sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, as_bf16x8(qf[t]), sc[k], 0, 0, 0);
+      }
+    }
+    float z[8];
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float x = sc[j >> 2][j & 3];
+      x = a.cap_x2 > 0.f ? softcap_log2(x * a.cap_x2, a.cap_log2) : x * a.scale_log2;
+      const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+      if (a.slopes) x -= slope * static_cast<float>(cur.len - 1 - key);
+      if (edge && (key < cur.lo || key >= cur.len || ((hole >> (j >> 2)) & 1u))) x = -INFINITY;
+      z[j] = x;
+      mloc = fmaxf(mloc, x);
+    }
+    // the offset moves only when some score passes it by more than 8 (weights stay
+    // below 2^8), decided by the wave; all four lanes of a head take the same one
+    if (__ballot(!(mloc <= m_run + 8.f))) {
+      mloc = fmaxf(mloc, __shfl_xor(mloc, 16, kWave));
+      mloc = fmaxf(mloc, __shfl_xor(mloc, 32, kWave));
+      const float m_new = fmaxf(m_run, mloc);
+      const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] *= alpha;
+    }
+    const float m_sub = m_run == -INFINITY ? 0.f : m_run;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = exp2_fast(z[j] - m_sub);
+    const uint4 pb = pack8_bf16(p);
+    unpack8(pb, p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l_run += p[j];
+    if constexpr (NV == 4) lds_settle_v4(vf);
+    else
+#pragma unroll
+      for (int v = 0; v < NV; v += 8) lds_settle_v(vf + v);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const bf16x8 vv = F8 ? e4m3_to_bf16(vf[d].x, vf[d].y)
+                           : as_bf16x8(uint4{vf[F8 ? 0 : 2 * d].x, vf[F8 ? 0 : 2 * d].y,
+                                             vf[F8 ? 0 : 2 * d + 1].x, vf[F8 ? 0 : 2 * d + 1].y});
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pb), acc[d], 0, 0, 0);
+    }
+    // every read of this stage has returned: the next step may land in it
+    if (issued < count) {
+      next(ib, iu, is, icur);
+      issue(st);
+      ++issued;
+    }
+    st = st + 1 == ST ? 0 : st + 1;
+
+    const bool head_end = s + 1 == cur.s1;
+    if (head_end || i + 1 == count) {
+      float l = l_run + __shfl_xor(l_run, 16, kWave);
+      l += __shfl_xor(l, 32, kWave);
+      // whole: the head's first step lies in this run too
+      const bool whole = head_end && i >= s - cur.s0;
+      if (whole) {
+        const float f = l > 0.f || l != l ? a.v_scale / l : 0.f;
+        uint16_t* o = a.out + (static_cast<long long>(b) * a.hq + h0 + col) * HD + 4 * g;
+        if (col < heads)
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+            *reinterpret_cast<uint2*>(o + 16 * d) =
+                make_uint2(pack_bf2(acc[d][0] * f, acc[d][1] * f),
+                           pack_bf2(acc[d][2] * f, acc[d][3] * f));
+      } else if (col < heads) {
+        // the run starts in this head (or at its first step): 0; else it ends in it: 1
+        const int part = i > s - cur.s0 ? 1 : 0;
+        const long long at = (2ll * blockIdx.x + part) * a.GT + col;
+        float* o = a.po + at * HD + 4 * g;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+          *reinterpret_cast<float4*>(o + 16 * d) =
+              make_float4(acc[d][0], acc[d][1], acc[d][2], acc[d][3]);
+        if (g == 0) *reinterpret_cast<float2*>(a.pml + 2 * at) = make_float2(m_run, l);
+      }
+      fresh = true;
+    }
+    if (i + 1 < count) next(b, u, s, cur);
+  }
+}
+
+// Joins the partials of one (sequence, query head): o = sum_i 2^(m_i - m) O_i /
+// sum_i 2^(m_i - m) l_i, in the runs' order within each of 512 / (HD / 4) lane groups
+// and then over the groups, so the result does not depend on timing.
+template <int HD>
+__global__ __launch_bounds__(512) void paged_join_kernel(const PagedArgs a) {
+  constexpr int LPP = HD / 4;       // lanes a partial
+  constexpr int NG = 512 / LPP;
+  __shared__ __align__(16) float so[NG][HD];
+  __shared__ float sm[NG], sl[NG];
+  const int lane = threadIdx.x & 63;
+  const int grp = threadIdx.x / LPP, c = threadIdx.x % LPP;
+  const int b = blockIdx.x / a.hq, h = blockIdx.x - b * a.hq;
+  const int kvh = h / a.G, ht = (h - kvh * a.G) / 16, row = h - kvh * a.G - 16 * ht;
+  const int units = a.hkv * a.HT, u = kvh * a.HT + ht;
+  uint16_t* out = a.out + static_cast<long long>(blockIdx.x) * HD;
+
+  const StepScan sc = scan_steps(a, lane);
+  const int q = run_steps(sc.total * units, a.runs);
+  const int blk = b / sc.per;
+  long long at = readlane64(sc.before, blk);
+  Seq s;
+  for (int x = blk * sc.per;; ++x) {  // ends at x = b
+    s = seq_of(scalar_at(a.lengths, x), a.cap_len, a.window);
+    if (x == b) break;
+    at += s.s1 - s.s0;
+  }
+  const int n = s.s1 - s.s0;
+  if (n == 0) {  // nothing visible: zeros
+    if (threadIdx.x < LPP) *reinterpret_cast<uint2*>(out + 4 * c) = make_uint2(0u, 0u);
+    return;
+  }
+  const long long first = at * units + static_cast<long long>(u) * n;
+  const int w0 = static_cast<int>(first / q), w1 = static_cast<int>((first + n - 1) / q);
+  if (w0 == w1) return;  // stored by its run
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = w0 + grp; w <= w1; w += NG) {
+    const int part = w == w0 && first != static_cast<long long>(w0) * q ? 1 : 0;
+    const long long i = (2ll * w + part) * a.GT + row;
+    const float2 ml = *reinterpret_cast<const float2*>(a.pml + 2 * i);
+    const float4 x = *reinterpret_cast<const float4*>(a.po + i * HD + 4 * c);
+    const float m_new = fmaxf(m, ml.x);
+    const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+    const float f = exp2_fast(m - m_sub), e = exp2_fast(ml.x - m_sub);
+    o.x = fmaf(x.x, e, o.x * f);
+    o.y = fmaf(x.y, e, o.y * f);
+    o.z = fmaf(x.z, e, o.z * f);
+    o.w = fmaf(x.w, e, o.w * f);
+    l = fmaf(ml.y, e, l * f);
+    m = m_new;
+  }
+  *reinterpret_cast<float4*>(&so[grp][4 * c]) = o;
+  if (c == 0) {
+    sm[grp] = m;
+    sl[grp] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < HD) {
+    const int d = threadIdx.x;
+    float mx = sm[0];
+    for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[i]);
+    const float m_sub = mx == -INFINITY ? 0.f : mx;
+    float num = 0.f, den = 0.f;
+    for (int i = 0; i < NG; ++i) {
+      const float e = exp2_fast(sm[i] - m_sub);
+      num = fmaf(so[i][d], e, num);
+      den = fmaf(sl[i], e, den);
+    }
+    out[d] = f2bf(den > 0.f || den != den ? num * (a.v_scale / den) : 0.f);
+  }
+}
+
+// Waves that the chip holds at once: what a CU's 160 KiB of LDS take, 8 at most.
+inline int paged_runs(int head_dim, bool f8) {
+  const int lds = head_dim == 128 ? (f8 ? 24576 : 32768) : (f8 ? 12288 : 24576);
+  const int per_cu = 163840 / lds;
+  return compute_units() * (per_cu < 8 ? per_cu : 8);
+}
+
+struct PagedPlan {
+  int G, HT, GT, runs;
+  long long cap_len, waves, ws;
+};
+
+inline bool paged_plan(int B, int Hq, int Hkv, int hd, int width, int page, int type,
+                       PagedPlan* p) {
+  if (B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > kMaxHeads || (hd != 64 && hd != 128) ||
+      width < 0 || page_shift(page) < 0 || (type != kCacheBf16 && type != kCacheE4m3))
+    return false;
+  p->G = Hq / Hkv;
+  p->HT = (p->G + 15) / 16;
+  p->GT = p->G < 16 ? p->G : 16;
+  p->cap_len = static_cast<long long>(width) * page;
+  if (p->cap_len >= (1ll << 31) - kStep) return false;  // positions are 32-bit
+  const bool cut = p->cap_len > kMinSteps * kStep;
+  p->runs = cut ? paged_runs(hd, type == kCacheE4m3) : 0;
+  p->waves = cut ? p->runs : static_cast<long long>(B) * Hkv * p->HT;
+  p->ws = cut ? 2ll * p->runs * p->GT * (hd + 2) * 4 : 0;
+  // a run's steps, a unit's number and the grids are 32-bit
+  const double steps = static_cast<double>(B) * Hkv * p->HT * (p->cap_len / kStep + 1);
+  return steps < 1e12 && p->waves < (1ll << 31) && static_cast<long long>(B) * Hq < (1ll << 31);
+}
+
+}  // namespace llmy
+
+using namespace llmy;
+
+extern "C" int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv,
+                                                   int32_t head_dim, int32_t width, int32_t page,
+                                                   int32_t cache_type) {
+  PagedPlan p;
+  return paged_plan(B, Hq, Hkv, head_dim, width, page, cache_type, &p) ? p.ws : -1;
+}
+
+extern "C" int32_t llmy_paged_attn_decode(
+    const llmy_bf16* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
+    int32_t cache_type, float k_scale, float v_scale, const int32_t* page_table,
+    const int32_t* lengths, const float* slopes, llmy_bf16* out, void* workspace,
+    int64_t workspace_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t width,
+    int32_t page, int32_t pages, int32_t window, float scale, float softcap, void* stream) {
+  PagedPlan p;
+  LLMY_REQUIRE(paged_plan(B, Hq, Hkv, head_dim, width, page, cache_type, &p));
+  LLMY_REQUIRE(pages >= 0 && window >= 0 && softcap >= 0.f &&
+               scales_ok(cache_type, k_scale, v_scale));
+  if (B == 0) return 0;
+  LLMY_REQUIRE(q && out && lengths && aligned(q, 16) && aligned(out, 16));
+  LLMY_REQUIRE(q_row % 8 == 0 && q_head % 8 == 0 && q_row >= 0 && q_head >= 0);
+  LLMY_REQUIRE(width == 0 || page_table);
+  // with no page at all every length counts as 0
+  LLMY_REQUIRE(pages == 0 || (k_cache && v_cache && aligned(k_cache, 16) && aligned(v_cache, 16)));
+  LLMY_REQUIRE(p.ws == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= p.ws));
+  PagedArgs a{};
+  a.q = q; a.qb = q_row; a.qh = q_head;
+  a.kc = static_cast<const uint8_t*>(k_cache);
+  a.vc = static_cast<const uint8_t*>(v_cache);
+  a.table = page_table; a.lengths = lengths; a.out = out; a.slopes = slopes;
+  a.po = static_cast<float*>(workspace);
+  a.pml = a.po + 2ll * p.runs * p.GT * head_dim;
+  const float log2e = 1.4426950408889634f, qk = scale * k_scale;
+  a.scale_log2 = qk * log2e;
+  a.cap_log2 = softcap * log2e;
+  a.cap_x2 = softcap > 0.f ? 2.f * log2e * qk / softcap : 0.f;
+  a.v_scale = v_scale;
+  a.B = B; a.hq = Hq; a.hkv = Hkv; a.G = p.G; a.HT = p.HT; a.GT = p.GT;
+  a.width = width; a.shift = page_shift(page); a.pages = pages; a.window = window;
+  a.cap_len = pages ? static_cast<int>(p.cap_len) : 0;
+  a.runs = p.runs;
+  const hipStream_t s = as_stream(stream);
+  const dim3 grid(static_cast<unsigned>(p.waves)), join(static_cast<unsigned>(B) * Hq);
+  const bool f8 = cache_type == kCacheE4m3;
+  if (head_dim == 64) {
+    if (f8) hipLaunchKernelGGL((paged_attn_kernel<64, true>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<64, false>), grid, dim3(64), 0, s, a);
+    if (p.runs) hipLaunchKernelGGL(paged_join_kernel<64>, join, dim3(512), 0, s, a);
+  } else {
+    if (f8) hipLaunchKernelGGL((paged_attn_kernel<128, true>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<128, false>), grid, dim3(64), 0, s, a);
+    if (p.runs) hipLaunchKernelGGL(paged_join_kernel<128>, join, dim3(512), 0, s, a);
+  }
+  return launch_status();
+}

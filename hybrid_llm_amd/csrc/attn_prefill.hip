@@ -37,6 +37,7 @@
 // (r & 3) + 8 (r >> 2) + 4 (l >> 5), column l & 31.
 #include "common.hpp"
 #include "abi_util.hpp"
+#include "attn_tile.hpp"
 
 namespace llmy {
 
@@ -44,49 +45,6 @@ typedef float f32x16v __attribute__((ext_vector_type(16)));
 
 constexpr int kBM = 128;    // queries per workgroup
 constexpr int kBN = 64;     // keys per staged tile
-
-typedef __attribute__((address_space(3))) void lds_void;
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ void dma16(const void* src, void* lds_dst) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void*)lds_dst, 16, 0, 0);
-}
-
-__device__ __forceinline__ uint32_t lds_addr(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void*)p));
-}
-
-// LDS reads as inline asm: with a DMA into the other stage in flight, the
-// compiler would make every LDS read wait for it.  Their results are valid
-// after lds_settle.
-__device__ __forceinline__ u32x4 lds_b128(uint32_t addr) {
-  u32x4 v;
-  asm volatile("ds_read_b128 %0, %1" : "=v"(v) : "v"(addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ u32x2 lds_tr16(uint32_t addr) {
-  u32x2 v;
-  asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(v) : "v"(addr) : "memory");
-  return v;
-}
-
-// Wait for every LDS read of this wave and tie the registers they filled to
-// the wait, so no use is scheduled above it.
-__device__ __forceinline__ void lds_settle4(u32x4* f) {
-  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3])::"memory");
-}
-
-__device__ __forceinline__ void lds_settle_v(u32x2* f) {
-  asm volatile("s_waitcnt lgkmcnt(0)"
-               : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]),
-                 "+v"(f[6]), "+v"(f[7])::"memory");
-}
-
-__device__ __forceinline__ uint4 pack8_bf16(const float* v) {
-  return uint4{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]),
-               pack_bf2(v[6], v[7])};
-}
 
 template <int HD>
 __global__ __launch_bounds__(256) void attn_prefill_kernel(const uint16_t* __restrict__ q,

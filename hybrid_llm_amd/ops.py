@@ -312,6 +312,184 @@ def banded_attn_decode_parts(parts: torch.Tensor, k_off: int, v_off: int, k_cach
     return out
 
 
+# ---------------------------------------------- full-length attention over a paged cache
+CACHE_BF16, CACHE_E4M3 = 0, 1
+_CACHE_TYPES = {torch.bfloat16: CACHE_BF16, torch.float8_e4m3fn: CACHE_E4M3}
+
+
+def _here(*tensors) -> None:
+    """Every tensor is on the current device, whose stream the call uses."""
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors must be on the current device (cuda:{dev}), got {t.device}")
+
+
+def _check_rows(t: torch.Tensor, name: str, shape: tuple, step: int) -> None:
+    """bf16 [N, H, hd] whose heads' dims are contiguous; strides multiples of ``step``."""
+    if t.dtype != torch.bfloat16 or t.shape != shape:
+        raise ValueError(f"{name} must be torch.bfloat16 {tuple(shape)}, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    row, head, one = t.stride()
+    if one != 1 or row % step or head % step:
+        raise ValueError(f"{name}: dims must be contiguous and strides multiples of {step}, got "
+                         f"{t.stride()}")
+
+
+def _check_f32(t: torch.Tensor | None, name: str, n: int) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous torch.float32 [{n}], got {t.dtype} "
+                         f"{tuple(t.shape)}")
+
+
+def _check_i32(t: torch.Tensor | None, name: str, shape: tuple) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous torch.int32 {tuple(shape)}, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+
+
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, hd: int) -> tuple:
+    """(pages, page, cache type) of a [pages, Hkv, page, hd] cache pair."""
+    kind = _CACHE_TYPES.get(k_cache.dtype)
+    if kind is None or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must both be torch.bfloat16 or "
+                         f"torch.float8_e4m3fn, got {k_cache.dtype} and {v_cache.dtype}")
+    if (k_cache.dim() != 4 or k_cache.shape[1] != Hkv or k_cache.shape[3] != hd
+            or v_cache.shape != k_cache.shape):
+        raise ValueError(f"caches must be [pages, {Hkv}, page, {hd}], got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    return k_cache.shape[0], k_cache.shape[2], kind
+
+
+def _half(inv_freq: torch.Tensor | None) -> int:
+    if inv_freq is None:
+        return 0
+    n = inv_freq.numel()
+    _check_f32(inv_freq, "inv_freq", n)
+    return n
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                 inv_freq: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                 interleaved: bool = False, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple:
+    """Per-head RMSNorm (where a norm is given) and position rotation of q [N,Hq,hd] and
+    k [N,Hkv,hd] bf16 in one pass (see llmy_qk_norm_rope_bf16); (q_out, k_out).  Views of a
+    fused projection pass as they are; q_out / k_out may be q / k.  positions [N] int32
+    (negative: a padding row, its outputs left as they were), inv_freq [half] fp32: pairs
+    (i, i + half), interleaved (2i, 2i + 1), of the first 2 half dims; None: no rotation."""
+    N, Hq, hd = q.shape
+    Hkv = k.shape[1]
+    if q_out is None:
+        q_out = torch.empty(N, Hq, hd, dtype=torch.bfloat16, device=q.device)
+    if k_out is None:
+        k_out = torch.empty(N, Hkv, hd, dtype=torch.bfloat16, device=q.device)
+    _here(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
+    for t, name, shape in ((q, "q", (N, Hq, hd)), (k, "k", (N, Hkv, hd)),
+                           (q_out, "q_out", (N, Hq, hd)), (k_out, "k_out", (N, Hkv, hd))):
+        _check_rows(t, name, shape, 4)
+    _check_i32(positions, "positions", (N,))
+    half = _half(inv_freq)
+    _check_f32(q_norm, "q_norm", hd)
+    _check_f32(k_norm, "k_norm", hd)
+    _lib.call("llmy_qk_norm_rope_bf16", _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0),
+              k.stride(1), _ptr(positions), _ptr(inv_freq), half, _ptr(q_norm), _ptr(k_norm),
+              eps, int(interleaved), _ptr(q_out), q_out.stride(0), q_out.stride(1), _ptr(k_out),
+              k_out.stride(0), k_out.stride(1), N, Hq, Hkv, hd, _stream())
+    return q_out, k_out
+
+
+def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor,
+                    rows: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
+                    k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                    interleaved: bool = False, k_scale: float = 1.0, v_scale: float = 1.0,
+                    q: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                    q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Keys (normed and rotated as in qk_norm_rope) and values of N tokens [N,Hkv,hd] into
+    the caches [pages,Hkv,page,hd] (bf16, or e4m3 holding x / scale), in place (see
+    llmy_paged_kv_append).  Token n goes to positions[n] of page_table[rows[n]] (rows None:
+    row n); a token without a valid slot is not stored, and no two tokens of a call may
+    name one slot.  With ``q`` [N,Hq,hd] its rows are normed and rotated in the same pass
+    and returned (q_out)."""
+    N, Hkv, hd = k.shape
+    pages, page, kind = _check_cache(k_cache, v_cache, Hkv, hd)
+    _check_rows(k, "k", (N, Hkv, hd), 4)
+    _check_rows(v, "v", (N, Hkv, hd), 4)
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    B, width = page_table.shape
+    if rows is None and N > B:
+        raise ValueError(f"{N} tokens and {B} page-table rows: name each token's row")
+    _check_i32(page_table, "page_table", (B, width))
+    _check_i32(positions, "positions", (N,))
+    _check_i32(rows, "rows", (N,))
+    half = _half(inv_freq)
+    _check_f32(k_norm, "k_norm", hd)
+    Hq, qs, qo = 0, (0, 0), (0, 0)
+    if q is not None:
+        Hq = q.shape[1]
+        _check_rows(q, "q", (N, Hq, hd), 4)
+        _check_f32(q_norm, "q_norm", hd)
+        if q_out is None:
+            q_out = torch.empty(N, Hq, hd, dtype=torch.bfloat16, device=q.device)
+        _check_rows(q_out, "q_out", (N, Hq, hd), 4)
+        qs, qo = q.stride(), q_out.stride()
+    elif q_norm is not None or q_out is not None:
+        raise ValueError("q_norm and q_out go with q")
+    _here(k, v, k_cache, v_cache, page_table, positions, rows, inv_freq, k_norm, q, q_norm, q_out)
+    _lib.call("llmy_paged_kv_append", _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
+              v.stride(1), _ptr(k_cache), _ptr(v_cache), kind, k_scale, v_scale,
+              _ptr(page_table), _ptr(rows), _ptr(positions), _ptr(inv_freq), half, _ptr(k_norm),
+              eps, int(interleaved), _ptr(q), qs[0], qs[1], _ptr(q_norm), _ptr(q_out), qo[0],
+              qo[1], N, Hq, Hkv, hd, B, width, page, pages, _stream())
+    return q_out
+
+
+def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      page_table: torch.Tensor, lengths: torch.Tensor,
+                      scale: float | None = None, window: int = 0, softcap: float = 0.0,
+                      slopes: torch.Tensor | None = None, k_scale: float = 1.0,
+                      v_scale: float = 1.0, out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """One new token per sequence, q [B,Hq,hd] bf16, over the first lengths[b] (int32)
+    positions of page_table[b] in the caches [pages,Hkv,page,hd] (see
+    llmy_paged_attn_decode): scores scale q.k, capped to softcap tanh(z / softcap), less
+    slopes[h] (fp32 [Hq]) a position of distance, over the last ``window`` positions (0:
+    all).  Returns out [B,Hq,hd] bf16, zeros where nothing is visible.  ``workspace``: a
+    buffer of llmy_paged_attn_workspace_bytes that no overlapping call uses."""
+    B, Hq, hd = q.shape
+    Hkv = k_cache.shape[1]
+    pages, page, kind = _check_cache(k_cache, v_cache, Hkv, hd)
+    _check_rows(q, "q", (B, Hq, hd), 8)
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    width = page_table.shape[1]
+    _check_i32(page_table, "page_table", (B, width))
+    _check_i32(lengths, "lengths", (B,))
+    _check_f32(slopes, "slopes", Hq)
+    if out is None:
+        out = torch.empty(B, Hq, hd, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous torch.bfloat16 {tuple(q.shape)}")
+    nbytes = int(_lib.load().llmy_paged_attn_workspace_bytes(B, Hq, Hkv, hd, width, page, kind))
+    if nbytes > 0 and workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if have < nbytes:
+        raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
+    _here(q, k_cache, v_cache, page_table, lengths, slopes, out, workspace)
+    scale = hd ** -0.5 if scale is None else scale
+    _lib.call("llmy_paged_attn_decode", _ptr(q), q.stride(0), q.stride(1), _ptr(k_cache),
+              _ptr(v_cache), kind, k_scale, v_scale, _ptr(page_table), _ptr(lengths),
+              _ptr(slopes), _ptr(out), _ptr(workspace), have, B, Hq, Hkv, hd, width, page, pages,
+              window, scale, softcap, _stream())
+    return out
+
+
 # --------------------------------------------------------------------------- GDN
 def _reset_arg(reset, shape, dev):
     """A reset mask as the device int32 array the kernels read (nonzero = reset)."""

@@ -177,6 +177,79 @@ int32_t llmy_banded_attn_decode_parts_bf16(const float* parts, int32_t nparts,
                                            int32_t head_dim, int32_t W, float scale,
                                            void* stream);
 
+/* --- Full-length attention: rotated rows, a paged cache, packed prompts -----------
+ * No counterpart in the reference, whose attention is banded, unrotated, one
+ * key-value head per query head: what a model with full-length grouped attention
+ * runs beside it.  Query head h reads key-value head h / (Hq / Hkv); Hq % Hkv == 0,
+ * at most 1024 heads, head_dim 64 or 128.  q, k and v rows are strided views (row
+ * and head strides in elements, the dims of a head contiguous), so the slices of one
+ * fused projection pass as they are.
+ *
+ * A paged cache is [pages, Hkv, page, head_dim], page 16, 32, 64, 128 or 256 tokens;
+ * position p of a sequence is slot p % page of page page_table[row][p / page]
+ * (page_table [B, width] int32).  cache_type 0: bf16; 1: OCP e4m3, standing for the
+ * value times k_scale or v_scale (> 0; both 1 for bf16).  Page ids outside [0, pages) name no page. */
+
+/* Per-head RMSNorm and position rotation of q [N, Hq, head_dim] and k [N, Hkv,
+ * head_dim] in one pass: y = x rsqrt(mean(x^2) + eps) norm (q_norm / k_norm [head_dim]
+ * fp32, NULL: no norm), then for the pairs (i, i + half) -- interleaved: (2i, 2i + 1) --
+ * of the first 2 half dims (y_a cos t - y_b sin t, y_b cos t + y_a sin t) with
+ * t = positions[n] * inv_freq[i] (fp32 [half]; the product in 64 bits), rounded once.
+ * half % 4 == 0, 2 half <= head_dim; half 0: norm only.  A row of negative position is
+ * padding: its outputs stay as they were.  Outputs may be the inputs themselves (same
+ * pointer and strides).  Rows 8-byte aligned, strides multiples of 4, norms 16-byte
+ * aligned. */
+int32_t llmy_qk_norm_rope_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head,
+                               const llmy_bf16* k, int64_t k_row, int64_t k_head,
+                               const int32_t* positions, const float* inv_freq, int32_t half,
+                               const float* q_norm, const float* k_norm, float eps,
+                               int32_t interleaved, llmy_bf16* q_out, int64_t qo_row,
+                               int64_t qo_head, llmy_bf16* k_out, int64_t ko_row,
+                               int64_t ko_head, int32_t N, int32_t Hq, int32_t Hkv,
+                               int32_t head_dim, void* stream);
+
+/* Appends N tokens' keys (normed and rotated as above) and values (as they are) to a
+ * paged cache: token n goes to position positions[n] of page-table row rows[n] (NULL:
+ * row n).  A token whose position is negative or past width * page, whose row is
+ * outside [0, B) or whose page is named by no entry is not stored.  e4m3 stores
+ * x / scale, saturated at 448, to nearest even.  Two tokens of one call must not name
+ * one slot.  With Hq > 0 the tokens' queries are normed and rotated in the same pass
+ * into q_out (negative positions: left as they were); q, q_norm, q_out NULL with
+ * Hq 0. */
+int32_t llmy_paged_kv_append(const llmy_bf16* k, int64_t k_row, int64_t k_head,
+                             const llmy_bf16* v, int64_t v_row, int64_t v_head, void* k_cache,
+                             void* v_cache, int32_t cache_type, float k_scale, float v_scale,
+                             const int32_t* page_table, const int32_t* rows,
+                             const int32_t* positions, const float* inv_freq, int32_t half,
+                             const float* k_norm, float eps, int32_t interleaved,
+                             const llmy_bf16* q, int64_t q_row, int64_t q_head,
+                             const float* q_norm, llmy_bf16* q_out, int64_t qo_row,
+                             int64_t qo_head, int32_t N, int32_t Hq, int32_t Hkv,
+                             int32_t head_dim, int32_t B, int32_t width, int32_t page,
+                             int32_t pages, void* stream);
+
+/* Workspace (bytes) of llmy_paged_attn_decode for these sizes; -1 where that call
+ * refuses them, 0 where it takes none.  No two calls that may overlap share one. */
+int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                                        int32_t width, int32_t page, int32_t cache_type);
+
+/* One query per sequence, q [B, Hq, head_dim] (strides in elements, multiples of 8, 16-byte
+ * aligned), over the first len = lengths[b] positions of its page-table row:
+ *   z_j = scale q . k_j; softcap c > 0: c tanh(z_j / c); slopes [Hq] or NULL:
+ *   z_j -= slopes[h] (len - 1 - j); out = sum_j softmax(z)_j v_j
+ * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
+ * zeros where there is none.  Lengths below 0 count as 0, past width * page as that.
+ * What the other slots of a page hold, NaN included, has no effect.  out [B, Hq,
+ * head_dim] bf16.  fp32 scores and sums; weights rounded to bf16 for their product. */
+int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head,
+                               const void* k_cache, const void* v_cache, int32_t cache_type,
+                               float k_scale, float v_scale, const int32_t* page_table,
+                               const int32_t* lengths, const float* slopes, llmy_bf16* out,
+                               void* workspace, int64_t workspace_bytes, int32_t B, int32_t Hq,
+                               int32_t Hkv, int32_t head_dim, int32_t width, int32_t page,
+                               int32_t pages, int32_t window, float scale, float softcap,
+                               void* stream);
+
 /* --- Gated delta rule, prefill (chunked; model/layers/gated_deltanet.py:140-149) */
 
 /* Workspace (bytes) that llmy_gdn_prefill_bf16 needs for (B, T, H, dk, dv):
