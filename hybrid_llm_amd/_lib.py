@@ -47,6 +47,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "llmy_paged_attn_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
     "llmy_paged_attn_decode": (_I, [_P, _I64, _I64, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P, _I64,
                                     _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "llmy_packed_attn_prefill_bf16": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P,
+                                           _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
     "llmy_gdn_prefill_workspace_bytes": (C.c_int64, [_I, _I, _I, _I, _I]),
     "llmy_gdn_prefill_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _P]),
     "llmy_gdn_prefill_bf16_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),

@@ -564,7 +564,7 @@ extern "C" int32_t llmy_paged_attn_decode(
     int32_t page, int32_t pages, int32_t window, float scale, float softcap, void* stream) {
   PagedPlan p;
   LLMY_REQUIRE(paged_plan(B, Hq, Hkv, head_dim, width, page, cache_type, &p));
-  LLMY_REQUIRE(pages >= 0 && window >= 0 && softcap >= 0.f &&
+  LLMY_REQUIRE(pages >= 0 && window >= 0 && scale >= 0.f && softcap >= 0.f &&
                scales_ok(cache_type, k_scale, v_scale));
   if (B == 0) return 0;
   LLMY_REQUIRE(q && out && lengths && aligned(q, 16) && aligned(out, 16));

@@ -490,6 +490,41 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
+def packed_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        cu_seqlens: torch.Tensor, scale: float | None = None, window: int = 0,
+                        softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                        prefix: torch.Tensor | None = None, out: torch.Tensor | None = None
+                        ) -> torch.Tensor:
+    """Causal attention within each of the packed documents whose rows cu_seqlens (int32
+    [docs + 1]) bounds: q [N,Hq,hd], k, v [N,Hkv,hd] bf16 (see
+    llmy_packed_attn_prefill_bf16).  ``window``: the last so many rows (0: all);
+    ``softcap`` and ``slopes`` (fp32 [Hq], a row of distance) as in paged_attn_decode;
+    ``prefix`` (int32 [docs]): every row of a document also sees its first so many rows.
+    Returns out [N,Hq,hd] bf16; rows of no document are left as they were."""
+    N, Hq, hd = q.shape
+    Hkv = k.shape[1]
+    _check_rows(q, "q", (N, Hq, hd), 8)
+    _check_rows(k, "k", (N, Hkv, hd), 8)
+    _check_rows(v, "v", (N, Hkv, hd), 8)
+    docs = cu_seqlens.numel() - 1
+    if docs < 0:
+        raise ValueError("cu_seqlens must hold at least one entry")
+    _check_i32(cu_seqlens, "cu_seqlens", (docs + 1,))
+    _check_i32(prefix, "prefix", (docs,))
+    _check_f32(slopes, "slopes", Hq)
+    if out is None:
+        out = torch.empty(N, Hq, hd, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous torch.bfloat16 {tuple(q.shape)}")
+    _here(q, k, v, cu_seqlens, prefix, slopes, out)
+    scale = hd ** -0.5 if scale is None else scale
+    _lib.call("llmy_packed_attn_prefill_bf16", _ptr(q), q.stride(0), q.stride(1), _ptr(k),
+              k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(cu_seqlens),
+              _ptr(prefix), _ptr(slopes), _ptr(out), N, docs, Hq, Hkv, hd, window, scale, softcap,
+              _stream())
+    return out
+
+
 # --------------------------------------------------------------------------- GDN
 def _reset_arg(reset, shape, dev):
     """A reset mask as the device int32 array the kernels read (nonzero = reset)."""

@@ -240,7 +240,8 @@ int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int3
  * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
  * zeros where there is none.  Lengths below 0 count as 0, past width * page as that.
  * What the other slots of a page hold, NaN included, has no effect.  out [B, Hq,
- * head_dim] bf16.  fp32 scores and sums; weights rounded to bf16 for their product. */
+ * head_dim] bf16.  scale >= 0.  fp32 scores and sums; weights rounded to bf16 for their
+ * product. */
 int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                const void* k_cache, const void* v_cache, int32_t cache_type,
                                float k_scale, float v_scale, const int32_t* page_table,
@@ -249,6 +250,23 @@ int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head
                                int32_t Hkv, int32_t head_dim, int32_t width, int32_t page,
                                int32_t pages, int32_t window, float scale, float softcap,
                                void* stream);
+
+/* Attention over N packed rows of `docs` documents: rows cu_seqlens[d] .. cu_seqlens[d + 1]
+ * (device int32 [docs + 1], ascending) are document d.  Row i of a document that starts
+ * at a sees its rows j <= i with i - j < window (0: all) and, with prefix [docs] (int32 or
+ * NULL), the rows j < a + prefix[d] before and after it (under the window only those
+ * with i - j < window).  Scores as in llmy_paged_attn_decode with slopes[h] |i - j|.
+ * q [N, Hq, head_dim], k, v [N, Hkv, head_dim] strided rows (strides multiples of 8,
+ * 16-byte aligned, k and v rows under 2^22 apart); out [N, Hq, head_dim] bf16, which
+ * must not overlap k or v.  Rows of no document stay as they were, and what they or
+ * other unseen rows hold, NaN included, has no effect.  scale >= 0. */
+int32_t llmy_packed_attn_prefill_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head,
+                                      const llmy_bf16* k, int64_t k_row, int64_t k_head,
+                                      const llmy_bf16* v, int64_t v_row, int64_t v_head,
+                                      const int32_t* cu_seqlens, const int32_t* prefix,
+                                      const float* slopes, llmy_bf16* out, int32_t N,
+                                      int32_t docs, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                                      int32_t window, float scale, float softcap, void* stream);
 
 /* --- Gated delta rule, prefill (chunked; model/layers/gated_deltanet.py:140-149) */
 

@@ -18,6 +18,10 @@ DECODE = dict(q=FAKE, q_row=512, q_head=64, kc=FAKE, vc=FAKE, kind=0, ks=1.0, vs
               lens=FAKE, slopes=None, out=FAKE, ws=FAKE, ws_bytes=1 << 30, B=4, Hq=8, Hkv=4,
               hd=64, width=30, page=16, pages=12, window=0, scale=0.125, cap=0.0, stream=None)
 
+PACKED = dict(q=FAKE, q_row=512, q_head=64, k=1 << 20, k_row=256, k_head=64, v=1 << 21, v_row=256,
+              v_head=64, cu=FAKE, prefix=None, slopes=None, out=1 << 22, N=100, docs=3, Hq=8,
+              Hkv=4, hd=64, window=0, scale=0.125, cap=0.0, stream=None)
+
 
 def _call(fn, base, **change):
     return fn(*{**base, **change}.values())
@@ -57,7 +61,7 @@ def test_append_of_no_tokens(lib):
     {"hd": 96}, {"Hq": 6}, {"Hkv": 0}, {"Hq": 0}, {"B": -1}, {"page": 17}, {"width": -1},
     {"pages": -1}, {"window": -1}, {"cap": -1.0}, {"cap": math.nan}, {"kind": 5}, {"vs": 2.0},
     {"kind": 1, "ks": math.nan}, {"q": None}, {"out": None}, {"lens": None}, {"table": None},
-    {"kc": None}, {"vc": FAKE + 4}, {"q": FAKE + 8}, {"q_row": 516}, {"q_head": 68},
+    {"kc": None}, {"scale": -0.1}, {"scale": math.nan}, {"vc": FAKE + 4}, {"q": FAKE + 8}, {"q_row": 516}, {"q_head": 68},
     {"out": FAKE + 8}, {"ws": None}, {"ws": FAKE + 8}, {"ws_bytes": 64},
     {"width": 1 << 27, "page": 16},
 ])
@@ -67,6 +71,22 @@ def test_decode_refuses(lib, change):
 
 def test_decode_of_no_sequences(lib):
     assert _call(lib.llmy_paged_attn_decode, DECODE, B=0, q=None, ws=None) == 0
+
+
+@pytest.mark.parametrize("change", [
+    {"hd": 80}, {"Hq": 6}, {"Hkv": 0}, {"Hq": 2048}, {"N": -1}, {"N": 1 << 30}, {"docs": -1},
+    {"window": -1}, {"scale": -1.0}, {"scale": math.nan}, {"cap": -0.5}, {"q": None}, {"k": None},
+    {"v": None}, {"out": None}, {"cu": None}, {"q": FAKE + 8}, {"out": (1 << 22) + 8},
+    {"k_row": 260}, {"v_head": 4}, {"q_row": -512}, {"k_row": 1 << 22},
+    {"out": 1 << 20}, {"out": (1 << 20) + 99 * 512 + 496}, {"out": (1 << 21) - 16},
+])
+def test_prefill_refuses(lib, change):
+    assert _call(lib.llmy_packed_attn_prefill_bf16, PACKED, **change) == INVALID
+
+
+def test_prefill_of_nothing(lib):
+    assert _call(lib.llmy_packed_attn_prefill_bf16, PACKED, N=0, q=None) == 0
+    assert _call(lib.llmy_packed_attn_prefill_bf16, PACKED, docs=0, cu=None) == 0
 
 
 def test_workspace_sizes(lib):
@@ -102,3 +122,10 @@ def test_wrappers_refuse_before_the_library():
         args = {**dict(q=q, k_cache=cache, v_cache=cache, page_table=table, lengths=pos), **bad}
         with pytest.raises(ValueError):
             ops.paged_attn_decode(**args)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    for bad in (dict(q=q.half()), dict(v=k[:3]), dict(cu_seqlens=cu.long()), dict(cu_seqlens=cu[:0]),
+                dict(prefix=pos), dict(slopes=freq), dict(out=q.transpose(0, 1)),
+                dict(k=k[..., :32])):
+        args = {**dict(q=q, k=k, v=k, cu_seqlens=cu), **bad}
+        with pytest.raises(ValueError):
+            ops.packed_attn_prefill(**args)
