@@ -125,14 +125,6 @@ __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ void lds_settle2(u32x4* f) {
-  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1])::"memory");
-}
-
-__device__ __forceinline__ void lds_settle_v4(u32x2* f) {
-  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3])::"memory");
-}
-
 // 8 e4m3 codes as bf16 (exact).
 __device__ __forceinline__ bf16x8 e4m3_to_bf16(uint32_t lo, uint32_t hi) {
   uint4 r;
@@ -223,6 +215,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     kdo[j] = (lane / T::CH) * RB + 16 * (sl ^ T::kswz(r));
     vdo[j] = (lane / T::CH) * RB + 16 * (sl ^ T::vswz(r));
   }
+  const uint32_t sbase = lds_addr(smem);
   unsigned bad = 0;  // two bits a stage: its 16-key tiles whose page the table does not name
   int ib = b, iu = u, is = s;
   Seq icur = cur;
@@ -241,7 +234,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     const long long row = static_cast<long long>(ib) * a.width;
     const int key0 = is * kStep;
     const int last = (icur.len - 1) >> a.shift;  // keys past the length stay in its page
-    uint8_t* sk = smem + st * 2 * T::BYTES;
+    const uint32_t dst = sbase + st * 2 * T::BYTES;
     bad &= ~(3u << (2 * st));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -255,14 +248,13 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
 #pragma unroll
       for (int j = 0; j < NB / 2; ++j) {
         const int blk = h * (NB / 2) + j;
-        dma16(kp + j * 1024 + kdo[blk], sk + blk * 1024);
-        dma16(vp + j * 1024 + vdo[blk], sk + T::BYTES + blk * 1024);
+        lds_fill16(kp + j * 1024, kdo[blk], dst + blk * 1024);
+        lds_fill16(vp + j * 1024, vdo[blk], dst + T::BYTES + blk * 1024);
       }
     }
   };
 
   // fragment offsets (bytes from a stage's K or V tile)
-  const uint32_t sbase = lds_addr(smem);
   uint32_t koff[NK], voff[ND];
 #pragma unroll
   for (int t = 0; t < NK; ++t) koff[t] = col * RB + 16 * ((4 * t + g) ^ T::kswz(col));
@@ -318,7 +310,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int t = 0; t < NK; ++t) kf[k * NK + t] = lds_b128(kst + 16 * k * RB + koff[t]);
+      for (int t = 0; t < NK; ++t) kf[k * NK + t] = lds_get16(kst + 16 * k * RB + koff[t]);
     if (edge) {  // masked keys' V rows are zeroed
       for (int e = lane; e < kStep * T::CH; e += 64) {
         const int row = e / T::CH, key = key0 + row;
@@ -328,19 +320,15 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
       }
       wave_lds_order();
     }
-    if constexpr (NK == 1) lds_settle2(kf);
-    else
-#pragma unroll
-      for (int t = 0; t < 2 * NK; t += 4) lds_settle4(kf + t);
     constexpr int NV = F8 ? ND : 2 * ND;
     u32x2 vf[NV];
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       if (F8) {
-        vf[d] = lds_tr8(vst + voff[d]);
+        vf[d] = lds_get_tr8(vst + voff[d]);
       } else {
-        vf[2 * d] = lds_tr16(vst + voff[d]);
-        vf[2 * d + 1] = lds_tr16(vst + voff[d] + 16 * RB);
+        vf[2 * d] = lds_get_tr16(vst + voff[d]);
+        vf[2 * d + 1] = lds_get_tr16(vst + voff[d] + 16 * RB);
       }
     }
     f32x4 sc[2];
@@ -391,10 +379,6 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     unpack8(pb, p);
 #pragma unroll
     for (int j = 0; j < 8; ++j) l_run += p[j];
-    if constexpr (NV == 4) lds_settle_v4(vf);
-    else
-#pragma unroll
-      for (int v = 0; v < NV; v += 8) lds_settle_v(vf + v);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const bf16x8 vv = F8 ? e4m3_to_bf16(vf[d].x, vf[d].y)
@@ -402,7 +386,8 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
                                              vf[F8 ? 0 : 2 * d + 1].x, vf[F8 ? 0 : 2 * d + 1].y});
       acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pb), acc[d], 0, 0, 0);
     }
-    // every read of this stage has returned: the next step may land in it
+    // once every read of this stage has returned, the next step may land in it
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (issued < count) {
       next(ib, iu, is, icur);
       issue(st);

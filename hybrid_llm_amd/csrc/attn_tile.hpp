@@ -33,14 +33,6 @@ __device__ __forceinline__ u32x2 lds_tr16(uint32_t addr) {
   return v;
 }
 
-// Lane 16 g + y addresses 8 bytes, half y & 1 of row y / 2 of a 16-lane group's 8 x 16
-// bytes, and receives column y of the 8 rows.
-__device__ __forceinline__ u32x2 lds_tr8(uint32_t addr) {
-  u32x2 v;
-  asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(v) : "v"(addr) : "memory");
-  return v;
-}
-
 // Wait for every LDS read of this wave and tie the registers they filled to
 // the wait, so no use is scheduled above it.
 __device__ __forceinline__ void lds_settle4(u32x4* f) {
@@ -51,6 +43,44 @@ __device__ __forceinline__ void lds_settle_v(u32x2* f) {
   asm volatile("s_waitcnt lgkmcnt(0)"
                : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]),
                  "+v"(f[6]), "+v"(f[7])::"memory");
+}
+
+// The same copy as a statement the compiler knows nothing of but its memory clobber, so
+// that LDS reads need not wait for copies into other stages; the kernel waits for its
+// copies (vmcnt) itself.  base is the same for every lane, off a lane's bytes from it,
+// dst the wave's LDS byte address.  s_nop 3 after the move of m0 makes the five wait
+// states that the load needs after a VALU write of an SGPR that it reads.  m0 is
+// reserved (hence a warning), but the compiler keeps values there for its own use:
+// the clobber says that they are gone.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void lds_fill16(const void* base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
+               ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// LDS reads at a byte address, for kernels that fill LDS by lds_fill16: the compiler
+// waits for each result where it is used.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ u32x4 lds_get16(uint32_t addr) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(addr);
+}
+
+// In each 16-lane group lane y addresses 8 bytes, 4 columns 4 (y & 3) .. of row y / 4, and
+// receives column y of the 4 rows.
+__device__ __forceinline__ u32x2 lds_get_tr16(uint32_t addr) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      reinterpret_cast<__attribute__((address_space(3))) s16x4*>(addr)));
+}
+
+// Lane y of a group addresses 8 bytes, half y & 1 of row y / 2 of 8 rows of 16 bytes, and
+// receives column y of the 8 rows.
+__device__ __forceinline__ u32x2 lds_get_tr8(uint32_t addr) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      reinterpret_cast<__attribute__((address_space(3))) i32x2*>(addr)));
 }
 
 __device__ __forceinline__ uint4 pack8_bf16(const float* v) {
