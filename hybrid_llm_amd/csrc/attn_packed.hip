@@ -6,16 +6,24 @@
 // key-value head h / (Hq / Hkv).
 //
 // Matrix work in the transposed form of attn_prefill.hip (S^T = K Q^T, O^T = V^T P^T on
-// v_mfma_f32_32x32x16_bf16, P never leaves its registers, K and V by DMA into two
-// swizzled LDS stages): a workgroup owns 128 consecutive rows of one head, whatever
-// documents they belong to, and walks the 64-key tiles that any of its rows sees; a
-// wave skips 32-key sub-tiles that none of its 32 rows sees and masks only those that
-// some of its rows see and some do not.
-// What a masked place holds, NaN and infinities included, must reach no row, and 0 * inf
-// is NaN in the product: such values are zeroed in the fragments of a sub-tile that
-// some row does not see in full, and the rows that do see them get them at the end.
+// v_mfma_f32_32x32x16_bf16, P never leaves its registers, K and V copied into two
+// swizzled LDS stages): a wave owns 32 consecutive rows of one head, whatever documents
+// they belong to, and takes 32 keys at a time; it skips those that none of its rows
+// sees and masks only those that some of its rows see and some do not.
+//   * Many rows: the four waves of a workgroup own 128 rows and share 64-key tiles.  A
+//     sub-tile is 82 vector instructions beside its 16 (128-wide heads) or 8 matrix
+//     ones, and two or four waves a SIMD run the one kind under the other's.
+//   * Few rows (less than a workgroup a CU): the four waves own the same 32 rows and
+//     take a quarter of each 128-key tile each; their sums are joined in LDS.  The
+//     longest chain is a quarter as long and there are four times the workgroups.
 // Blocks run from the last rows to the first, the longest ones of a document first,
 // heads fastest: with 8 or 16 heads a head's blocks share an XCD's L2.
+//
+// What a masked place holds, NaN and infinities included, must reach no row, and 0 * inf
+// is NaN in the product.  The values are not looked at as they pass (96 instructions a
+// masked sub-tile): a workgroup that ends with an output that is not finite runs once
+// more, with such values zeroed in masked sub-tiles and given to the rows that do see
+// them at the end.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "attn_tile.hpp"
@@ -25,8 +33,7 @@ namespace llmy {
 
 typedef float f32x16v __attribute__((ext_vector_type(16)));
 
-constexpr int kPM = 128;  // rows per workgroup
-constexpr int kPN = 64;   // keys per staged tile
+constexpr int kDocsInLds = 511;
 
 struct PackedArgs {
   const uint16_t *q, *k, *v;
@@ -62,44 +69,55 @@ struct Int {
   static constexpr int value = V;
 };
 
-// SCORE: scores are capped or biased (otherwise the scale goes into the exponent).
-template <int HD, bool SCORE>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(const PackedArgs a) {
-  constexpr int ND = HD / 32;   // 32-dim output tiles
-  constexpr int NS = HD / 16;   // 16-dim slices of the score product
-  constexpr int RB = 2 * HD;    // bytes of a staged row
-  constexpr int TB = kPN * RB;  // bytes of a staged K or V tile
+enum { kPlain = 0, kCapped = 1, kBiased = 2 };  // kBiased: a distance bias, a cap or not
+
+// KW: waves along the keys (1 or 4); 4 / KW waves along the rows.
+template <int HD, int MODE, int KW>
+__global__ __launch_bounds__(256, HD == 64 && KW == 1 ? 4 : HD == 64 || KW == 1 ? 2 : 1)
+void packed_attn_kernel(const PackedArgs a) {
+  constexpr int ND = HD / 32;             // 32-dim output tiles
+  constexpr int NS = HD / 16;             // 16-dim slices of the score product
+  constexpr int RB = 2 * HD;              // bytes of a staged row
+  constexpr int PM = 128 / KW;            // rows per workgroup
+  constexpr int PN = KW == 1 ? 64 : 128;  // keys per staged tile
+  constexpr int TB = PN * RB;             // bytes of a staged K or V tile
   __shared__ __align__(1024) uint8_t smem[2 * 2 * TB];
   __shared__ int range[2][4];
+  __shared__ int cu_s[kDocsInLds + 1];
 
-  const int nblk = (a.N + kPM - 1) / kPM;
+  const int nblk = (a.N + PM - 1) / PM;
   const int h = blockIdx.x % a.hq;
-  const int q0 = (nblk - 1 - static_cast<int>(blockIdx.x / a.hq)) * kPM;
+  const int q0 = (nblk - 1 - static_cast<int>(blockIdx.x / a.hq)) * PM;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5;
   const int col = lane & 31;
-  const int qi = q0 + 32 * wave + col;  // this lane's row
+  const int qi = q0 + (KW == 1 ? 32 * wave : 0) + col;  // this lane's row
 
-  // its document by bisection, its keys [lo, lo + n); none for a row of no document
+  // its document by bisection (few documents: in LDS, one load's latency instead of a
+  // chain), its keys [lo, hi); none for a row of no document
+  const bool few = a.docs <= kDocsInLds;
+  if (few)
+    for (int i = threadIdx.x; i <= a.docs; i += 256) cu_s[i] = a.cu[i];
+  __syncthreads();
+  auto cu = [&](int i) { return few ? cu_s[i] : a.cu[i]; };
   int lo = 0, hi = 0;
   bool mine = false;
   if (qi < a.N) {
     int b = 0, e = a.docs + 1;  // the first entry past qi
     while (b < e) {
       const int mid = (b + e) >> 1;
-      if (a.cu[mid] <= qi) b = mid + 1;
+      if (cu(mid) <= qi) b = mid + 1;
       else e = mid;
     }
     if (b > 0 && b <= a.docs) {
-      const int first = max(a.cu[b - 1], 0), end = min(a.cu[b], a.N);
+      const int first = max(cu(b - 1), 0), end = min(cu(b), a.N);
       const int two_way = a.prefix ? min(max(a.prefix[b - 1], 0), end - first) : 0;
       mine = true;
       lo = a.window > 0 ? max(first, qi - min(a.window - 1, qi)) : first;
       hi = max(qi + 1, first + two_way);
     }
   }
-  const unsigned n = hi - lo;
   // the wave's rows see keys in [wlo, whi), all of them those in [ilo, ihi)
   const int big = 0x7fffffff;
   const int wlo = wave_min_i(mine ? lo : big), whi = wave_max_i(mine ? hi : 0);
@@ -112,8 +130,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
   const int glo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
   const int ghi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
   if (ghi <= 0) return;  // no row of any document
-  const int t_lo = __builtin_amdgcn_readfirstlane(glo / kPN);
-  const int t_hi = __builtin_amdgcn_readfirstlane((ghi - 1) / kPN);
+  const int t_lo = __builtin_amdgcn_readfirstlane(glo / PN);
+  const int t_hi = __builtin_amdgcn_readfirstlane((ghi - 1) / PN);
 
   u32x4 qf[NS];
   {
@@ -121,22 +139,17 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
 #pragma unroll
     for (int t = 0; t < NS; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + 16 * t);
   }
-  float slope = 0.f;
-  if (SCORE && a.slopes) slope = a.slopes[h] * 1.4426950408889634f;
-  const float sc = SCORE ? 1.f : a.scale_log2;
+  const float slope =
+      MODE == kBiased && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
 
   f32x16v acc[ND];
-  float m = -1e38f, l = 0.f;  // the exponent's offset (scaled, log2) and the sum of weights
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  float m, l;  // the exponent's offset (scaled, log2) and the sum of weights
 
   // DMA: 1 KiB blocks j = wave + 4 i of RPB rows; lane p fills row RPB j + p / CH, chunk
   // slot p % CH.  Rows past the last re-read it (no row sees them).
   constexpr int CH = HD / 8;
   constexpr int RPB = 64 / CH;
-  constexpr int BPW = kPN / RPB / 4;
+  constexpr int BPW = PN / RPB / 4;
   const uint16_t* kb = a.k + (h / a.G) * a.kh;
   const uint16_t* vb = a.v + (h / a.G) * a.vh;
   const int kr = static_cast<int>(a.kr), vr = static_cast<int>(a.vr);
@@ -149,11 +162,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
   }
   const uint32_t sbase = lds_addr(smem);
   auto issue = [&](int tile, int st) __attribute__((always_inline)) {
-    const int kt = tile * kPN;
+    const int kt = tile * PN;
     const uint32_t dst = sbase + st * 2 * TB + wave * 1024;
     const uint16_t* kp = kb + kt * a.kr;
     const uint16_t* vp = vb + kt * a.vr;
-    if (kt + kPN <= a.N) {
+    if (kt + PN <= a.N) {
 #pragma unroll
       for (int i = 0; i < BPW; ++i) {
         lds_fill16(kp, kdo[i], dst + 4096 * i);
@@ -183,10 +196,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
       va[d] = sbase + TB + (4 * half + i) * RB + 16 * ((dim0 >> 3) ^ (2 * i)) + 2 * (dim0 & 7);
     }
   }
-  bool dirty = false;
-  auto sub_tile = [&](auto subc, int tile, uint32_t off) __attribute__((always_inline)) {
+  bool careful = false;  // the second run: see the top
+  auto sub_tile = [&](auto subc, int ks, uint32_t off) __attribute__((always_inline)) {
     constexpr int S = decltype(subc)::value * 32 * RB;
-    const int ks = tile * kPN + 32 * decltype(subc)::value;
     if (ks >= whi || ks + 32 <= wlo) return;  // no row of this wave sees it
     f32x16v s;
 #pragma unroll
@@ -207,35 +219,29 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
         for (int e = 0; e < 2; ++e)
           vf[sl][d][e] =
               lds_get_tr16(va[d & 1] + off + (S + (16 * sl + 8 * e) * RB + 128 * (d >> 1)));
-    // register r holds key ks + (r & 3) + 8 (r >> 2) + 4 half
-    const int k0 = ks + 4 * half;
-    if (SCORE) {
-      const float dq = static_cast<float>(qi - k0);
+    // register r holds key ks + 4 half + c(r), c(r) = (r & 3) + 8 (r >> 2)
+    const bool whole = ks >= ilo && ks + 32 <= ihi;
+    if (MODE == kBiased) {
+      const float dq = static_cast<float>(qi - ks - 4 * half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float c = (r & 3) + 8 * (r >> 2);
-        float z = a.cap_x2 > 0.f ? softcap_log2(s[r] * a.cap_x2, a.cap_log2)
-                                 : s[r] * a.scale_log2;
-        if (a.slopes) z = fmaf(-slope, fabsf(dq - c), z);
-        s[r] = z;
+        const float z = a.cap_x2 > 0.f ? softcap_log2(s[r] * a.cap_x2, a.cap_log2)
+                                       : s[r] * a.scale_log2;
+        s[r] = fmaf(-slope, fabsf(dq - c), z);
       }
     }
-    const bool whole = ks >= ilo && ks + 32 <= ihi;
+    uint32_t seen = 0xffffffffu;  // bit c(r): this lane's row sees the key
     if (!whole) {
+      const uint64_t one = 1;
+      seen = static_cast<uint32_t>((one << min(max(hi - ks, 0), 32)) -
+                                   (one << min(max(lo - ks, 0), 32))) >> (4 * half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int cr = (r & 3) + 8 * (r >> 2);
-        s[r] = static_cast<unsigned>(k0 + cr - lo) < n ? s[r] : -INFINITY;
+        const uint32_t v = __builtin_amdgcn_sbfe(seen, (r & 3) + 8 * (r >> 2), 1);
+        s[r] = __uint_as_float((v & __float_as_uint(s[r])) | (~v & 0xff800000u));  // else -inf
       }
-      // values that are not finite are left out here; the rows that see them get them
-      // after the last tile
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 4 * ND; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) top |= ((&vf[0][0][0])[i][e] & 0x7f807f80u) + 0x00800080u;
-      if (__ballot((top & 0x80008000u) != 0)) {
-        dirty = true;
+      if (careful) {
 #pragma unroll
         for (int i = 0; i < 4 * ND; ++i)
 #pragma unroll
@@ -251,10 +257,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
           __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
       x = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     }
+    // the cap ascends, so the largest score is the largest capped one
+    if (MODE == kPlain) x *= a.scale_log2;
+    if (MODE == kCapped)
+      x = x == -INFINITY ? x : softcap_log2(x * a.cap_x2, a.cap_log2);
     // the offset moves when some row's largest score passes it by 8 (log2), decided by
     // the wave, so most sub-tiles rescale nothing
-    if (__ballot(fmaf(x, sc, -8.f) > m)) {
-      const float m_new = fmaxf(m, x * sc);
+    if (__ballot(x - 8.f > m)) {
+      const float m_new = fmaxf(m, x);
       const float alpha = exp2_fast(m - m_new);
       m = m_new;
       l *= alpha;
@@ -266,7 +276,17 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
     // weights, rounded, and the sum of the rounded ones
     float p[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) p[r] = exp2_fast(fmaf(s[r], sc, -m));
+    for (int r = 0; r < 16; ++r) {
+      if (MODE == kPlain) p[r] = exp2_fast(fmaf(s[r], a.scale_log2, -m));
+      if (MODE == kCapped) p[r] = exp2_fast(softcap_log2(s[r] * a.cap_x2, a.cap_log2) - m);
+      if (MODE == kBiased) p[r] = exp2_fast(s[r] - m);
+    }
+    if (MODE == kCapped && !whole) {  // -inf is capped to -cap: out of the sum here
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        p[r] = __uint_as_float(__float_as_uint(p[r]) &
+                               __builtin_amdgcn_sbfe(seen, (r & 3) + 8 * (r >> 2), 1));
+    }
     const uint4 pb[2] = {pack8_bf16(p), pack8_bf16(p + 8)};
     const bf16x2v one = __builtin_bit_cast(bf16x2v, 0x3f803f80u);
 #pragma unroll
@@ -282,24 +302,45 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
             as_bf16x8(pb[sl]), acc[d], 0, 0, 0);
   };
 
-  issue(t_lo, 0);
-  for (int tile = t_lo; tile <= t_hi; ++tile) {
-    const int st = (tile - t_lo) & 1;
-    // this wave's copies of the tile have landed; after the barrier every wave's have,
-    // and every wave is done with the other stage, which the next tile then fills
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tile < t_hi) issue(tile + 1, st ^ 1);
-    sub_tile(Int<0>{}, tile, st * 2 * TB);
-    sub_tile(Int<1>{}, tile, st * 2 * TB);
+  for (;;) {
+    m = -1e38f;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    issue(t_lo, 0);
+    for (int tile = t_lo; tile <= t_hi; ++tile) {
+      const int st = (tile - t_lo) & 1;
+      // this wave's copies of the tile have landed; after the barrier every wave's have,
+      // and every wave is done with the other stage, which the next tile then fills
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tile < t_hi) issue(tile + 1, st ^ 1);
+      const int ks = tile * PN;
+      const uint32_t off = st * 2 * TB;
+      if (KW == 1) {
+        sub_tile(Int<0>{}, ks, off);
+        sub_tile(Int<1>{}, ks + 32, off);
+      } else {
+        sub_tile(Int<0>{}, ks + 32 * wave, off + 32 * RB * wave);
+      }
+    }
+    if (careful) break;
+    float bad = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) bad = fmaf(acc[d][r], 0.f, bad);
+    if (!__syncthreads_or(mine && bad != 0.f)) break;  // NaN: some value is not finite
+    careful = true;
   }
-
-  if (dirty) {
+  if (careful) {
     // the values left out, straight from memory: this lane's dims 8 e + 4 half .. + 3 of
     // every key that its row sees (one that was added before adds nothing new: inf + inf)
     for (int key = wlo; key < whi; ++key) {
       const uint16_t* row = vb + key * a.vr + 4 * half;
-      const uint32_t sees = static_cast<unsigned>(key - lo) < n ? 0xffffffffu : 0u;
+      const uint32_t sees = key >= lo && key < hi ? 0xffffffffu : 0u;
 #pragma unroll
       for (int e = 0; e < 4 * ND; ++e) {
         const uint2 w = *reinterpret_cast<const uint2*>(row + 8 * e);
@@ -312,7 +353,60 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
     }
   }
 
-  const float l_tot = l + __shfl_xor(l, 32, kWave);
+  float l_tot = l + __shfl_xor(l, 32, kWave);
+  if constexpr (KW > 1) {
+    // the waves' (m, l, acc) joined: wave w keeps 32-row columns of dims' quarter w
+    constexpr int LD = HD + 4;
+    float* const so = reinterpret_cast<float*>(smem);
+    float* const sm = so + 4 * 32 * LD;
+    float* const sl = sm + 4 * 32;
+    static_assert((4 * 32 * LD + 8 * 32) * 4 <= 2 * 2 * TB, "the join fits the stages");
+    // the barrier of the check above, or of the last tile, is behind every read of a stage
+    if (careful) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<float4*>(so + (32 * wave + col) * LD + 32 * d + 8 * g4 + 4 * half) =
+            make_float4(acc[d][4 * g4], acc[d][4 * g4 + 1], acc[d][4 * g4 + 2],
+                        acc[d][4 * g4 + 3]);
+    if (half == 0) {
+      sm[32 * wave + col] = m;
+      sl[32 * wave + col] = l_tot;
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (HD / 8);
+    float mx = sm[row];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mx = fmaxf(mx, sm[32 * w + row]);
+    float o[HD / 8], den = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float e = exp2_fast(sm[32 * w + row] - mx);
+      if (e == 0.f) continue;  // no weight: its infinities, which the others have too, add NaN
+      den = fmaf(sl[32 * w + row], e, den);
+#pragma unroll
+      for (int i = 0; i < HD / 8; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(so + (32 * w + row) * LD + c0 + i);
+        o[i] = fmaf(v.x, e, o[i]);
+        o[i + 1] = fmaf(v.y, e, o[i + 1]);
+        o[i + 2] = fmaf(v.z, e, o[i + 2]);
+        o[i + 3] = fmaf(v.w, e, o[i + 3]);
+      }
+    }
+    // whether the row is of a document: lane `row` of every wave knows
+    const uint64_t rows = __ballot(mine);
+    if (!((rows >> row) & 1)) return;
+    const float inv = 1.0f / den;
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i] *= inv;
+    uint16_t* dst = a.o + (static_cast<long long>(q0 + row) * a.hq + h) * HD + c0;
+#pragma unroll
+    for (int i = 0; i < HD / 8; i += 8) *reinterpret_cast<uint4*>(dst + i) = pack8_bf16(o + i);
+    return;
+  }
   if (!mine) return;
   const float inv = 1.0f / l_tot;
   uint16_t* orow = a.o + (static_cast<long long>(qi) * a.hq + h) * HD;
@@ -327,9 +421,19 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_attn_kernel(cons
     }
 }
 
-template <int HD, bool SCORE>
-void launch_packed(const PackedArgs& a, unsigned blocks, hipStream_t s) {
-  hipLaunchKernelGGL((packed_attn_kernel<HD, SCORE>), dim3(blocks), dim3(256), 0, s, a);
+template <int HD, int MODE>
+int32_t launch_packed(const PackedArgs& a, hipStream_t s) {
+  // less than a 128-row workgroup a CU: the waves share rows instead of keys
+  const long long wide = static_cast<long long>((a.N + 127) / 128) * a.hq;
+  const bool few = wide < compute_units();
+  const long long blocks = few ? static_cast<long long>((a.N + 31) / 32) * a.hq : wide;
+  LLMY_REQUIRE(blocks < (1ll << 31));
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (few)
+    hipLaunchKernelGGL((packed_attn_kernel<HD, MODE, 4>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((packed_attn_kernel<HD, MODE, 1>), grid, dim3(256), 0, s, a);
+  return launch_status();
 }
 
 }  // namespace llmy
@@ -353,8 +457,6 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
   for (const int64_t x : {q_row, q_head, k_row, k_head, v_row, v_head})
     LLMY_REQUIRE(x >= 0 && x % 8 == 0);
   LLMY_REQUIRE(k_row < (1 << 22) && v_row < (1 << 22));  // 64-row offsets are 32-bit
-  const long long blocks = static_cast<long long>((N + kPM - 1) / kPM) * Hq;
-  LLMY_REQUIRE(blocks < (1ll << 31));
   // out is written while other workgroups still read k and v
   const int64_t hd = head_dim;
   const auto apart = [&](const llmy_bf16* p, int64_t row, int64_t head) {
@@ -373,12 +475,13 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
   a.cap_x2 = softcap > 0.f ? 2.f * log2e * scale / softcap : 0.f;
   a.N = N; a.docs = docs; a.hq = Hq; a.G = Hq / Hkv; a.window = window;
   const hipStream_t st = as_stream(stream);
-  const unsigned grid = static_cast<unsigned>(blocks);
   // a scale of 0 would turn the masked scores' -inf into NaN in the exponent
-  const bool score = softcap > 0.f || slopes || scale == 0.f;
+  const int mode = slopes || scale == 0.f ? kBiased : softcap > 0.f ? kCapped : kPlain;
   if (head_dim == 64)
-    score ? launch_packed<64, true>(a, grid, st) : launch_packed<64, false>(a, grid, st);
-  else
-    score ? launch_packed<128, true>(a, grid, st) : launch_packed<128, false>(a, grid, st);
-  return launch_status();
+    return mode == kPlain    ? launch_packed<64, kPlain>(a, st)
+           : mode == kCapped ? launch_packed<64, kCapped>(a, st)
+                             : launch_packed<64, kBiased>(a, st);
+  return mode == kPlain    ? launch_packed<128, kPlain>(a, st)
+         : mode == kCapped ? launch_packed<128, kCapped>(a, st)
+                           : launch_packed<128, kBiased>(a, st);
 }

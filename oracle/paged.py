@@ -99,14 +99,22 @@ def packed_prefill(q, k, v, cu_seqlens, scale=None, window=0, softcap=0.0, slope
     for d, (a, e) in enumerate(zip(cu, cu[1:])):
         p = 0 if prefix is None else int(prefix[d])
         j = torch.arange(max(0, e - a))
-        for i in range(a, e):
-            t = i - a
+        for i in range(a, e, 32):
+            t = torch.arange(i, min(i + 32, e))[:, None] - a
             seen = (j <= t) | (j < p)
             if window:
                 seen &= t - j < window
             for h in range(Hq):
                 g = h // (Hq // Hkv)
-                bias = None if slopes is None else slopes[h].double() * (t - j).abs()
-                out[i, h], spread[i, h] = attend(q[i, h], k[a:e, g], v[a:e, g], seen, scale,
-                                                 softcap, bias)
+                x, y = k[a:e, g].double(), v[a:e, g].double()
+                z = scale * (q[i:i + len(t), h].double() @ x.T)
+                if softcap:
+                    z = softcap * torch.tanh(z / softcap)
+                if slopes is not None:
+                    z = z - slopes[h].double() * (t - j).abs()
+                w = torch.softmax(z.masked_fill(~seen, -math.inf), -1)
+                o = w @ y
+                out[i:i + len(t), h] = o
+                spread[i:i + len(t), h] = torch.einsum("nj,njd->nd", w,
+                                                       (y - o[:, None]).abs())
     return out, spread

@@ -93,6 +93,26 @@ def test_longer_prompt(hd):
     _ok(*_both(q * 2, k, v, _cu([1400, 100])))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kw", [{}, {"softcap": 10.0}, {"slopes": True, "window": 150},
+                                {"prefix": [100, 0, 150, 9, 400, 1]}], ids=str)
+def test_many_heads(kw, hd):
+    """Enough rows and heads for workgroups of 128 rows (fewer give 32-row ones)."""
+    g, (q, k, v) = _inputs(640, 64, 2, hd, 4)
+    kw = dict(kw)
+    if kw.pop("slopes", False):
+        kw["slopes"] = torch.rand(64, generator=g) * 0.1
+    if "prefix" in kw:
+        kw["prefix"] = torch.tensor(kw["prefix"], dtype=torch.int32)
+    _ok(*_both(q, k, v, _cu([130, 1, 200, 0, 290, 19]), **kw))
+
+
+def test_more_documents_than_fit_the_table():
+    """Over 511 documents the bounds are bisected in memory."""
+    _, (q, k, v) = _inputs(900, 2, 1, 64, 5)
+    _ok(*_both(q, k, v, _cu([1] * 300 + [0] * 20 + [2] * 300)))
+
+
 def test_rows_of_no_document_are_left():
     _, (q, k, v) = _inputs(200, 4, 2, 64, 5)
     for t in (q, k, v):  # what they hold reaches nobody
@@ -106,14 +126,15 @@ def test_rows_of_no_document_are_left():
     _ok(got[10:150], want[10:150], spread[10:150])
 
 
+@pytest.mark.parametrize("heads", [2, 128])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_values_that_are_not_finite_reach_only_rows_that_see_them(bad, hd):
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(bad, hd, heads):
     """In v: the dims of rows that see the key; in k: every dim of such rows (a NaN score);
     windowed, prefixed and other documents' rows do not."""
     lens = [70, 90, 40]
     prefix = torch.tensor([0, 30, 0], dtype=torch.int32)
-    _, (q, k, v) = _inputs(200, 2, 1, hd, 6)
+    _, (q, k, v) = _inputs(200, heads, 1, hd, 6)
     v[40, 0, 5] = bad
     v[120, 0, hd - 1] = bad
     v[120, 0, 7] = -bad
@@ -130,7 +151,7 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(bad, hd):
         clean_v[r, 0, d] = 0
     clean_k[165] = 0
     want, spread = ref.packed_prefill(q, clean_k, clean_v, cu, **kw)
-    hit = torch.zeros(200, 2, hd, dtype=torch.bool)
+    hit = torch.zeros(200, heads, hd, dtype=torch.bool)
     for r, d, x in ((40, 5, bad), (120, hd - 1, bad), (120, 7, -bad)):
         rows = sees[:, r]
         hit[rows, :, d] = True
