@@ -13,11 +13,17 @@
 //   * Many rows: the four waves of a workgroup own 128 rows and share 64-key tiles.  A
 //     sub-tile is 82 vector instructions beside its 16 (128-wide heads) or 8 matrix
 //     ones, and two or four waves a SIMD run the one kind under the other's.
-//   * Few rows (less than a workgroup a CU): the four waves own the same 32 rows and
-//     take a quarter of each 128-key tile each; their sums are joined in LDS.  The
-//     longest chain is a quarter as long and there are four times the workgroups.
-// Blocks run from the last rows to the first, the longest ones of a document first,
-// heads fastest: with 8 or 16 heads a head's blocks share an XCD's L2.
+//   * Few rows: two or four waves own the same 32 rows and take a half of each 64-key or
+//     a quarter of each 128-key tile; their sums are joined in LDS.  The longest chain
+//     of sub-tiles, 1100 cycles each where a SIMD has little else, is a half or a quarter
+//     as long and there are more workgroups, against two or four times the copies.
+//     One prompt, 16 heads over 4, us with 1 / 2 / 4 waves along the keys (a workgroup a
+//     128 rows and head): 1024 rows (128 workgroups) x 64 21 / 15 / 12, x 128 31 / 22 / 22;
+//     2048 (256) 40 / 30 / 28, 57 / 41 / 60; 4096 (512) 78 / 61 / 82, 112 / 98 / 197;
+//     8192 (1024) 175 / 178 / 285, 307 / 350 / 744.  So four up to half a workgroup a
+//     CU, two up to two.
+// Blocks run from the last rows to the first, the longest ones of a document first; the
+// query heads of a key-value head run side by side on one XCD and share its L2.
 //
 // What a masked place holds, NaN and infinities included, must reach no row, and 0 * inf
 // is NaN in the product.  The values are not looked at as they pass (96 instructions a
@@ -42,20 +48,8 @@ struct PackedArgs {
   const int32_t *cu, *prefix;
   const float* slopes;
   float scale_log2, cap_log2, cap_x2;
-  int N, docs, hq, G, window;
+  int N, docs, hq, hkv, G, window;
 };
-
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v = min(v, __shfl_xor(v, d, kWave));
-  return __builtin_amdgcn_readfirstlane(v);
-}
-
-__device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v = max(v, __shfl_xor(v, d, kWave));
-  return __builtin_amdgcn_readfirstlane(v);
-}
 
 // Per 16-bit half, 0xffff where its exponent is all ones (infinities and NaN).
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
@@ -69,30 +63,45 @@ struct Int {
   static constexpr int value = V;
 };
 
-enum { kPlain = 0, kCapped = 1, kBiased = 2 };  // kBiased: a distance bias, a cap or not
+enum { kPlain = 0, kCapped = 1, kBiased = 2, kBiasedCapped = 3 };
 
-// KW: waves along the keys (1 or 4); 4 / KW waves along the rows.
+// KW: waves along the keys (1, 2 or 4); 4 / KW waves along the rows.
 template <int HD, int MODE, int KW>
-__global__ __launch_bounds__(256, HD == 64 && KW == 1 ? 4 : HD == 64 || KW == 1 ? 2 : 1)
+__global__ __launch_bounds__(256, (HD == 64 ? 4 : 2) / (KW == 4 ? 2 : 1))
 void packed_attn_kernel(const PackedArgs a) {
   constexpr int ND = HD / 32;             // 32-dim output tiles
   constexpr int NS = HD / 16;             // 16-dim slices of the score product
   constexpr int RB = 2 * HD;              // bytes of a staged row
   constexpr int PM = 128 / KW;            // rows per workgroup
-  constexpr int PN = KW == 1 ? 64 : 128;  // keys per staged tile
+  constexpr int PN = KW == 4 ? 128 : 64;  // keys per staged tile
   constexpr int TB = PN * RB;             // bytes of a staged K or V tile
-  __shared__ __align__(1024) uint8_t smem[2 * 2 * TB];
+  // the two stages; with two waves along the keys the join takes 4 KiB more
+  __shared__ __align__(1024) uint8_t smem[2 * 2 * TB + (KW == 2 ? 4096 : 0)];
   __shared__ int range[2][4];
   __shared__ int cu_s[kDocsInLds + 1];
 
+  // workgroup i runs on XCD i % 8: a unit, PM rows of one key-value head, goes to one of
+  // them with all its query heads
   const int nblk = (a.N + PM - 1) / PM;
-  const int h = blockIdx.x % a.hq;
-  const int q0 = (nblk - 1 - static_cast<int>(blockIdx.x / a.hq)) * PM;
+  const int unit = static_cast<int>(blockIdx.x / (8u * a.G)) * 8 + static_cast<int>(blockIdx.x % 8u);
+  const int qb = unit / a.hkv;
+  if (qb >= nblk) return;
+  const int kvh = unit - qb * a.hkv;
+  const int h = kvh * a.G + static_cast<int>(blockIdx.x / 8u) % a.G;
+  const int q0 = (nblk - 1 - qb) * PM;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5;
   const int col = lane & 31;
-  const int qi = q0 + (KW == 1 ? 32 * wave : 0) + col;  // this lane's row
+  const int rg = wave / KW, part = wave % KW;  // 32 rows, 1 / KW of the sub-tiles
+  const int qi = q0 + 32 * rg + col;           // this lane's row
+
+  u32x4 qf[NS];
+  {
+    const uint16_t* qp = a.q + min(qi, a.N - 1) * a.qr + h * a.qh + 8 * half;
+#pragma unroll
+    for (int t = 0; t < NS; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + 16 * t);
+  }
 
   // its document by bisection (few documents: in LDS, one load's latency instead of a
   // chain), its keys [lo, hi); none for a row of no document
@@ -118,10 +127,13 @@ void packed_attn_kernel(const PackedArgs a) {
       hi = max(qi + 1, first + two_way);
     }
   }
-  // the wave's rows see keys in [wlo, whi), all of them those in [ilo, ihi)
-  const int big = 0x7fffffff;
-  const int wlo = wave_min_i(mine ? lo : big), whi = wave_max_i(mine ? hi : 0);
-  const int ilo = wave_max_i(mine ? lo : 0), ihi = wave_min_i(mine ? hi : big);
+  // the wave's rows see keys in [wlo, whi), all of them those in [ilo, ihi): both bounds
+  // ascend with the row, so the first and the last row of a document say it
+  const uint32_t rows = static_cast<uint32_t>(__ballot(mine));
+  const int r0 = rows ? __ffs(rows) - 1 : 0, r1 = rows ? 31 - __clz(rows) : 0;
+  const int wlo = rows ? __builtin_amdgcn_readlane(lo, r0) : 0x7fffffff;
+  const int whi = rows ? __builtin_amdgcn_readlane(hi, r1) : 0;
+  const int ilo = __builtin_amdgcn_readlane(lo, r1), ihi = __builtin_amdgcn_readlane(hi, r0);
   if (lane == 0) {
     range[0][wave] = wlo;
     range[1][wave] = whi;
@@ -133,14 +145,8 @@ void packed_attn_kernel(const PackedArgs a) {
   const int t_lo = __builtin_amdgcn_readfirstlane(glo / PN);
   const int t_hi = __builtin_amdgcn_readfirstlane((ghi - 1) / PN);
 
-  u32x4 qf[NS];
-  {
-    const uint16_t* qp = a.q + min(qi, a.N - 1) * a.qr + h * a.qh + 8 * half;
-#pragma unroll
-    for (int t = 0; t < NS; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + 16 * t);
-  }
   const float slope =
-      MODE == kBiased && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
+      MODE >= kBiased && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
 
   f32x16v acc[ND];
   float m, l;  // the exponent's offset (scaled, log2) and the sum of weights
@@ -150,8 +156,8 @@ void packed_attn_kernel(const PackedArgs a) {
   constexpr int CH = HD / 8;
   constexpr int RPB = 64 / CH;
   constexpr int BPW = PN / RPB / 4;
-  const uint16_t* kb = a.k + (h / a.G) * a.kh;
-  const uint16_t* vb = a.v + (h / a.G) * a.vh;
+  const uint16_t* kb = a.k + kvh * a.kh;
+  const uint16_t* vb = a.v + kvh * a.vh;
   const int kr = static_cast<int>(a.kr), vr = static_cast<int>(a.vr);
   uint32_t kdo[BPW], vdo[BPW];
 #pragma unroll
@@ -221,13 +227,13 @@ void packed_attn_kernel(const PackedArgs a) {
               lds_get_tr16(va[d & 1] + off + (S + (16 * sl + 8 * e) * RB + 128 * (d >> 1)));
     // register r holds key ks + 4 half + c(r), c(r) = (r & 3) + 8 (r >> 2)
     const bool whole = ks >= ilo && ks + 32 <= ihi;
-    if (MODE == kBiased) {
+    if (MODE >= kBiased) {
       const float dq = static_cast<float>(qi - ks - 4 * half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float c = (r & 3) + 8 * (r >> 2);
-        const float z = a.cap_x2 > 0.f ? softcap_log2(s[r] * a.cap_x2, a.cap_log2)
-                                       : s[r] * a.scale_log2;
+        const float z = MODE == kBiasedCapped ? softcap_log2(s[r] * a.cap_x2, a.cap_log2)
+                                              : s[r] * a.scale_log2;
         s[r] = fmaf(-slope, fabsf(dq - c), z);
       }
     }
@@ -279,7 +285,7 @@ void packed_attn_kernel(const PackedArgs a) {
     for (int r = 0; r < 16; ++r) {
       if (MODE == kPlain) p[r] = exp2_fast(fmaf(s[r], a.scale_log2, -m));
       if (MODE == kCapped) p[r] = exp2_fast(softcap_log2(s[r] * a.cap_x2, a.cap_log2) - m);
-      if (MODE == kBiased) p[r] = exp2_fast(s[r] - m);
+      if (MODE >= kBiased) p[r] = exp2_fast(s[r] - m);
     }
     if (MODE == kCapped && !whole) {  // -inf is capped to -cap: out of the sum here
 #pragma unroll
@@ -323,7 +329,7 @@ void packed_attn_kernel(const PackedArgs a) {
         sub_tile(Int<0>{}, ks, off);
         sub_tile(Int<1>{}, ks + 32, off);
       } else {
-        sub_tile(Int<0>{}, ks + 32 * wave, off + 32 * RB * wave);
+        sub_tile(Int<0>{}, ks + 32 * part, off + 32 * RB * part);
       }
     }
     if (careful) break;
@@ -355,13 +361,13 @@ void packed_attn_kernel(const PackedArgs a) {
 
   float l_tot = l + __shfl_xor(l, 32, kWave);
   if constexpr (KW > 1) {
-    // the waves' (m, l, acc) joined: wave w keeps 32-row columns of dims' quarter w
-    constexpr int LD = HD + 4;
+    // the (m, l, acc) of the KW waves of each 32 rows joined, HD / LPR dims a thread
+    constexpr int PMR = 128 / KW, LPR = 256 / PMR, NO = HD / LPR, LD = HD + 4;
     float* const so = reinterpret_cast<float*>(smem);
-    float* const sm = so + 4 * 32 * LD;
-    float* const sl = sm + 4 * 32;
-    static_assert((4 * 32 * LD + 8 * 32) * 4 <= 2 * 2 * TB, "the join fits the stages");
-    // the barrier of the check above, or of the last tile, is behind every read of a stage
+    float* const sm = so + 128 * LD;
+    float* const sl = sm + 128;
+    static_assert((128 * LD + 256) * 4 <= 2 * 2 * TB + (KW == 2 ? 4096 : 0), "the join fits");
+    // the barrier of the check above is behind every read of a stage, but for a second run
     if (careful) __syncthreads();
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -371,40 +377,39 @@ void packed_attn_kernel(const PackedArgs a) {
             make_float4(acc[d][4 * g4], acc[d][4 * g4 + 1], acc[d][4 * g4 + 2],
                         acc[d][4 * g4 + 3]);
     if (half == 0) {
-      sm[32 * wave + col] = m;
+      sm[32 * wave + col] = mine ? m : INFINITY;  // a row of no document: not stored
       sl[32 * wave + col] = l_tot;
     }
     __syncthreads();
-    const int row = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (HD / 8);
-    float mx = sm[row];
+    const int row = threadIdx.x / LPR, c0 = (threadIdx.x % LPR) * NO;
+    const int at = (row >> 5) * KW * 32 + (row & 31);  // of its first wave
+    float mx = sm[at];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) mx = fmaxf(mx, sm[32 * w + row]);
-    float o[HD / 8], den = 0.f;
+    for (int w = 1; w < KW; ++w) mx = fmaxf(mx, sm[at + 32 * w]);
+    if (mx == INFINITY) return;
+    float o[NO], den = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i] = 0.f;
+    for (int i = 0; i < NO; ++i) o[i] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float e = exp2_fast(sm[32 * w + row] - mx);
+    for (int w = 0; w < KW; ++w) {
+      const float e = exp2_fast(sm[at + 32 * w] - mx);
       if (e == 0.f) continue;  // no weight: its infinities, which the others have too, add NaN
-      den = fmaf(sl[32 * w + row], e, den);
+      den = fmaf(sl[at + 32 * w], e, den);
 #pragma unroll
-      for (int i = 0; i < HD / 8; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(so + (32 * w + row) * LD + c0 + i);
+      for (int i = 0; i < NO; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(so + (at + 32 * w) * LD + c0 + i);
         o[i] = fmaf(v.x, e, o[i]);
         o[i + 1] = fmaf(v.y, e, o[i + 1]);
         o[i + 2] = fmaf(v.z, e, o[i + 2]);
         o[i + 3] = fmaf(v.w, e, o[i + 3]);
       }
     }
-    // whether the row is of a document: lane `row` of every wave knows
-    const uint64_t rows = __ballot(mine);
-    if (!((rows >> row) & 1)) return;
     const float inv = 1.0f / den;
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i] *= inv;
+    for (int i = 0; i < NO; ++i) o[i] *= inv;
     uint16_t* dst = a.o + (static_cast<long long>(q0 + row) * a.hq + h) * HD + c0;
 #pragma unroll
-    for (int i = 0; i < HD / 8; i += 8) *reinterpret_cast<uint4*>(dst + i) = pack8_bf16(o + i);
+    for (int i = 0; i < NO; i += 8) *reinterpret_cast<uint4*>(dst + i) = pack8_bf16(o + i);
     return;
   }
   if (!mine) return;
@@ -423,14 +428,17 @@ void packed_attn_kernel(const PackedArgs a) {
 
 template <int HD, int MODE>
 int32_t launch_packed(const PackedArgs& a, hipStream_t s) {
-  // less than a 128-row workgroup a CU: the waves share rows instead of keys
   const long long wide = static_cast<long long>((a.N + 127) / 128) * a.hq;
-  const bool few = wide < compute_units();
-  const long long blocks = few ? static_cast<long long>((a.N + 31) / 32) * a.hq : wide;
+  const int cus = compute_units();
+  const int kw = wide <= cus / 2 ? 4 : wide <= 2 * cus ? 2 : 1;
+  const long long units = static_cast<long long>((a.N + 128 / kw - 1) / (128 / kw)) * a.hkv;
+  const long long blocks = (units + 7) / 8 * 8 * a.G;
   LLMY_REQUIRE(blocks < (1ll << 31));
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (few)
+  if (kw == 4)
     hipLaunchKernelGGL((packed_attn_kernel<HD, MODE, 4>), grid, dim3(256), 0, s, a);
+  else if (kw == 2)
+    hipLaunchKernelGGL((packed_attn_kernel<HD, MODE, 2>), grid, dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((packed_attn_kernel<HD, MODE, 1>), grid, dim3(256), 0, s, a);
   return launch_status();
@@ -473,15 +481,18 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
   a.scale_log2 = scale * log2e;
   a.cap_log2 = softcap * log2e;
   a.cap_x2 = softcap > 0.f ? 2.f * log2e * scale / softcap : 0.f;
-  a.N = N; a.docs = docs; a.hq = Hq; a.G = Hq / Hkv; a.window = window;
+  a.N = N; a.docs = docs; a.hq = Hq; a.hkv = Hkv; a.G = Hq / Hkv; a.window = window;
   const hipStream_t st = as_stream(stream);
-  // a scale of 0 would turn the masked scores' -inf into NaN in the exponent
-  const int mode = slopes || scale == 0.f ? kBiased : softcap > 0.f ? kCapped : kPlain;
-  if (head_dim == 64)
-    return mode == kPlain    ? launch_packed<64, kPlain>(a, st)
-           : mode == kCapped ? launch_packed<64, kCapped>(a, st)
-                             : launch_packed<64, kBiased>(a, st);
-  return mode == kPlain    ? launch_packed<128, kPlain>(a, st)
-         : mode == kCapped ? launch_packed<128, kCapped>(a, st)
-                           : launch_packed<128, kBiased>(a, st);
+  // a scale of 0 would turn the masked scores' -inf into NaN in the exponent of kPlain
+  const bool cap = softcap > 0.f;
+  const int mode = slopes || scale == 0.f ? (cap ? kBiasedCapped : kBiased)
+                                          : (cap ? kCapped : kPlain);
+  const auto launch = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    return mode == kPlain    ? launch_packed<HD, kPlain>(a, st)
+           : mode == kCapped ? launch_packed<HD, kCapped>(a, st)
+           : mode == kBiased ? launch_packed<HD, kBiased>(a, st)
+                             : launch_packed<HD, kBiasedCapped>(a, st);
+  };
+  return head_dim == 64 ? launch(Int<64>{}) : launch(Int<128>{});
 }
