@@ -48,7 +48,8 @@ __device__ __forceinline__ int32_t scalar_at(const int32_t* p, long long i) {
 }
 
 constexpr int kStep = 32;      // keys a step
-constexpr int kMinSteps = 4;   // least steps of a run: 128 keys
+constexpr int kMinSteps = 1;   // least steps of a run
+constexpr int kWhole = 128;    // tokens that are not cut
 
 struct PagedArgs {
   const uint16_t* q;
@@ -57,6 +58,7 @@ struct PagedArgs {
   const int32_t *table, *lengths;
   uint16_t* out;               // [B, Hq, HD]
   float *po, *pml;             // partials: O [2 runs, GT, HD] and (m, l) [2 runs, GT, 2]
+  int32_t* starts;             // [B + 1]: steps of the sequences before each, and of all
   const float* slopes;
   float scale_log2, cap_log2, cap_x2, v_scale;
   int B, hq, hkv, G, HT, GT;   // G = Hq / Hkv in HT tiles of GT <= 16 heads
@@ -77,28 +79,17 @@ __device__ __forceinline__ Seq seq_of(int len, int cap_len, int window) {
   return s;
 }
 
-__device__ __forceinline__ long long shfl_up64(long long v, int d) {
-  const int lo = __shfl_up(static_cast<int>(v & 0xffffffffll), d, kWave);
-  const int hi = __shfl_up(static_cast<int>(v >> 32), d, kWave);
-  return (static_cast<long long>(hi) << 32) | static_cast<uint32_t>(lo);
-}
-
-__device__ __forceinline__ long long readlane64(long long v, int l) {
-  const int lo = __builtin_amdgcn_readlane(static_cast<int>(v & 0xffffffffll), l);
-  const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
-  return (static_cast<long long>(hi) << 32) | static_cast<uint32_t>(lo);
-}
-
-// Steps of all sequences, as sums over 64 blocks of `per` sequences, one per lane.
+// Steps of all sequences (the host sees to it that they fit 31 bits), as sums over 64
+// blocks of `per` sequences, one per lane.
 struct StepScan {
-  long long before, upto, total;  // this lane's block: exclusive and inclusive sums
+  int before, upto, total;  // this lane's block: exclusive and inclusive sums
   int per;
 };
 
 __device__ __forceinline__ StepScan scan_steps(const PagedArgs& a, int lane) {
   StepScan r;
   r.per = (a.B + kWave - 1) / kWave;
-  long long n = 0;
+  int n = 0;
   const int b1 = min(a.B, (lane + 1) * r.per);
   for (int b = lane * r.per; b < b1; ++b) {
     const Seq s = seq_of(a.lengths[b], a.cap_len, a.window);
@@ -107,11 +98,11 @@ __device__ __forceinline__ StepScan scan_steps(const PagedArgs& a, int lane) {
   r.upto = n;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
-    const long long o = shfl_up64(r.upto, d);
+    const int o = __shfl_up(r.upto, d, kWave);
     if (lane >= d) r.upto += o;
   }
   r.before = r.upto - n;
-  r.total = readlane64(r.upto, kWave - 1);
+  r.total = __builtin_amdgcn_readlane(r.upto, kWave - 1);
   return r;
 }
 
@@ -145,7 +136,8 @@ struct Tile {
   static constexpr int RPB = 64 / CH;                // rows of one 1 KiB DMA
   static constexpr int NB = kStep / RPB;             // DMAs of a K or V tile
   static constexpr int BYTES = kStep * RB;           // of a K or V tile
-  static constexpr int STAGES = BYTES >= 8192 ? 2 : 3;
+  static constexpr int STAGES = F8 || HD == 128 ? 2 : 3;
+  static constexpr int LDS = 2 * STAGES * BYTES;
   static __device__ __forceinline__ int kswz(int row) {
     return CH == 4 ? (row >> 1) & 3 : row & 7;
   }
@@ -163,7 +155,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
   constexpr int NS = HD / 32;                 // 32-dim slices of the score product
   constexpr int ND = HD / 16;                 // 16-dim output tiles
   constexpr int NK = F8 ? HD / 64 : HD / 32;  // 16-byte K reads of a 16-key tile
-  __shared__ __align__(1024) uint8_t smem[ST * 2 * T::BYTES];
+  __shared__ __align__(1024) uint8_t smem[T::LDS];
 
   const int lane = threadIdx.x;
   const int g = lane >> 4, col = lane & 15;
@@ -189,13 +181,23 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     }
   } else {
     const StepScan sc = scan_steps(a, lane);
-    const long long total = sc.total * units;
+    if (blockIdx.x == 0) {  // where each sequence's steps begin, for the join
+      int at = sc.before;
+      const int b1 = min(a.B, (lane + 1) * sc.per);
+      for (int i = lane * sc.per; i < b1; ++i) {
+        a.starts[i] = at;
+        const Seq q = seq_of(a.lengths[i], a.cap_len, a.window);
+        at += q.s1 - q.s0;
+      }
+      if (lane == 0) a.starts[a.B] = sc.total;
+    }
+    const long long total = static_cast<long long>(sc.total) * units;
     run_q = run_steps(total, a.runs);
     run_at = static_cast<long long>(blockIdx.x) * run_q;
     if (run_at >= total) return;
     count = static_cast<int>(min(static_cast<long long>(run_q), total - run_at));
-    const int blk = __ffsll(static_cast<unsigned long long>(__ballot(sc.upto * units > run_at))) - 1;
-    long long at = readlane64(sc.before, blk);
+    const int blk = __ffsll(static_cast<unsigned long long>(__ballot(static_cast<long long>(sc.upto) * units > run_at))) - 1;
+    long long at = __builtin_amdgcn_readlane(sc.before, blk);
     b = blk * sc.per;
     for (;; ++b) {  // ends: the block's sum passes run_at
       cur = seq_of(scalar_at(a.lengths, b), a.cap_len, a.window);
@@ -248,8 +250,8 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
 #pragma unroll
       for (int j = 0; j < NB / 2; ++j) {
         const int blk = h * (NB / 2) + j;
-        lds_fill16(kp + j * 1024, kdo[blk], dst + blk * 1024);
-        lds_fill16(vp + j * 1024, vdo[blk], dst + T::BYTES + blk * 1024);
+        lds_fill16<true>(kp + j * 1024, kdo[blk], dst + blk * 1024);
+        lds_fill16<true>(vp + j * 1024, vdo[blk], dst + T::BYTES + blk * 1024);
       }
     }
   };
@@ -375,16 +377,23 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = exp2_fast(z[j] - m_sub);
+    // the weights as a sum of two bf16: the matrix cores have time to spare here
     const uint4 pb = pack8_bf16(p);
-    unpack8(pb, p);
+    float hi[8];
+    unpack8(pb, hi);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l_run += p[j];
+    for (int j = 0; j < 8; ++j) {
+      l_run += p[j];
+      hi[j] = p[j] - hi[j];
+    }
+    const uint4 pl = pack8_bf16(hi);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const bf16x8 vv = F8 ? e4m3_to_bf16(vf[d].x, vf[d].y)
                            : as_bf16x8(uint4{vf[F8 ? 0 : 2 * d].x, vf[F8 ? 0 : 2 * d].y,
                                              vf[F8 ? 0 : 2 * d + 1].x, vf[F8 ? 0 : 2 * d + 1].y});
       acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pb), acc[d], 0, 0, 0);
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pl), acc[d], 0, 0, 0);
     }
     // once every read of this stage has returned, the next step may land in it
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -428,37 +437,28 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
 }
 
 // Joins the partials of one (sequence, query head): o = sum_i 2^(m_i - m) O_i /
-// sum_i 2^(m_i - m) l_i, in the runs' order within each of 512 / (HD / 4) lane groups
-// and then over the groups, so the result does not depend on timing.
-template <int HD>
-__global__ __launch_bounds__(512) void paged_join_kernel(const PagedArgs a) {
+// sum_i 2^(m_i - m) l_i, in the runs' order within each of T / (HD / 4) lane groups and
+// then over the groups, so the result does not depend on timing.  T threads: 64 where
+// the heads alone fill the chip, 512 where few heads have many partials each.
+template <int HD, int T>
+__global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
   constexpr int LPP = HD / 4;       // lanes a partial
-  constexpr int NG = 512 / LPP;
+  constexpr int NG = T / LPP;
   __shared__ __align__(16) float so[NG][HD];
   __shared__ float sm[NG], sl[NG];
-  const int lane = threadIdx.x & 63;
   const int grp = threadIdx.x / LPP, c = threadIdx.x % LPP;
   const int b = blockIdx.x / a.hq, h = blockIdx.x - b * a.hq;
   const int kvh = h / a.G, ht = (h - kvh * a.G) / 16, row = h - kvh * a.G - 16 * ht;
   const int units = a.hkv * a.HT, u = kvh * a.HT + ht;
   uint16_t* out = a.out + static_cast<long long>(blockIdx.x) * HD;
 
-  const StepScan sc = scan_steps(a, lane);
-  const int q = run_steps(sc.total * units, a.runs);
-  const int blk = b / sc.per;
-  long long at = readlane64(sc.before, blk);
-  Seq s;
-  for (int x = blk * sc.per;; ++x) {  // ends at x = b
-    s = seq_of(scalar_at(a.lengths, x), a.cap_len, a.window);
-    if (x == b) break;
-    at += s.s1 - s.s0;
-  }
-  const int n = s.s1 - s.s0;
+  const int start = scalar_at(a.starts, b), n = scalar_at(a.starts, b + 1) - start;
   if (n == 0) {  // nothing visible: zeros
     if (threadIdx.x < LPP) *reinterpret_cast<uint2*>(out + 4 * c) = make_uint2(0u, 0u);
     return;
   }
-  const long long first = at * units + static_cast<long long>(u) * n;
+  const int q = run_steps(static_cast<long long>(scalar_at(a.starts, a.B)) * units, a.runs);
+  const long long first = static_cast<long long>(start) * units + static_cast<long long>(u) * n;
   const int w0 = static_cast<int>(first / q), w1 = static_cast<int>((first + n - 1) / q);
   if (w0 == w1) return;  // stored by its run
   float m = -INFINITY, l = 0.f;
@@ -484,12 +484,13 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedArgs a) {
     sl[grp] = l;
   }
   __syncthreads();
-  if (threadIdx.x < HD) {
-    const int d = threadIdx.x;
-    float mx = sm[0];
-    for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[i]);
-    const float m_sub = mx == -INFINITY ? 0.f : mx;
+  float mx = sm[0];
+#pragma unroll
+  for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[i]);
+  const float m_sub = mx == -INFINITY ? 0.f : mx;
+  for (int d = threadIdx.x; d < HD; d += T) {
     float num = 0.f, den = 0.f;
+#pragma unroll
     for (int i = 0; i < NG; ++i) {
       const float e = exp2_fast(sm[i] - m_sub);
       num = fmaf(so[i][d], e, num);
@@ -499,11 +500,12 @@ __global__ __launch_bounds__(512) void paged_join_kernel(const PagedArgs a) {
   }
 }
 
-// Waves that the chip holds at once: what a CU's 160 KiB of LDS take, 8 at most.
+// Waves that the chip holds at once: what a CU's 160 KiB of LDS take, 12 at most.
 inline int paged_runs(int head_dim, bool f8) {
-  const int lds = head_dim == 128 ? (f8 ? 24576 : 32768) : (f8 ? 12288 : 24576);
-  const int per_cu = 163840 / lds;
-  return compute_units() * (per_cu < 8 ? per_cu : 8);
+  const int lds = head_dim == 128 ? (f8 ? Tile<128, true>::LDS : Tile<128, false>::LDS)
+                                  : (f8 ? Tile<64, true>::LDS : Tile<64, false>::LDS);
+  const int per_cu = (163840 - 1) / lds;  // five of 32 KiB do not fit beside each other
+  return compute_units() * (per_cu < 12 ? per_cu : 12);
 }
 
 struct PagedPlan {
@@ -521,13 +523,14 @@ inline bool paged_plan(int B, int Hq, int Hkv, int hd, int width, int page, int 
   p->GT = p->G < 16 ? p->G : 16;
   p->cap_len = static_cast<long long>(width) * page;
   if (p->cap_len >= (1ll << 31) - kStep) return false;  // positions are 32-bit
-  const bool cut = p->cap_len > kMinSteps * kStep;
+  const bool cut = p->cap_len > kWhole;
   p->runs = cut ? paged_runs(hd, type == kCacheE4m3) : 0;
   p->waves = cut ? p->runs : static_cast<long long>(B) * Hkv * p->HT;
-  p->ws = cut ? 2ll * p->runs * p->GT * (hd + 2) * 4 : 0;
-  // a run's steps, a unit's number and the grids are 32-bit
-  const double steps = static_cast<double>(B) * Hkv * p->HT * (p->cap_len / kStep + 1);
-  return steps < 1e12 && p->waves < (1ll << 31) && static_cast<long long>(B) * Hq < (1ll << 31);
+  p->ws = cut ? 2ll * p->runs * p->GT * (hd + 2) * 4 + (static_cast<long long>(B) + 1) * 4 : 0;
+  // all steps, a run's steps and the grids are 32-bit
+  const double steps = static_cast<double>(B) * (p->cap_len / kStep + 1);
+  return steps < 2147483647. && p->waves < (1ll << 31) &&
+         static_cast<long long>(B) * Hq < (1ll << 31);
 }
 
 }  // namespace llmy
@@ -565,6 +568,7 @@ extern "C" int32_t llmy_paged_attn_decode(
   a.table = page_table; a.lengths = lengths; a.out = out; a.slopes = slopes;
   a.po = static_cast<float*>(workspace);
   a.pml = a.po + 2ll * p.runs * p.GT * head_dim;
+  a.starts = reinterpret_cast<int32_t*>(a.pml + 4ll * p.runs * p.GT);
   const float log2e = 1.4426950408889634f, qk = scale * k_scale;
   a.scale_log2 = qk * log2e;
   a.cap_log2 = softcap * log2e;
@@ -575,16 +579,18 @@ extern "C" int32_t llmy_paged_attn_decode(
   a.cap_len = pages ? static_cast<int>(p.cap_len) : 0;
   a.runs = p.runs;
   const hipStream_t s = as_stream(stream);
-  const dim3 grid(static_cast<unsigned>(p.waves)), join(static_cast<unsigned>(B) * Hq);
-  const bool f8 = cache_type == kCacheE4m3;
+  const dim3 grid(static_cast<unsigned>(p.waves)), heads(static_cast<unsigned>(B) * Hq);
+  const bool f8 = cache_type == kCacheE4m3, many = heads.x >= 1024;
   if (head_dim == 64) {
     if (f8) hipLaunchKernelGGL((paged_attn_kernel<64, true>), grid, dim3(64), 0, s, a);
     else hipLaunchKernelGGL((paged_attn_kernel<64, false>), grid, dim3(64), 0, s, a);
-    if (p.runs) hipLaunchKernelGGL(paged_join_kernel<64>, join, dim3(512), 0, s, a);
+    if (p.runs && many) hipLaunchKernelGGL((paged_join_kernel<64, 64>), heads, dim3(64), 0, s, a);
+    else if (p.runs) hipLaunchKernelGGL((paged_join_kernel<64, 512>), heads, dim3(512), 0, s, a);
   } else {
     if (f8) hipLaunchKernelGGL((paged_attn_kernel<128, true>), grid, dim3(64), 0, s, a);
     else hipLaunchKernelGGL((paged_attn_kernel<128, false>), grid, dim3(64), 0, s, a);
-    if (p.runs) hipLaunchKernelGGL(paged_join_kernel<128>, join, dim3(512), 0, s, a);
+    if (p.runs && many) hipLaunchKernelGGL((paged_join_kernel<128, 64>), heads, dim3(64), 0, s, a);
+    else if (p.runs) hipLaunchKernelGGL((paged_join_kernel<128, 512>), heads, dim3(512), 0, s, a);
   }
   return launch_status();
 }

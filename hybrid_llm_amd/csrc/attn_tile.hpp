@@ -51,12 +51,17 @@ __device__ __forceinline__ void lds_settle_v(u32x2* f) {
 // dst the wave's LDS byte address.  s_nop 3 after the move of m0 makes the five wait
 // states that the load needs after a VALU write of an SGPR that it reads.  m0 is
 // reserved (hence a warning), but the compiler keeps values there for its own use:
-// the clobber says that they are gone.
+// the clobber says that they are gone.  STREAM: data read once, not kept in the caches.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+template <bool STREAM = false>
 __device__ __forceinline__ void lds_fill16(const void* base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
-               ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
+                 ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
