@@ -314,61 +314,63 @@ def banded_attn_decode_parts(parts: torch.Tensor, k_off: int, v_off: int, k_cach
 
 # ---------------------------------------------- full-length attention over a paged cache
 CACHE_BF16, CACHE_E4M3 = 0, 1
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _CACHE_TYPES = {torch.bfloat16: CACHE_BF16, torch.float8_e4m3fn: CACHE_E4M3}
+# One test a tensor, its message formed only where it fails: these calls take 3 us on the
+# GPU at their smallest, less than checks that name each property in turn.
 
 
-def _here(*tensors) -> None:
-    """Every tensor is on the current device, whose stream the call uses."""
-    dev = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensors must be on the current device (cuda:{dev}), got {t.device}")
+def _heads(t: torch.Tensor, name: str, shape: tuple, dev: int) -> int:
+    """The address of bf16 rows [N, H, hd] on device ``dev`` whose heads' dims are
+    contiguous (the library checks the other strides)."""
+    if (t.dtype is _BF16 and t.shape == shape and t.stride(2) == 1 and t.get_device() == dev):
+        return t.data_ptr()
+    raise ValueError(f"{name} must be torch.bfloat16 {shape} with contiguous dims on cuda:{dev}, "
+                     f"the current device; got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, "
+                     f"{t.device}")
 
 
-def _check_rows(t: torch.Tensor, name: str, shape: tuple, step: int) -> None:
-    """bf16 [N, H, hd] whose heads' dims are contiguous; strides multiples of ``step``."""
-    if t.dtype != torch.bfloat16 or t.shape != shape:
-        raise ValueError(f"{name} must be torch.bfloat16 {tuple(shape)}, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    row, head, one = t.stride()
-    if one != 1 or row % step or head % step:
-        raise ValueError(f"{name}: dims must be contiguous and strides multiples of {step}, got "
-                         f"{t.stride()}")
+def _out_heads(t: torch.Tensor | None, name: str, like: torch.Tensor, shape: tuple,
+               dev: int) -> tuple:
+    """The output, given or made, its address, row and head strides."""
+    if t is None:
+        t = like.new_empty(shape)
+        return t, t.data_ptr(), shape[1] * shape[2], shape[2]
+    return t, _heads(t, name, shape, dev), t.stride(0), t.stride(1)
 
 
-def _check_f32(t: torch.Tensor | None, name: str, n: int) -> None:
-    if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous torch.float32 [{n}], got {t.dtype} "
-                         f"{tuple(t.shape)}")
+def _vec(t: torch.Tensor | None, name: str, dtype: torch.dtype, shape: tuple, dev: int):
+    """The address of a contiguous tensor on device ``dev``; None: none given."""
+    if t is None:
+        return None
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+        return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous {dtype} {shape} on cuda:{dev}, the current "
+                     f"device; got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, {t.device}")
 
 
-def _check_i32(t: torch.Tensor | None, name: str, shape: tuple) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous torch.int32 {tuple(shape)}, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-
-
-def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, hd: int) -> tuple:
+def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, hd: int, dev: int) -> tuple:
     """(pages, page, cache type) of a [pages, Hkv, page, hd] cache pair."""
     kind = _CACHE_TYPES.get(k_cache.dtype)
-    if kind is None or v_cache.dtype != k_cache.dtype:
-        raise ValueError("k_cache and v_cache must both be torch.bfloat16 or "
-                         f"torch.float8_e4m3fn, got {k_cache.dtype} and {v_cache.dtype}")
-    if (k_cache.dim() != 4 or k_cache.shape[1] != Hkv or k_cache.shape[3] != hd
-            or v_cache.shape != k_cache.shape):
-        raise ValueError(f"caches must be [pages, {Hkv}, page, {hd}], got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError("caches must be contiguous")
-    return k_cache.shape[0], k_cache.shape[2], kind
+    shape = k_cache.shape
+    if (kind is not None and v_cache.dtype is k_cache.dtype and len(shape) == 4
+            and shape[1] == Hkv and shape[3] == hd and v_cache.shape == shape
+            and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_cache.get_device() == dev and v_cache.get_device() == dev):
+        return shape[0], shape[2], kind
+    raise ValueError(
+        f"k_cache and v_cache must be contiguous [pages, {Hkv}, page, {hd}] of torch.bfloat16 or "
+        f"torch.float8_e4m3fn on cuda:{dev}, the current device; got {k_cache.dtype} "
+        f"{tuple(shape)} {k_cache.device} and {v_cache.dtype} {tuple(v_cache.shape)} "
+        f"{v_cache.device}")
 
 
-def _half(inv_freq: torch.Tensor | None) -> int:
-    if inv_freq is None:
+def _device() -> int:
+    """The current device, whose stream the calls below use; their tensors lie on it."""
+    try:
+        return torch._C._cuda_getDevice()
+    except (AttributeError, RuntimeError):  # no GPU: the checks say so
         return 0
-    n = inv_freq.numel()
-    _check_f32(inv_freq, "inv_freq", n)
-    return n
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
@@ -383,22 +385,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     (i, i + half), interleaved (2i, 2i + 1), of the first 2 half dims; None: no rotation."""
     N, Hq, hd = q.shape
     Hkv = k.shape[1]
-    if q_out is None:
-        q_out = torch.empty(N, Hq, hd, dtype=torch.bfloat16, device=q.device)
-    if k_out is None:
-        k_out = torch.empty(N, Hkv, hd, dtype=torch.bfloat16, device=q.device)
-    _here(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
-    for t, name, shape in ((q, "q", (N, Hq, hd)), (k, "k", (N, Hkv, hd)),
-                           (q_out, "q_out", (N, Hq, hd)), (k_out, "k_out", (N, Hkv, hd))):
-        _check_rows(t, name, shape, 4)
-    _check_i32(positions, "positions", (N,))
-    half = _half(inv_freq)
-    _check_f32(q_norm, "q_norm", hd)
-    _check_f32(k_norm, "k_norm", hd)
-    _lib.call("llmy_qk_norm_rope_bf16", _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0),
-              k.stride(1), _ptr(positions), _ptr(inv_freq), half, _ptr(q_norm), _ptr(k_norm),
-              eps, int(interleaved), _ptr(q_out), q_out.stride(0), q_out.stride(1), _ptr(k_out),
-              k_out.stride(0), k_out.stride(1), N, Hq, Hkv, hd, _stream())
+    dev = _device()
+    pq, pk = _heads(q, "q", (N, Hq, hd), dev), _heads(k, "k", (N, Hkv, hd), dev)
+    pp = _vec(positions, "positions", _I32, (N,), dev)
+    half = 0 if inv_freq is None else inv_freq.numel()
+    pf = _vec(inv_freq, "inv_freq", _F32, (half,), dev)
+    wq, wk = _vec(q_norm, "q_norm", _F32, (hd,), dev), _vec(k_norm, "k_norm", _F32, (hd,), dev)
+    q_out, oq, oqr, oqh = _out_heads(q_out, "q_out", q, (N, Hq, hd), dev)
+    k_out, ok, okr, okh = _out_heads(k_out, "k_out", k, (N, Hkv, hd), dev)
+    qr, qh, _ = q.stride()
+    kr, kh, _ = k.stride()
+    _lib.call("llmy_qk_norm_rope_bf16", pq, qr, qh, pk, kr, kh, pp, pf, half, wq, wk, eps,
+              interleaved, oq, oqr, oqh, ok, okr, okh, N, Hq, Hkv, hd, _stream())
     return q_out, k_out
 
 
@@ -416,36 +414,31 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     name one slot.  With ``q`` [N,Hq,hd] its rows are normed and rotated in the same pass
     and returned (q_out)."""
     N, Hkv, hd = k.shape
-    pages, page, kind = _check_cache(k_cache, v_cache, Hkv, hd)
-    _check_rows(k, "k", (N, Hkv, hd), 4)
-    _check_rows(v, "v", (N, Hkv, hd), 4)
+    dev = _device()
+    pk, pv = _heads(k, "k", (N, Hkv, hd), dev), _heads(v, "v", (N, Hkv, hd), dev)
+    pages, page, kind = _caches(k_cache, v_cache, Hkv, hd, dev)
     if page_table.dim() != 2:
         raise ValueError("page_table must be [sequences, pages]")
     B, width = page_table.shape
     if rows is None and N > B:
         raise ValueError(f"{N} tokens and {B} page-table rows: name each token's row")
-    _check_i32(page_table, "page_table", (B, width))
-    _check_i32(positions, "positions", (N,))
-    _check_i32(rows, "rows", (N,))
-    half = _half(inv_freq)
-    _check_f32(k_norm, "k_norm", hd)
-    Hq, qs, qo = 0, (0, 0), (0, 0)
+    pt = _vec(page_table, "page_table", _I32, (B, width), dev)
+    pp, pr = _vec(positions, "positions", _I32, (N,), dev), _vec(rows, "rows", _I32, (N,), dev)
+    half = 0 if inv_freq is None else inv_freq.numel()
+    pf = _vec(inv_freq, "inv_freq", _F32, (half,), dev)
+    wk = _vec(k_norm, "k_norm", _F32, (hd,), dev)
+    Hq, pq, qr, qh, po, por, poh, wq = 0, None, 0, 0, None, 0, 0, None
     if q is not None:
         Hq = q.shape[1]
-        _check_rows(q, "q", (N, Hq, hd), 4)
-        _check_f32(q_norm, "q_norm", hd)
-        if q_out is None:
-            q_out = torch.empty(N, Hq, hd, dtype=torch.bfloat16, device=q.device)
-        _check_rows(q_out, "q_out", (N, Hq, hd), 4)
-        qs, qo = q.stride(), q_out.stride()
+        pq, wq = _heads(q, "q", (N, Hq, hd), dev), _vec(q_norm, "q_norm", _F32, (hd,), dev)
+        q_out, po, por, poh = _out_heads(q_out, "q_out", q, (N, Hq, hd), dev)
+        qr, qh, _ = q.stride()
     elif q_norm is not None or q_out is not None:
         raise ValueError("q_norm and q_out go with q")
-    _here(k, v, k_cache, v_cache, page_table, positions, rows, inv_freq, k_norm, q, q_norm, q_out)
-    _lib.call("llmy_paged_kv_append", _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
-              v.stride(1), _ptr(k_cache), _ptr(v_cache), kind, k_scale, v_scale,
-              _ptr(page_table), _ptr(rows), _ptr(positions), _ptr(inv_freq), half, _ptr(k_norm),
-              eps, int(interleaved), _ptr(q), qs[0], qs[1], _ptr(q_norm), _ptr(q_out), qo[0],
-              qo[1], N, Hq, Hkv, hd, B, width, page, pages, _stream())
+    ks, vs = k.stride(), v.stride()
+    _lib.call("llmy_paged_kv_append", pk, ks[0], ks[1], pv, vs[0], vs[1], _ptr(k_cache),
+              _ptr(v_cache), kind, k_scale, v_scale, pt, pr, pp, pf, half, wk, eps, interleaved,
+              pq, qr, qh, wq, po, por, poh, N, Hq, Hkv, hd, B, width, page, pages, _stream())
     return q_out
 
 
@@ -463,30 +456,33 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     buffer of llmy_paged_attn_workspace_bytes that no overlapping call uses."""
     B, Hq, hd = q.shape
     Hkv = k_cache.shape[1]
-    pages, page, kind = _check_cache(k_cache, v_cache, Hkv, hd)
-    _check_rows(q, "q", (B, Hq, hd), 8)
+    dev = _device()
+    pq = _heads(q, "q", (B, Hq, hd), dev)
+    pages, page, kind = _caches(k_cache, v_cache, Hkv, hd, dev)
     if page_table.dim() != 2:
         raise ValueError("page_table must be [sequences, pages]")
     width = page_table.shape[1]
-    _check_i32(page_table, "page_table", (B, width))
-    _check_i32(lengths, "lengths", (B,))
-    _check_f32(slopes, "slopes", Hq)
+    pt = _vec(page_table, "page_table", _I32, (B, width), dev)
+    pl, ps = _vec(lengths, "lengths", _I32, (B,), dev), _vec(slopes, "slopes", _F32, (Hq,), dev)
     if out is None:
-        out = torch.empty(B, Hq, hd, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous torch.bfloat16 {tuple(q.shape)}")
-    nbytes = int(_lib.load().llmy_paged_attn_workspace_bytes(B, Hq, Hkv, hd, width, page, kind))
-    if nbytes > 0 and workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    if have < nbytes:
-        raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
-    _here(q, k_cache, v_cache, page_table, lengths, slopes, out, workspace)
-    scale = hd ** -0.5 if scale is None else scale
-    _lib.call("llmy_paged_attn_decode", _ptr(q), q.stride(0), q.stride(1), _ptr(k_cache),
-              _ptr(v_cache), kind, k_scale, v_scale, _ptr(page_table), _ptr(lengths),
-              _ptr(slopes), _ptr(out), _ptr(workspace), have, B, Hq, Hkv, hd, width, page, pages,
-              window, scale, softcap, _stream())
+        out = q.new_empty((B, Hq, hd))
+        po = out.data_ptr()
+    else:
+        po = _vec(out, "out", _BF16, (B, Hq, hd), dev)
+    nbytes = _lib.load().llmy_paged_attn_workspace_bytes(B, Hq, Hkv, hd, width, page, kind)
+    pw, have = None, 0
+    if workspace is not None:
+        pw, have = _vec(workspace, "workspace", workspace.dtype, workspace.shape, dev), \
+            workspace.numel() * workspace.element_size()
+        if have < nbytes:
+            raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
+    elif nbytes > 0:
+        workspace = q.new_empty((nbytes + 1) // 2)  # bf16 words
+        pw, have = workspace.data_ptr(), nbytes
+    qs = q.stride()
+    _lib.call("llmy_paged_attn_decode", pq, qs[0], qs[1], _ptr(k_cache), _ptr(v_cache), kind,
+              k_scale, v_scale, pt, pl, ps, po, pw, have, B, Hq, Hkv, hd, width, page, pages,
+              window, hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 
 
@@ -503,25 +499,23 @@ def packed_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Returns out [N,Hq,hd] bf16; rows of no document are left as they were."""
     N, Hq, hd = q.shape
     Hkv = k.shape[1]
-    _check_rows(q, "q", (N, Hq, hd), 8)
-    _check_rows(k, "k", (N, Hkv, hd), 8)
-    _check_rows(v, "v", (N, Hkv, hd), 8)
+    dev = _device()
+    pq, pk = _heads(q, "q", (N, Hq, hd), dev), _heads(k, "k", (N, Hkv, hd), dev)
+    pv = _heads(v, "v", (N, Hkv, hd), dev)
     docs = cu_seqlens.numel() - 1
     if docs < 0:
         raise ValueError("cu_seqlens must hold at least one entry")
-    _check_i32(cu_seqlens, "cu_seqlens", (docs + 1,))
-    _check_i32(prefix, "prefix", (docs,))
-    _check_f32(slopes, "slopes", Hq)
+    pc = _vec(cu_seqlens, "cu_seqlens", _I32, (docs + 1,), dev)
+    px, ps = _vec(prefix, "prefix", _I32, (docs,), dev), _vec(slopes, "slopes", _F32, (Hq,), dev)
     if out is None:
-        out = torch.empty(N, Hq, hd, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous torch.bfloat16 {tuple(q.shape)}")
-    _here(q, k, v, cu_seqlens, prefix, slopes, out)
-    scale = hd ** -0.5 if scale is None else scale
-    _lib.call("llmy_packed_attn_prefill_bf16", _ptr(q), q.stride(0), q.stride(1), _ptr(k),
-              k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(cu_seqlens),
-              _ptr(prefix), _ptr(slopes), _ptr(out), N, docs, Hq, Hkv, hd, window, scale, softcap,
-              _stream())
+        out = q.new_empty((N, Hq, hd))
+        po = out.data_ptr()
+    else:
+        po = _vec(out, "out", _BF16, (N, Hq, hd), dev)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    _lib.call("llmy_packed_attn_prefill_bf16", pq, qs[0], qs[1], pk, ks[0], ks[1], pv, vs[0],
+              vs[1], pc, px, ps, po, N, docs, Hq, Hkv, hd, window,
+              hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 
 

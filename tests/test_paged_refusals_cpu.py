@@ -95,8 +95,9 @@ def test_workspace_sizes(lib):
     assert ws(4, 8, 4, 64, 9, 16, 0) > 0
     assert ws(4, 8, 3, 64, 9, 16, 0) == -1
     assert ws(4, 8, 4, 64, 9, 20, 0) == -1
-    # the batch and the length do not change it
-    assert ws(400, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 9, 16, 0)
+    # the length does not change it, a sequence takes one word
+    assert ws(1, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 9, 16, 0)
+    assert ws(400, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 9, 16, 0) + 399 * 4
 
 
 def test_wrappers_refuse_before_the_library():
