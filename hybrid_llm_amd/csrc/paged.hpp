@@ -20,6 +20,24 @@ inline int page_shift(int32_t page) {
   return -1;
 }
 
+// Scores: a scale of at least 0; a cap of 0 (none) or up to 1024, since the fp32 form of the
+// cap is off by 2^-23 of it, and not so small beside the scale that their ratio overflows.
+inline bool scale_ok(float scale, float softcap) {
+  const float inf = __builtin_inff();
+  return scale >= 0.f && scale < inf && softcap >= 0.f && softcap <= 1024.f &&
+         (softcap == 0.f || 4.f * scale / softcap < inf);
+}
+
+// Elements from the first to the last of strided rows [n, H, hd].
+inline int64_t rows_extent(int64_t row, int64_t head, int32_t n, int32_t H, int32_t hd) {
+  return (n - 1) * row + (H - 1) * head + hd;
+}
+
+// Whether two ranges of 16-bit words lie apart.
+inline bool apart(const uint16_t* a, int64_t na, const uint16_t* b, int64_t nb) {
+  return a + na <= b || b + nb <= a;
+}
+
 // An 8-bit cache holds x / scale; a bf16 one x itself.
 inline bool scales_ok(int32_t cache_type, float k_scale, float v_scale) {
   const float inf = __builtin_inff();

@@ -231,6 +231,7 @@ extern "C" int32_t llmy_qk_norm_rope_bf16(
   LLMY_REQUIRE(N >= 0 && Hq > 0 && Hkv > 0 && Hq <= kMaxHeads && Hkv <= kMaxHeads);
   LLMY_REQUIRE(head_dim == 64 || head_dim == 128);
   LLMY_REQUIRE(half >= 0 && half % 4 == 0 && 2 * half <= head_dim && (half == 0 || inv_freq));
+  LLMY_REQUIRE(eps >= 0.f);
   if (N == 0) return 0;
   LLMY_REQUIRE(positions && rows_ok(q, q_row, q_head, Hq, head_dim) &&
                rows_ok(k, k_row, k_head, Hkv, head_dim) &&
@@ -261,6 +262,7 @@ extern "C" int32_t llmy_paged_kv_append(
   LLMY_REQUIRE(N >= 0 && Hq >= 0 && Hkv > 0 && Hq <= kMaxHeads && Hkv <= kMaxHeads);
   LLMY_REQUIRE(head_dim == 64 || head_dim == 128);
   LLMY_REQUIRE(half >= 0 && half % 4 == 0 && 2 * half <= head_dim && (half == 0 || inv_freq));
+  LLMY_REQUIRE(eps >= 0.f);
   LLMY_REQUIRE(B >= 0 && width >= 0 && pages >= 0 && page_shift(page) > 0);
   LLMY_REQUIRE(cache_type == kCacheBf16 || cache_type == kCacheE4m3);
   LLMY_REQUIRE(scales_ok(cache_type, k_scale, v_scale));
@@ -269,6 +271,10 @@ extern "C" int32_t llmy_paged_kv_append(
                rows_ok(v, v_row, v_head, Hkv, head_dim));
   LLMY_REQUIRE((B == 0 || width == 0 || page_table) &&
                (pages == 0 || (k_cache && v_cache && aligned(k_cache, 16) && aligned(v_cache, 16))));
+  const int64_t cache_words = static_cast<int64_t>(pages) * Hkv * page * head_dim /
+                              (cache_type == kCacheE4m3 ? 2 : 1);
+  LLMY_REQUIRE(apart(static_cast<uint16_t*>(k_cache), cache_words,
+                     static_cast<uint16_t*>(v_cache), cache_words));
   LLMY_REQUIRE(aligned(q_norm, 16) && aligned(k_norm, 16));
   LLMY_REQUIRE(Hq == 0 || (rows_ok(q, q_row, q_head, Hq, head_dim) &&
                            rows_ok(q_out, qo_row, qo_head, Hq, head_dim) &&

@@ -163,6 +163,18 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(bad, hd, heads
     _ok(torch.where(hit, want.to(BF16), got), want, spread)
 
 
+@pytest.mark.parametrize("heads", [1, 8, 128])
+def test_infinite_scores_stay_with_their_rows(heads):
+    """A key of infinities makes the rows that see it NaN, in every split of the keys; rows
+    before it are those of the finite keys."""
+    _, (q, k, v) = _inputs(300, heads, 1, 64, 16)
+    k[250] = math.inf
+    got = _ops().packed_attn_prefill(q.cuda(), k.cuda(), v.cuda(), _cu([300]).cuda()).cpu()
+    want, spread = ref.packed_prefill(q[:250], k[:250], v[:250], _cu([250]))
+    _ok(got[:250], want, spread)
+    assert got[250:].isnan().all()
+
+
 def test_one_visible_key_is_returned_exactly():
     _, (q, k, v) = _inputs(77, 6, 3, 128, 8)
     got = _ops().packed_attn_prefill(q.cuda(), k.cuda(), v.cuda(), _cu([50, 27]).cuda(), window=1)

@@ -9,8 +9,8 @@ a tree of at most 12 additions and its root, weight and two products, 2^-20 of t
 value together; the angle's fraction of a turn in fp32, 2^-25 turns or 2^-22 of a
 radian, and sincospi within 2^-22.  Under 2^-19 of the row's largest value.
 
-attention: weights w_j are rounded to bf16 (2^-8 each) and divided by the sum of the
-rounded ones, so the result moves by at most 2^-8 sum_j w_j |v_j - out|.  Scores in
+attention: weights w_j are rounded to bf16 at the worst (2^-8 each) and divided by their
+sum, so the result moves by at most 2^-8 sum_j w_j |v_j - out|.  Scores in
 fp32: the products of hd <= 128 terms, sum |q_d k_d| scale <= 2^5 on these inputs, off
 by 2^-24 * 132 * 2^5 < 2^-11; exp2 and the cap add under 2^-16.  A score's error e moves a
 weight by e, twice that with the sum's: 2^-10 of the same spread.  Then one store.
@@ -364,6 +364,37 @@ def test_lengths_outside_the_table():
     got, want, spread = _decode_both(q, kc, vc, table, lens, ks, vs)
     _attn_ok(got.cpu(), want, spread)
     assert (got[0] == 0).all()
+
+
+def test_a_table_of_no_pages():
+    q = torch.ones(3, 4, 64, dtype=BF16, device="cuda")
+    c = torch.ones(2, 2, 16, 64, dtype=BF16, device="cuda")
+    table = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    lens = torch.full((3,), 9, dtype=torch.int32, device="cuda")
+    assert (_ops().paged_attn_decode(q, c, c, table, lens) == 0).all()
+    pos = torch.zeros(3, dtype=torch.int32, device="cuda")
+    before = c.clone()
+    _ops().paged_kv_append(q[:, :2], q[:, :2], c, torch.zeros_like(c), table, pos)
+    assert torch.equal(c, before)
+
+
+def test_keys_and_values_in_one_cache():
+    """One tensor as both caches is an ordinary read."""
+    g = torch.Generator().manual_seed(14)
+    q, kc, _, table, lens, ks, vs = _decode_case(2, 8, 1, 64, 16, [200, 31], False, g)
+    one = kc.cuda()
+    got = _ops().paged_attn_decode(q.cuda(), one, one, table.cuda(), lens.cuda())
+    want, spread = ref.paged_decode(q, kc, kc, table, lens)
+    _attn_ok(got.cpu(), want, spread)
+
+
+@pytest.mark.parametrize("cap", [0.01, 1024.0])
+def test_smallest_and_largest_cap(cap):
+    """The cap's own error is 2^-23 of it: a score of the largest is off by 2^-13."""
+    g = torch.Generator().manual_seed(15)
+    got, want, spread = _decode_both(*_decode_case(2, 4, 2, 64, 16, [150, 40], False, g),
+                                     softcap=cap)
+    _attn_ok(got.cpu(), want, spread)
 
 
 def test_strided_queries_and_given_buffers():
