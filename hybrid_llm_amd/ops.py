@@ -320,23 +320,15 @@ _CACHE_TYPES = {torch.bfloat16: CACHE_BF16, torch.float8_e4m3fn: CACHE_E4M3}
 # GPU at their smallest, less than checks that name each property in turn.
 
 
-def _heads(t: torch.Tensor, name: str, shape: tuple, dev: int) -> int:
-    """The address of bf16 rows [N, H, hd] on device ``dev`` whose heads' dims are
-    contiguous (the library checks the other strides)."""
-    if (t.dtype is _BF16 and t.shape == shape and t.stride(2) == 1 and t.get_device() == dev):
-        return t.data_ptr()
+def _heads(t: torch.Tensor, name: str, shape: tuple, dev: int) -> tuple:
+    """Address, row and head strides of bf16 rows [N, H, hd] on device ``dev`` whose heads'
+    dims are contiguous (the library checks the other strides)."""
+    st = t.stride()
+    if t.dtype is _BF16 and t.shape == shape and st[2] == 1 and t.get_device() == dev:
+        return t.data_ptr(), st[0], st[1]
     raise ValueError(f"{name} must be torch.bfloat16 {shape} with contiguous dims on cuda:{dev}, "
-                     f"the current device; got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, "
+                     f"the current device; got {t.dtype} {tuple(t.shape)}, strides {st}, "
                      f"{t.device}")
-
-
-def _out_heads(t: torch.Tensor | None, name: str, like: torch.Tensor, shape: tuple,
-               dev: int) -> tuple:
-    """The output, given or made, its address, row and head strides."""
-    if t is None:
-        t = like.new_empty(shape)
-        return t, t.data_ptr(), shape[1] * shape[2], shape[2]
-    return t, _heads(t, name, shape, dev), t.stride(0), t.stride(1)
 
 
 def _vec(t: torch.Tensor | None, name: str, dtype: torch.dtype, shape: tuple, dev: int):
@@ -386,15 +378,22 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     N, Hq, hd = q.shape
     Hkv = k.shape[1]
     dev = _device()
-    pq, pk = _heads(q, "q", (N, Hq, hd), dev), _heads(k, "k", (N, Hkv, hd), dev)
+    pq, qr, qh = _heads(q, "q", (N, Hq, hd), dev)
+    pk, kr, kh = _heads(k, "k", (N, Hkv, hd), dev)
     pp = _vec(positions, "positions", _I32, (N,), dev)
     half = 0 if inv_freq is None else inv_freq.numel()
     pf = _vec(inv_freq, "inv_freq", _F32, (half,), dev)
     wq, wk = _vec(q_norm, "q_norm", _F32, (hd,), dev), _vec(k_norm, "k_norm", _F32, (hd,), dev)
-    q_out, oq, oqr, oqh = _out_heads(q_out, "q_out", q, (N, Hq, hd), dev)
-    k_out, ok, okr, okh = _out_heads(k_out, "k_out", k, (N, Hkv, hd), dev)
-    qr, qh, _ = q.stride()
-    kr, kh, _ = k.stride()
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        oq, oqr, oqh = q_out.data_ptr(), Hq * hd, hd
+    else:
+        oq, oqr, oqh = _heads(q_out, "q_out", (N, Hq, hd), dev)
+    if k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        ok, okr, okh = k_out.data_ptr(), Hkv * hd, hd
+    else:
+        ok, okr, okh = _heads(k_out, "k_out", (N, Hkv, hd), dev)
     _lib.call("llmy_qk_norm_rope_bf16", pq, qr, qh, pk, kr, kh, pp, pf, half, wq, wk, eps,
               interleaved, oq, oqr, oqh, ok, okr, okh, N, Hq, Hkv, hd, _stream())
     return q_out, k_out
@@ -415,7 +414,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     and returned (q_out)."""
     N, Hkv, hd = k.shape
     dev = _device()
-    pk, pv = _heads(k, "k", (N, Hkv, hd), dev), _heads(v, "v", (N, Hkv, hd), dev)
+    pk, kr, kh = _heads(k, "k", (N, Hkv, hd), dev)
+    pv, vr, vh = _heads(v, "v", (N, Hkv, hd), dev)
     pages, page, kind = _caches(k_cache, v_cache, Hkv, hd, dev)
     if page_table.dim() != 2:
         raise ValueError("page_table must be [sequences, pages]")
@@ -430,15 +430,18 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     Hq, pq, qr, qh, po, por, poh, wq = 0, None, 0, 0, None, 0, 0, None
     if q is not None:
         Hq = q.shape[1]
-        pq, wq = _heads(q, "q", (N, Hq, hd), dev), _vec(q_norm, "q_norm", _F32, (hd,), dev)
-        q_out, po, por, poh = _out_heads(q_out, "q_out", q, (N, Hq, hd), dev)
-        qr, qh, _ = q.stride()
+        pq, qr, qh = _heads(q, "q", (N, Hq, hd), dev)
+        wq = _vec(q_norm, "q_norm", _F32, (hd,), dev)
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            po, por, poh = q_out.data_ptr(), Hq * hd, hd
+        else:
+            po, por, poh = _heads(q_out, "q_out", (N, Hq, hd), dev)
     elif q_norm is not None or q_out is not None:
         raise ValueError("q_norm and q_out go with q")
-    ks, vs = k.stride(), v.stride()
-    _lib.call("llmy_paged_kv_append", pk, ks[0], ks[1], pv, vs[0], vs[1], _ptr(k_cache),
-              _ptr(v_cache), kind, k_scale, v_scale, pt, pr, pp, pf, half, wk, eps, interleaved,
-              pq, qr, qh, wq, po, por, poh, N, Hq, Hkv, hd, B, width, page, pages, _stream())
+    _lib.call("llmy_paged_kv_append", pk, kr, kh, pv, vr, vh, k_cache.data_ptr(),
+              v_cache.data_ptr(), kind, k_scale, v_scale, pt, pr, pp, pf, half, wk, eps,
+              interleaved, pq, qr, qh, wq, po, por, poh, N, Hq, Hkv, hd, B, width, page, pages, _stream())
     return q_out
 
 
@@ -457,7 +460,7 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     B, Hq, hd = q.shape
     Hkv = k_cache.shape[1]
     dev = _device()
-    pq = _heads(q, "q", (B, Hq, hd), dev)
+    pq, qr, qh = _heads(q, "q", (B, Hq, hd), dev)
     pages, page, kind = _caches(k_cache, v_cache, Hkv, hd, dev)
     if page_table.dim() != 2:
         raise ValueError("page_table must be [sequences, pages]")
@@ -465,7 +468,7 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     pt = _vec(page_table, "page_table", _I32, (B, width), dev)
     pl, ps = _vec(lengths, "lengths", _I32, (B,), dev), _vec(slopes, "slopes", _F32, (Hq,), dev)
     if out is None:
-        out = q.new_empty((B, Hq, hd))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         po = out.data_ptr()
     else:
         po = _vec(out, "out", _BF16, (B, Hq, hd), dev)
@@ -479,8 +482,7 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     elif nbytes > 0:
         workspace = q.new_empty((nbytes + 1) // 2)  # bf16 words
         pw, have = workspace.data_ptr(), nbytes
-    qs = q.stride()
-    _lib.call("llmy_paged_attn_decode", pq, qs[0], qs[1], _ptr(k_cache), _ptr(v_cache), kind,
+    _lib.call("llmy_paged_attn_decode", pq, qr, qh, k_cache.data_ptr(), v_cache.data_ptr(), kind,
               k_scale, v_scale, pt, pl, ps, po, pw, have, B, Hq, Hkv, hd, width, page, pages,
               window, hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
@@ -500,21 +502,20 @@ def packed_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     N, Hq, hd = q.shape
     Hkv = k.shape[1]
     dev = _device()
-    pq, pk = _heads(q, "q", (N, Hq, hd), dev), _heads(k, "k", (N, Hkv, hd), dev)
-    pv = _heads(v, "v", (N, Hkv, hd), dev)
+    pq, qr, qh = _heads(q, "q", (N, Hq, hd), dev)
+    pk, kr, kh = _heads(k, "k", (N, Hkv, hd), dev)
+    pv, vr, vh = _heads(v, "v", (N, Hkv, hd), dev)
     docs = cu_seqlens.numel() - 1
     if docs < 0:
         raise ValueError("cu_seqlens must hold at least one entry")
     pc = _vec(cu_seqlens, "cu_seqlens", _I32, (docs + 1,), dev)
     px, ps = _vec(prefix, "prefix", _I32, (docs,), dev), _vec(slopes, "slopes", _F32, (Hq,), dev)
     if out is None:
-        out = q.new_empty((N, Hq, hd))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         po = out.data_ptr()
     else:
         po = _vec(out, "out", _BF16, (N, Hq, hd), dev)
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    _lib.call("llmy_packed_attn_prefill_bf16", pq, qs[0], qs[1], pk, ks[0], ks[1], pv, vs[0],
-              vs[1], pc, px, ps, po, N, docs, Hq, Hkv, hd, window,
+    _lib.call("llmy_packed_attn_prefill_bf16", pq, qr, qh, pk, kr, kh, pv, vr, vh, pc, px, ps, po, N, docs, Hq, Hkv, hd, window,
               hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 
