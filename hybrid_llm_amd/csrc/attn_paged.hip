@@ -13,17 +13,20 @@
 //     product O^T += V^T P^T under the key order 4 g + j, 16 + 4 g + j, so the
 //     weights never leave their registers; V^T comes from transposing LDS reads of
 //     row-major V rows in that order.
-//   * a wave is a workgroup and works alone: its 32-key steps arrive by DMA into 2 or
-//     3 LDS stages of its own and nothing ever waits for another wave.  Four to ten
-//     waves a CU keep 64 KiB and more in flight per CU, several times what the read
-//     rate needs to cover a load's latency.
-//   * the work is the flat list of all (sequence, key-value head, step), cut into
+//   * a wave works alone: its 32-key steps arrive by DMA into 2 or 3 LDS stages of its
+//     own and it waits for no other wave.  Four to twelve waves a CU keep 64 KiB and
+//     more in flight per CU, several times what the read rate needs to cover a load's
+//     latency.
+//   * short tables: a workgroup takes a head, its waves every fourth or eighth step, and
+//     joins their (m, l, O) in LDS.
+//   * long ones: the work is the flat list of all (sequence, key-value head, step), cut into
 //     equal runs: one run per wave, found from the lengths on the device.  A batch of
 //     any mixture of lengths is balanced, and the host never learns the lengths.  A
 //     run that starts or ends inside a head's steps leaves (m, l, O) partials in the
 //     workspace, at most two, and a second kernel joins them; a head that lies in
-//     one run is stored by that wave.  A cache too short to be cut takes one wave a
-//     head and no second launch.
+//     one run is stored by that wave.  64 sequences of up to 4096 tokens, 32 heads
+//     over 8 x 128: 97 us, 5.6 TB/s of the visible keys (all of 4096: 169 us, 6.1); four of
+//     131072 in e4m3: 179 us, 5.9.
 //   * the page ids come by scalar loads (a page holds whole 16-key tiles, so they are
 //     the same for every lane of a DMA), which leaves the vector counter to the DMAs.
 // Masked keys (past the length, before the window, in a page that the table does not
@@ -50,7 +53,6 @@ __device__ __forceinline__ int32_t scalar_at(const int32_t* p, long long i) {
 
 constexpr int kStep = 32;      // keys a step
 constexpr int kMinSteps = 1;   // least steps of a run
-constexpr int kWhole = 128;    // tokens that are not cut
 
 struct PagedArgs {
   const uint16_t* q;
@@ -64,7 +66,7 @@ struct PagedArgs {
   float scale_log2, cap_log2, cap_x2, v_scale;
   int B, hq, hkv, G, HT, GT;   // G = Hq / Hkv in HT tiles of GT <= 16 heads
   int width, shift, pages, window, cap_len;
-  int runs;                    // 0: one wave a (sequence, head tile), no join
+  int runs;
 };
 
 struct Seq {
@@ -130,15 +132,15 @@ __device__ __forceinline__ bf16x8 e4m3_to_bf16(uint32_t lo, uint32_t hi) {
 // Staged rows keep their 16-byte chunks XOR-swizzled so that the fragment reads below
 // spread over the banks: 8 lanes reading one chunk of 8 consecutive key rows, and a
 // 16-lane group reading 4 (bf16) or 8 (e4m3) key rows of one transposed V tile.
-template <int HD, bool F8>
+template <int HD, bool F8, int W>
 struct Tile {
   static constexpr int RB = HD * (F8 ? 1 : 2);       // bytes a row
   static constexpr int CH = RB / 16;                 // chunks a row
   static constexpr int RPB = 64 / CH;                // rows of one 1 KiB DMA
   static constexpr int NB = kStep / RPB;             // DMAs of a K or V tile
   static constexpr int BYTES = kStep * RB;           // of a K or V tile
-  static constexpr int STAGES = F8 || HD == 128 ? 2 : 3;
-  static constexpr int LDS = 2 * STAGES * BYTES;
+  static constexpr int STAGES = F8 || HD == 128 || W > 1 ? 2 : 3;
+  static constexpr int LDS = 2 * STAGES * BYTES;     // of a wave
   static __device__ __forceinline__ int kswz(int row) {
     return CH == 4 ? (row >> 1) & 3 : row & 7;
   }
@@ -149,16 +151,20 @@ struct Tile {
   }
 };
 
-template <int HD, bool F8>
-__global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
-  using T = Tile<HD, F8>;
+// W waves: 1: a run of the flat list; more: a head tile, each wave every W-th of its steps.
+// (Waves a SIMD: as many as paged_runs counts on; 129 registers for e4m3 of 128 dims.)
+template <int HD, bool F8, int W>
+__global__ __launch_bounds__(64 * W, W > 1 ? W / 4 : F8 ? 3 : HD == 64 ? 2 : 1)
+void paged_attn_kernel(const PagedArgs a) {
+  using T = Tile<HD, F8, W>;
   constexpr int RB = T::RB, NB = T::NB, ST = T::STAGES;
   constexpr int NS = HD / 32;                 // 32-dim slices of the score product
   constexpr int ND = HD / 16;                 // 16-dim output tiles
   constexpr int NK = F8 ? HD / 64 : HD / 32;  // 16-byte K reads of a 16-key tile
-  __shared__ __align__(1024) uint8_t smem[T::LDS];
+  __shared__ __align__(1024) uint8_t smem[W * T::LDS];
 
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int g = lane >> 4, col = lane & 15;
   const int units = a.hkv * a.HT;
 
@@ -166,17 +172,17 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
   int b, u, s, count, run_q = 0;
   long long run_at = 0;
   Seq cur;
-  if (a.runs == 0) {
+  if (W > 1) {
     b = blockIdx.x / units;
     u = blockIdx.x - b * units;
     cur = seq_of(scalar_at(a.lengths, b), a.cap_len, a.window);
-    s = cur.s0;
-    count = cur.s1 - cur.s0;
-    if (count == 0) {  // nothing visible: zeros
+    s = cur.s0 + wave;
+    count = max(0, (cur.s1 - s + W - 1) / W);
+    if (cur.s0 == cur.s1) {  // nothing visible: zeros
       const int kvh = u / a.HT, ht = u - kvh * a.HT;
       const int heads = min(16, a.G - 16 * ht);
       uint16_t* o = a.out + (static_cast<long long>(b) * a.hq + kvh * a.G + 16 * ht) * HD;
-      for (int e = 8 * lane; e < heads * HD; e += 512)
+      for (int e = 8 * threadIdx.x; e < heads * HD; e += 512 * W)
         *reinterpret_cast<uint4*>(o + e) = uint4{0u, 0u, 0u, 0u};
       return;
     }
@@ -218,12 +224,14 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     kdo[j] = (lane / T::CH) * RB + 16 * (sl ^ T::kswz(r));
     vdo[j] = (lane / T::CH) * RB + 16 * (sl ^ T::vswz(r));
   }
-  const uint32_t sbase = lds_addr(smem);
+  uint8_t* const mem = smem + wave * T::LDS;  // this wave's stages
+  const uint32_t sbase = lds_addr(mem);
   unsigned bad = 0;  // two bits a stage: its 16-key tiles whose page the table does not name
   int ib = b, iu = u, is = s;
   Seq icur = cur;
   auto next = [&](int& nb, int& nu, int& ns, Seq& q) {  // the step after; the caller counts
-    if (++ns < q.s1) return;
+    ns += W;
+    if (W > 1 || ns < q.s1) return;
     if (++nu == units) {
       nu = 0;
       do {
@@ -281,6 +289,8 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
   uint4 qf[NS];
   f32x4 acc[ND];
   float m_run = -INFINITY, l_run = 0.f, slope = 0.f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   bool fresh = true;
   int st = 0;
   for (int i = 0; i < count; ++i) {
@@ -318,7 +328,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
       for (int e = lane; e < kStep * T::CH; e += 64) {
         const int row = e / T::CH, key = key0 + row;
         if (key < cur.lo || key >= cur.len || ((hole >> (row >> 4)) & 1u))
-          *reinterpret_cast<uint4*>(smem + st * 2 * T::BYTES + T::BYTES + 16 * e) =
+          *reinterpret_cast<uint4*>(mem + st * 2 * T::BYTES + T::BYTES + 16 * e) =
               uint4{0u, 0u, 0u, 0u};
       }
       wave_lds_order();
@@ -378,16 +388,20 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = exp2_fast(z[j] - m_sub);
-    // the weights as a sum of two bf16: the matrix cores have time to spare here
-    const uint4 pb = pack8_bf16(p);
-    float hi[8];
-    unpack8(pb, hi);
+    // the weights as a sum of two bf16: the matrix cores have time to spare here.  The
+    // first is cut off below the weight, so both are positive and an infinite value
+    // stays that infinity
+    uint32_t h8[8];
+    float lo8[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       l_run += p[j];
-      hi[j] = p[j] - hi[j];
+      h8[j] = __float_as_uint(p[j] * (1.f - 0x1p-8f)) & 0xffff0000u;
+      lo8[j] = p[j] - __uint_as_float(h8[j]);
     }
-    const uint4 pl = pack8_bf16(hi);
+    const uint4 pb = uint4{h8[0] >> 16 | h8[1], h8[2] >> 16 | h8[3], h8[4] >> 16 | h8[5],
+                           h8[6] >> 16 | h8[7]};
+    const uint4 pl = pack8_bf16(lo8);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const bf16x8 vv = F8 ? e4m3_to_bf16(vf[d].x, vf[d].y)
@@ -406,7 +420,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
     st = st + 1 == ST ? 0 : st + 1;
 
     const bool head_end = s + 1 == cur.s1;
-    if (head_end || i + 1 == count) {
+    if (W == 1 && (head_end || i + 1 == count)) {
       float l = l_run + __shfl_xor(l_run, 16, kWave);
       l += __shfl_xor(l, 32, kWave);
       // whole: the head's first step lies in this run too
@@ -434,6 +448,49 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(const PagedArgs a) {
       fresh = true;
     }
     if (i + 1 < count) next(b, u, s, cur);
+  }
+  if constexpr (W > 1) {
+    // the waves' (m, l, O) joined through each one's stages, which it has done with
+    constexpr int LD = HD + 4;
+    static_assert((16 * LD + 32) * 4 <= T::LDS, "a wave's part fits its stages");
+    const int kvh = u / a.HT, ht = u - kvh * a.HT;
+    const int heads = min(16, a.G - 16 * ht);
+    float l = l_run + __shfl_xor(l_run, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+    float* const so = reinterpret_cast<float*>(mem);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<float4*>(so + col * LD + 16 * d + 4 * g) =
+          make_float4(acc[d][0], acc[d][1], acc[d][2], acc[d][3]);
+    if (g == 0) *reinterpret_cast<float2*>(so + 16 * LD + 2 * col) = make_float2(m_run, l);
+    __syncthreads();
+    uint16_t* o = a.out + (static_cast<long long>(b) * a.hq + kvh * a.G + 16 * ht) * HD;
+    for (int e = threadIdx.x; e < heads * (HD / 4); e += 64 * W) {
+      const int h = e / (HD / 4), c = 4 * (e - h * (HD / 4));
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        mx = fmaxf(mx, reinterpret_cast<const float*>(smem + w * T::LDS)[16 * LD + 2 * h]);
+      const float m_sub = mx == -INFINITY ? 0.f : mx;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float* part = reinterpret_cast<const float*>(smem + w * T::LDS);
+        const float2 ml = *reinterpret_cast<const float2*>(part + 16 * LD + 2 * h);
+        const float4 x = *reinterpret_cast<const float4*>(part + h * LD + c);
+        const float f = exp2_fast(ml.x - m_sub);
+        if (f == 0.f) continue;  // no weight beside the others
+        den = fmaf(ml.y, f, den);
+        sum.x = fmaf(x.x, f, sum.x);
+        sum.y = fmaf(x.y, f, sum.y);
+        sum.z = fmaf(x.z, f, sum.z);
+        sum.w = fmaf(x.w, f, sum.w);
+      }
+      const float r = den > 0.f || den != den ? a.v_scale / den : 0.f;
+      *reinterpret_cast<uint2*>(o + h * HD + c) =
+          make_uint2(pack_bf2(sum.x * r, sum.y * r), pack_bf2(sum.z * r, sum.w * r));
+    }
   }
 }
 
@@ -472,12 +529,14 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
     const float m_new = fmaxf(m, ml.x);
     const float m_sub = m_new == -INFINITY ? 0.f : m_new;
     const float f = exp2_fast(m - m_sub), e = exp2_fast(ml.x - m_sub);
+    m = m_new;
+    if (e == 0.f) continue;  // no weight beside the others
+    if (f == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f), l = 0.f;
     o.x = fmaf(x.x, e, o.x * f);
     o.y = fmaf(x.y, e, o.y * f);
     o.z = fmaf(x.z, e, o.z * f);
     o.w = fmaf(x.w, e, o.w * f);
     l = fmaf(ml.y, e, l * f);
-    m = m_new;
   }
   *reinterpret_cast<float4*>(&so[grp][4 * c]) = o;
   if (c == 0) {
@@ -494,6 +553,7 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const float e = exp2_fast(sm[i] - m_sub);
+      if (e == 0.f) continue;
       num = fmaf(so[i][d], e, num);
       den = fmaf(sl[i], e, den);
     }
@@ -503,15 +563,16 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
 
 // Waves that the chip holds at once: what a CU's 160 KiB of LDS take, 12 at most.
 inline int paged_runs(int head_dim, bool f8) {
-  const int lds = head_dim == 128 ? (f8 ? Tile<128, true>::LDS : Tile<128, false>::LDS)
-                                  : (f8 ? Tile<64, true>::LDS : Tile<64, false>::LDS);
+  const int lds = head_dim == 128 ? (f8 ? Tile<128, true, 1>::LDS : Tile<128, false, 1>::LDS)
+                                  : (f8 ? Tile<64, true, 1>::LDS : Tile<64, false, 1>::LDS);
   const int per_cu = (163840 - 1) / lds;  // five of 32 KiB do not fit beside each other
   return compute_units() * (per_cu < 12 ? per_cu : 12);
 }
 
 struct PagedPlan {
-  int G, HT, GT, runs;
-  long long cap_len, waves, ws;
+  int G, HT, GT, waves, runs;
+  bool wide;  // a workgroup of `waves` waves a head tile; else `runs` waves and their join
+  long long cap_len, groups, ws;
 };
 
 inline bool paged_plan(int B, int Hq, int Hkv, int hd, int width, int page, int type,
@@ -524,14 +585,41 @@ inline bool paged_plan(int B, int Hq, int Hkv, int hd, int width, int page, int 
   p->GT = p->G < 16 ? p->G : 16;
   p->cap_len = static_cast<long long>(width) * page;
   if (p->cap_len >= (1ll << 31) - kStep) return false;  // positions are 32-bit
-  const bool cut = p->cap_len > kWhole;
-  p->runs = cut ? paged_runs(hd, type == kCacheE4m3) : 0;
-  p->waves = cut ? p->runs : static_cast<long long>(B) * Hkv * p->HT;
-  p->ws = cut ? 2ll * p->runs * p->GT * (hd + 2) * 4 + (static_cast<long long>(B) + 1) * 4 : 0;
+  const long long units = static_cast<long long>(B) * Hkv * p->HT;
+  // Short tables: a head tile a workgroup, one launch.  us of it / of runs and their join,
+  // lengths near the table's unless ragged: 1 x 16 heads over 4 x 64, 256 tokens 4.3 / 8.6,
+  // 1024 8.0 / 9.4, 2048 13 / 10; 64 sequences of them, 1024 14 / 21, 2048 24 / 31 (ragged
+  // 19 / 22), 4096 ragged 33 / 34; 32 heads over 8 x 128 in e4m3, 64 x 1024 29 / 34, 2048
+  // 48 / 55 (ragged 37 / 37), in bf16, 1 x 256 6.2 / 8.8, 512 9.8 / 9.2, 64 x 512 30 / 32,
+  // 1024 49 / 52 (ragged 41 / 36).  So up to four steps a wave, and up to eight where
+  // there are many heads and eight waves.
+  const int W = p->waves = hd == 128 && type == kCacheBf16 ? 4 : 8;
+  const long long deep = (p->cap_len + kStep * W - 1) / (kStep * W);
+  p->wide = deep <= 4 || (W == 8 && deep <= 8 && 2 * units >= compute_units());
+  p->runs = p->wide ? 0 : paged_runs(hd, type == kCacheE4m3);
+  p->groups = p->wide ? units : p->runs;
+  p->ws = p->wide ? 0
+                  : 2ll * p->runs * p->GT * (hd + 2) * 4 + (static_cast<long long>(B) + 1) * 4;
   // all steps, a run's steps and the grids are 32-bit
   const double steps = static_cast<double>(B) * (p->cap_len / kStep + 1);
-  return steps < 2147483647. && p->waves < (1ll << 31) &&
+  return steps < 2147483647. && p->groups < (1ll << 31) &&
          static_cast<long long>(B) * Hq < (1ll << 31);
+}
+
+template <int HD, bool F8>
+int32_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+  constexpr int W = HD == 128 && !F8 ? 4 : 8;  // 128 KiB of stages at the most (p.waves)
+  const dim3 grid(static_cast<unsigned>(p.groups)), heads(static_cast<unsigned>(a.B) * a.hq);
+  if (p.wide) {
+    hipLaunchKernelGGL((paged_attn_kernel<HD, F8, W>), grid, dim3(64 * W), 0, s, a);
+    return launch_status();
+  }
+  hipLaunchKernelGGL((paged_attn_kernel<HD, F8, 1>), grid, dim3(64), 0, s, a);
+  if (heads.x >= 1024)
+    hipLaunchKernelGGL((paged_join_kernel<HD, 64>), heads, dim3(64), 0, s, a);
+  else
+    hipLaunchKernelGGL((paged_join_kernel<HD, 512>), heads, dim3(512), 0, s, a);
+  return launch_status();
 }
 
 }  // namespace llmy
@@ -582,18 +670,8 @@ extern "C" int32_t llmy_paged_attn_decode(
   a.cap_len = pages ? static_cast<int>(p.cap_len) : 0;
   a.runs = p.runs;
   const hipStream_t s = as_stream(stream);
-  const dim3 grid(static_cast<unsigned>(p.waves)), heads(static_cast<unsigned>(B) * Hq);
-  const bool f8 = cache_type == kCacheE4m3, many = heads.x >= 1024;
-  if (head_dim == 64) {
-    if (f8) hipLaunchKernelGGL((paged_attn_kernel<64, true>), grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<64, false>), grid, dim3(64), 0, s, a);
-    if (p.runs && many) hipLaunchKernelGGL((paged_join_kernel<64, 64>), heads, dim3(64), 0, s, a);
-    else if (p.runs) hipLaunchKernelGGL((paged_join_kernel<64, 512>), heads, dim3(512), 0, s, a);
-  } else {
-    if (f8) hipLaunchKernelGGL((paged_attn_kernel<128, true>), grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<128, false>), grid, dim3(64), 0, s, a);
-    if (p.runs && many) hipLaunchKernelGGL((paged_join_kernel<128, 64>), heads, dim3(64), 0, s, a);
-    else if (p.runs) hipLaunchKernelGGL((paged_join_kernel<128, 512>), heads, dim3(512), 0, s, a);
-  }
-  return launch_status();
+  return cache_type == kCacheE4m3
+             ? (head_dim == 64 ? launch_paged<64, true>(a, p, s) : launch_paged<128, true>(a, p, s))
+             : (head_dim == 64 ? launch_paged<64, false>(a, p, s)
+                               : launch_paged<128, false>(a, p, s));
 }

@@ -271,12 +271,43 @@ def test_decode_edges(Hq, Hkv, hd, page, fp8):
 
 
 @pytest.mark.parametrize("lens,page", [([1], 16), ([16], 16), ([100], 128), ([77, 3, 0], 64),
-                                       ([0, 0], 16)])
-def test_decode_short_tables(lens, page):
-    """Tables of at most 128 tokens: one wave a head and no second launch."""
-    g = torch.Generator().manual_seed(sum(lens))
-    got, want, spread = _decode_both(*_decode_case(len(lens), 8, 2, 64, page, lens, False, g))
+                                       ([0, 0], 16), ([512, 480, 1, 33], 16), ([1024, 1], 32),
+                                       ([1025, 1000], 16)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_short_tables(lens, page, hd, fp8):
+    """Around the table lengths up to which a workgroup takes a whole head (no second
+    launch): 512 tokens for bf16 of 128 dims, else 1024."""
+    g = torch.Generator().manual_seed(sum(lens) + hd)
+    got, want, spread = _decode_both(*_decode_case(len(lens), 8, 2, hd, page, lens, fp8, g))
     _attn_ok(got.cpu(), want, spread)
+
+
+@pytest.mark.parametrize("hd,fp8,n", [(64, False, 2048), (128, True, 2048), (64, True, 2064)])
+def test_decode_many_heads_of_short_tables(hd, fp8, n):
+    """128 heads and more: whole heads up to 2048 tokens."""
+    g = torch.Generator().manual_seed(n + hd)
+    lens = [n] + [(97 * i) % n for i in range(31)]
+    case = _decode_case(32, 4, 4, hd, 16, lens, fp8, g)
+    got, want, spread = _decode_both(*case, window=70)
+    _attn_ok(got.cpu(), want, spread)
+
+
+@pytest.mark.parametrize("lens", [[300], [5000, 40]])
+def test_visible_infinities(lens):
+    """A value of +inf, -inf or NaN that a query sees is what its dim becomes."""
+    g = torch.Generator().manual_seed(17)
+    q, kc, vc, table, n, ks, vs = _decode_case(len(lens), 8, 2, 64, 16, lens, False, g)
+    want, spread = ref.paged_decode(q, kc, vc, table, n)
+    for t, d, bad in ((7, 3, math.inf), (0, 5, -math.inf), (22, 6, math.nan), (8, 9, math.inf),
+                      (9, 9, -math.inf)):
+        vc[int(table[0, t // 16]), :, t % 16, d] = bad
+    got = _ops().paged_attn_decode(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), n.cuda()).cpu()
+    assert (got[0, :, 3] == math.inf).all() and (got[0, :, 5] == -math.inf).all()
+    assert got[0, :, 6].isnan().all() and got[0, :, 9].isnan().all()
+    for d in (3, 5, 6, 9):
+        got[0, :, d] = want[0, :, d].to(BF16)
+    _attn_ok(got, want, spread)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -517,3 +548,43 @@ def test_another_stream():
         got = _ops().paged_attn_decode(late, kd, vd, td, ld)
     s.synchronize()
     _attn_ok(got.cpu(), want, spread)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap, each with a workspace of its own, do not disturb each other."""
+    g = torch.Generator().manual_seed(18)
+    cases = [_decode_case(3, 8, 2, 128, 16, [4000, 700 + i, 90], False, g) for i in range(2)]
+    dev = [[t.cuda() for t in c[:5]] for c in cases]
+    alone = [_ops().paged_attn_decode(*d) for d in dev]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in dev]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_ops().paged_attn_decode(*dev[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in got[i])
+
+
+def test_row_offsets_past_32_bits():
+    """Rows 2^21 elements apart, the last one past 2^31."""
+    wide = torch.empty(1100, 2 ** 21, dtype=BF16, device="cuda")
+    g = torch.Generator().manual_seed(19)
+    small = torch.randn(1100, 6 * 64, generator=g).to(BF16)
+    wide[:, 64:64 + 6 * 64] = small.cuda()
+    q = wide[:, 64:64 + 256].view(1100, 4, 64)
+    k = wide[:, 320:320 + 128].view(1100, 2, 64)
+    pos = torch.arange(1100, dtype=torch.int32)
+    f = _inv_freq(64)
+    qo, ko = _ops().qk_norm_rope(q, k, pos.cuda(), f.cuda())
+    _rope_ok(qo.cpu(), ref.norm_rope(small[:, :256].view(1100, 4, 64), pos, f))
+    _rope_ok(ko.cpu(), ref.norm_rope(small[:, 256:].view(1100, 2, 64), pos, f))
+    cu = torch.tensor([0, 1040, 1100], dtype=torch.int32)
+    got = _ops().packed_attn_prefill(q, k, k, cu.cuda()).cpu()
+    want, spread = ref.packed_prefill(small[1040:, :256].view(60, 4, 64),
+                                      small[1040:, 256:].view(60, 2, 64),
+                                      small[1040:, 256:].view(60, 2, 64),
+                                      torch.tensor([0, 60], dtype=torch.int32))
+    _attn_ok(got[1040:], want, spread)

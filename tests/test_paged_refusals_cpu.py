@@ -16,7 +16,7 @@ APPEND = dict(k=FAKE, k_row=256, k_head=64, v=FAKE, v_row=256, v_head=64, kc=1 <
               qo_head=64, N=4, Hq=8, Hkv=4, hd=64, B=4, width=3, page=16, pages=12, stream=None)
 DECODE = dict(q=1 << 20, q_row=512, q_head=64, kc=FAKE, vc=FAKE, kind=0, ks=1.0, vs=1.0, table=FAKE,
               lens=FAKE, slopes=None, out=FAKE, ws=FAKE, ws_bytes=1 << 30, B=4, Hq=8, Hkv=4,
-              hd=64, width=30, page=16, pages=12, window=0, scale=0.125, cap=0.0, stream=None)
+              hd=64, width=90, page=16, pages=12, window=0, scale=0.125, cap=0.0, stream=None)
 
 PACKED = dict(q=1 << 19, q_row=512, q_head=64, k=1 << 20, k_row=256, k_head=64, v=1 << 21, v_row=256,
               v_head=64, cu=FAKE, prefix=None, slopes=None, out=1 << 22, N=100, docs=3, Hq=8,
@@ -94,13 +94,15 @@ def test_prefill_of_nothing(lib):
 
 def test_workspace_sizes(lib):
     ws = lib.llmy_paged_attn_workspace_bytes
-    assert ws(4, 8, 4, 64, 8, 16, 0) == 0          # 128 tokens: nothing is cut
-    assert ws(4, 8, 4, 64, 9, 16, 0) > 0
+    assert ws(4, 8, 4, 64, 64, 16, 0) == 0         # 1024 tokens: a workgroup a head
+    assert ws(4, 8, 4, 128, 32, 16, 0) == 0        # 512
+    assert ws(4, 8, 4, 128, 33, 16, 0) > 0
+    assert ws(4, 8, 4, 64, 65, 16, 0) > 0
     assert ws(4, 8, 3, 64, 9, 16, 0) == -1
     assert ws(4, 8, 4, 64, 9, 20, 0) == -1
     # the length does not change it, a sequence takes one word
-    assert ws(1, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 9, 16, 0)
-    assert ws(400, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 9, 16, 0) + 399 * 4
+    assert ws(1, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 65, 16, 0)
+    assert ws(400, 8, 4, 64, 900, 16, 0) == ws(1, 8, 4, 64, 65, 16, 0) + 399 * 4
 
 
 def test_wrappers_refuse_before_the_library():
