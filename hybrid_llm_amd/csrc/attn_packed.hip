@@ -63,11 +63,13 @@ struct Int {
   static constexpr int value = V;
 };
 
-enum { kPlain = 0, kCapped = 1, kBiased = 2, kBiasedCapped = 3 };
+// kBiased: a distance bias alone; kAny: with a cap or a two-way prefix
+// too, or a scale near 0
+enum { kPlain = 0, kCapped = 1, kBiased = 2, kAny = 3 };
 
 // KW: waves along the keys (1, 2 or 4); 4 / KW waves along the rows.
 template <int HD, int MODE, int KW>
-__global__ __launch_bounds__(256, (HD == 64 ? 4 : 2) / (KW == 4 ? 2 : 1))
+__global__ __launch_bounds__(256, (HD == 128 ? 2 : MODE == kAny ? 3 : 4) / (KW == 4 ? 2 : 1))
 void packed_attn_kernel(const PackedArgs a) {
   constexpr int ND = HD / 32;             // 32-dim output tiles
   constexpr int NS = HD / 16;             // 16-dim slices of the score product
@@ -148,6 +150,8 @@ void packed_attn_kernel(const PackedArgs a) {
   const float slope =
       MODE >= kBiased && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
 
+  const float ratio = MODE == kBiased ? slope / a.scale_log2 : 0.f;
+
   f32x16v acc[ND];
   float m, l;  // the exponent's offset (scaled, log2) and the sum of weights
 
@@ -227,13 +231,21 @@ void packed_attn_kernel(const PackedArgs a) {
               lds_get_tr16(va[d & 1] + off + (S + (16 * sl + 8 * e) * RB + 128 * (d >> 1)));
     // register r holds key ks + 4 half + c(r), c(r) = (r & 3) + 8 (r >> 2)
     const bool whole = ks >= ilo && ks + 32 <= ihi;
-    if (MODE >= kBiased) {
-      const float dq = static_cast<float>(qi - ks - 4 * half);
+    // No key after its row: the bias -slope (row - key) is slope c(r), the same for every
+    // lane, plus a lane's own part, which joins the offset; in units of the raw scores the
+    // first is one multiply-add by a constant
+    const float dq = static_cast<float>(qi - ks - 4 * half);
+    const float lane_bias = MODE == kBiased ? -slope * dq : 0.f;
+    if (MODE == kBiased) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(ratio, (r & 3) + 8 * (r >> 2), s[r]);
+    }
+    if (MODE == kAny) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float c = (r & 3) + 8 * (r >> 2);
-        const float z = MODE == kBiasedCapped ? softcap_log2(s[r] * a.cap_x2, a.cap_log2)
-                                              : s[r] * a.scale_log2;
+        const float z = a.cap_x2 > 0.f ? softcap_log2(s[r] * a.cap_x2, a.cap_log2)
+                                       : s[r] * a.scale_log2;
         s[r] = fmaf(-slope, fabsf(dq - c), z);
       }
     }
@@ -258,6 +270,7 @@ void packed_attn_kernel(const PackedArgs a) {
     float x = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) x = fmaxf(x, s[r]);
+    if (MODE == kBiased) x = fmaf(x, a.scale_log2, lane_bias);
     {  // the other lane half's (lanes l and l ^ 32 hold one row)
       const auto sw =
           __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -285,7 +298,8 @@ void packed_attn_kernel(const PackedArgs a) {
     for (int r = 0; r < 16; ++r) {
       if (MODE == kPlain) p[r] = exp2_fast(fmaf(s[r], a.scale_log2, -m));
       if (MODE == kCapped) p[r] = exp2_fast(softcap_log2(s[r] * a.cap_x2, a.cap_log2) - m);
-      if (MODE >= kBiased) p[r] = exp2_fast(s[r] - m);
+      if (MODE == kBiased) p[r] = exp2_fast(fmaf(s[r], a.scale_log2, lane_bias - m));
+      if (MODE == kAny) p[r] = exp2_fast(s[r] - m);
     }
     if (MODE == kCapped && !whole) {  // -inf is capped to -cap: out of the sum here
 #pragma unroll
@@ -418,18 +432,30 @@ void packed_attn_kernel(const PackedArgs a) {
     for (int i = 0; i < NO; i += 8) *reinterpret_cast<uint4*>(dst + i) = pack8_bf16(o + i);
     return;
   }
-  if (!mine) return;
+  // rows put together in LDS, so that whole ones are stored: a lane holds 4 dims of every 8
+  // (8192 rows x 16 heads x 64: 5 us of 34 less).  The barrier of the check above is
+  // behind every read of a stage, but for a second run
+  if (careful) __syncthreads();
+  constexpr int LB = RB + 16;  // bytes a row
+  uint8_t* const so = smem + 32 * LB * wave;
+  static_assert(128 * LB <= 2 * 2 * TB, "the rows fit the stages");
   const float inv = 1.0f / l_tot;
-  uint16_t* orow = a.o + (static_cast<long long>(qi) * a.hq + h) * HD;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4) {
-      const int dim = 32 * d + 8 * g4 + 4 * half;
-      *reinterpret_cast<uint2*>(orow + dim) =
+    for (int g4 = 0; g4 < 4; ++g4)
+      *reinterpret_cast<uint2*>(so + col * LB + 2 * (32 * d + 8 * g4 + 4 * half)) =
           make_uint2(pack_bf2(acc[d][4 * g4] * inv, acc[d][4 * g4 + 1] * inv),
                      pack_bf2(acc[d][4 * g4 + 2] * inv, acc[d][4 * g4 + 3] * inv));
-    }
+  wave_lds_order();
+#pragma unroll
+  for (int i = 0; i < CH / 2; ++i) {
+    const int row = (64 / CH) * i + lane / CH, c = lane % CH;
+    if ((rows >> row) & 1u)
+      *reinterpret_cast<uint4*>(
+          a.o + (static_cast<long long>(q0 + 32 * rg + row) * a.hq + h) * HD + 8 * c) =
+          *reinterpret_cast<const uint4*>(so + row * LB + 16 * c);
+  }
 }
 
 template <int HD, int MODE>
@@ -488,14 +514,14 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
   const hipStream_t st = as_stream(stream);
   // a scale of 0 would turn the masked scores' -inf into NaN in the exponent of kPlain
   const bool cap = softcap > 0.f;
-  const int mode = slopes || scale == 0.f ? (cap ? kBiasedCapped : kBiased)
-                                          : (cap ? kCapped : kPlain);
+  const int mode = scale == 0.f || (slopes && (cap || prefix || scale < 1e-6f)) ? kAny
+                   : slopes ? kBiased : cap ? kCapped : kPlain;
   const auto launch = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     return mode == kPlain    ? launch_packed<HD, kPlain>(a, st)
            : mode == kCapped ? launch_packed<HD, kCapped>(a, st)
            : mode == kBiased ? launch_packed<HD, kBiased>(a, st)
-                             : launch_packed<HD, kBiasedCapped>(a, st);
+                             : launch_packed<HD, kAny>(a, st);
   };
   return head_dim == 64 ? launch(Int<64>{}) : launch(Int<128>{});
 }
