@@ -170,6 +170,6 @@ class LlmyError(RuntimeError):
 def call(name: str, *args) -> None:
     """Call an entry point and raise LlmyError on a nonzero status
     (the reference caller's rule, sample_standalone.py:3059-3063)."""
-    code = int(getattr(load(), name)(*args))
+    code = getattr(_LIB or load(), name)(*args)
     if code != 0:
         raise LlmyError(name, code)

@@ -331,14 +331,26 @@ def _heads(t: torch.Tensor, name: str, shape: tuple, dev: int) -> tuple:
                      f"{t.device}")
 
 
-def _vec(t: torch.Tensor | None, name: str, dtype: torch.dtype, shape: tuple, dev: int):
-    """The address of a contiguous tensor on device ``dev``; None: none given."""
+def _vec(t: torch.Tensor | None, name: str, dtype: torch.dtype, n: int, dev: int):
+    """The address of n contiguous entries on device ``dev``; None: none given."""
     if t is None:
         return None
-    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+    if t.dtype is dtype and t.numel() == n and t.is_contiguous() and t.get_device() == dev:
         return t.data_ptr()
-    raise ValueError(f"{name} must be contiguous {dtype} {shape} on cuda:{dev}, the current "
+    raise ValueError(f"{name} must be {n} contiguous entries of {dtype} on cuda:{dev}, the current "
                      f"device; got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, {t.device}")
+
+
+def _out(t: torch.Tensor | None, like: torch.Tensor, dev: int) -> torch.Tensor:
+    """The output, given or made: contiguous, of the shape and type of ``like``."""
+    if t is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    if t.dtype is like.dtype and t.shape == like.shape and t.is_contiguous() \
+            and t.get_device() == dev:
+        return t
+    raise ValueError(f"out must be contiguous {like.dtype} {tuple(like.shape)} on cuda:{dev}, the "
+                     f"current device; got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, "
+                     f"{t.device}")
 
 
 def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, hd: int, dev: int) -> tuple:
@@ -380,10 +392,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     dev = _device()
     pq, qr, qh = _heads(q, "q", (N, Hq, hd), dev)
     pk, kr, kh = _heads(k, "k", (N, Hkv, hd), dev)
-    pp = _vec(positions, "positions", _I32, (N,), dev)
+    pp = _vec(positions, "positions", _I32, N, dev)
     half = 0 if inv_freq is None else inv_freq.numel()
-    pf = _vec(inv_freq, "inv_freq", _F32, (half,), dev)
-    wq, wk = _vec(q_norm, "q_norm", _F32, (hd,), dev), _vec(k_norm, "k_norm", _F32, (hd,), dev)
+    pf = _vec(inv_freq, "inv_freq", _F32, half, dev)
+    wq, wk = _vec(q_norm, "q_norm", _F32, hd, dev), _vec(k_norm, "k_norm", _F32, hd, dev)
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         oq, oqr, oqh = q_out.data_ptr(), Hq * hd, hd
@@ -422,16 +434,16 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     B, width = page_table.shape
     if rows is None and N > B:
         raise ValueError(f"{N} tokens and {B} page-table rows: name each token's row")
-    pt = _vec(page_table, "page_table", _I32, (B, width), dev)
-    pp, pr = _vec(positions, "positions", _I32, (N,), dev), _vec(rows, "rows", _I32, (N,), dev)
+    pt = _vec(page_table, "page_table", _I32, B * width, dev)
+    pp, pr = _vec(positions, "positions", _I32, N, dev), _vec(rows, "rows", _I32, N, dev)
     half = 0 if inv_freq is None else inv_freq.numel()
-    pf = _vec(inv_freq, "inv_freq", _F32, (half,), dev)
-    wk = _vec(k_norm, "k_norm", _F32, (hd,), dev)
+    pf = _vec(inv_freq, "inv_freq", _F32, half, dev)
+    wk = _vec(k_norm, "k_norm", _F32, hd, dev)
     Hq, pq, qr, qh, po, por, poh, wq = 0, None, 0, 0, None, 0, 0, None
     if q is not None:
         Hq = q.shape[1]
         pq, qr, qh = _heads(q, "q", (N, Hq, hd), dev)
-        wq = _vec(q_norm, "q_norm", _F32, (hd,), dev)
+        wq = _vec(q_norm, "q_norm", _F32, hd, dev)
         if q_out is None:
             q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             po, por, poh = q_out.data_ptr(), Hq * hd, hd
@@ -462,28 +474,24 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     dev = _device()
     pq, qr, qh = _heads(q, "q", (B, Hq, hd), dev)
     pages, page, kind = _caches(k_cache, v_cache, Hkv, hd, dev)
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [sequences, pages]")
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError(f"page_table must be [{B}, pages], got {tuple(page_table.shape)}")
     width = page_table.shape[1]
-    pt = _vec(page_table, "page_table", _I32, (B, width), dev)
-    pl, ps = _vec(lengths, "lengths", _I32, (B,), dev), _vec(slopes, "slopes", _F32, (Hq,), dev)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        po = out.data_ptr()
-    else:
-        po = _vec(out, "out", _BF16, (B, Hq, hd), dev)
+    pt = _vec(page_table, "page_table", _I32, B * width, dev)
+    pl, ps = _vec(lengths, "lengths", _I32, B, dev), _vec(slopes, "slopes", _F32, Hq, dev)
+    out = _out(out, q, dev)
     nbytes = _lib.load().llmy_paged_attn_workspace_bytes(B, Hq, Hkv, hd, width, page, kind)
     pw, have = None, 0
     if workspace is not None:
-        pw, have = _vec(workspace, "workspace", workspace.dtype, workspace.shape, dev), \
-            workspace.numel() * workspace.element_size()
+        pw = _vec(workspace, "workspace", workspace.dtype, workspace.numel(), dev)
+        have = workspace.numel() * workspace.element_size()
         if have < nbytes:
             raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
     elif nbytes > 0:
         workspace = q.new_empty((nbytes + 1) // 2)  # bf16 words
         pw, have = workspace.data_ptr(), nbytes
     _lib.call("llmy_paged_attn_decode", pq, qr, qh, k_cache.data_ptr(), v_cache.data_ptr(), kind,
-              k_scale, v_scale, pt, pl, ps, po, pw, have, B, Hq, Hkv, hd, width, page, pages,
+              k_scale, v_scale, pt, pl, ps, out.data_ptr(), pw, have, B, Hq, Hkv, hd, width, page, pages,
               window, hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 
@@ -508,14 +516,10 @@ def packed_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     docs = cu_seqlens.numel() - 1
     if docs < 0:
         raise ValueError("cu_seqlens must hold at least one entry")
-    pc = _vec(cu_seqlens, "cu_seqlens", _I32, (docs + 1,), dev)
-    px, ps = _vec(prefix, "prefix", _I32, (docs,), dev), _vec(slopes, "slopes", _F32, (Hq,), dev)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        po = out.data_ptr()
-    else:
-        po = _vec(out, "out", _BF16, (N, Hq, hd), dev)
-    _lib.call("llmy_packed_attn_prefill_bf16", pq, qr, qh, pk, kr, kh, pv, vr, vh, pc, px, ps, po, N, docs, Hq, Hkv, hd, window,
+    pc = _vec(cu_seqlens, "cu_seqlens", _I32, docs + 1, dev)
+    px, ps = _vec(prefix, "prefix", _I32, docs, dev), _vec(slopes, "slopes", _F32, Hq, dev)
+    out = _out(out, q, dev)
+    _lib.call("llmy_packed_attn_prefill_bf16", pq, qr, qh, pk, kr, kh, pv, vr, vh, pc, px, ps, out.data_ptr(), N, docs, Hq, Hkv, hd, window,
               hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 

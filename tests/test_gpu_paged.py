@@ -588,3 +588,23 @@ def test_row_offsets_past_32_bits():
                                       small[1040:, 256:].view(60, 2, 64),
                                       torch.tensor([0, 60], dtype=torch.int32))
     _attn_ok(got[1040:], want, spread)
+
+
+def test_a_later_piece_of_a_prompt():
+    """Rows appended behind a cached prefix, each as a sequence of its own over the same
+    pages, are causal attention of the whole prompt's tail."""
+    g = torch.Generator().manual_seed(20)
+    n, tail, Hq, Hkv, hd, page = 150, 37, 8, 2, 64, 16
+    q, k, v = (torch.randn(n, h, hd, generator=g).to(BF16) for h in (Hq, Hkv, Hkv))
+    table = torch.randperm(12, generator=g)[:10].view(1, 10).to(torch.int32).cuda()
+    kc = torch.zeros(12, Hkv, page, hd, dtype=BF16, device="cuda")
+    vc = torch.zeros_like(kc)
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    zero = torch.zeros_like(pos)
+    for a, b in ((0, n - tail), (n - tail, n)):
+        _ops().paged_kv_append(k[a:b].cuda(), v[a:b].cuda(), kc, vc, table, pos[a:b],
+                               rows=zero[a:b])
+    got = _ops().paged_attn_decode(q[n - tail:].cuda(), kc, vc, table.repeat(tail, 1),
+                                   pos[n - tail:] + 1)
+    want, spread = ref.packed_prefill(q, k, v, torch.tensor([0, n], dtype=torch.int32))
+    _attn_ok(got.cpu(), want[n - tail:], spread[n - tail:])
