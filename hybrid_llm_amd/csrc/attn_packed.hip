@@ -147,9 +147,10 @@ void packed_attn_kernel(const PackedArgs a) {
   const int t_lo = __builtin_amdgcn_readfirstlane(glo / PN);
   const int t_hi = __builtin_amdgcn_readfirstlane((ghi - 1) / PN);
 
-  const float slope =
-      MODE >= kBiased && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
-
+  // kBiased rounds the bias and the largest score apart: 2^-24 of the farthest row's
+  // bias, 2^31 at the most, stays inside the exponent's range
+  const float slope = MODE >= kBiased && a.slopes
+      ? slope_log2(a.slopes[h], fminf(kMaxSlope, 0x1p31f / a.N)) : 0.f;
   const float ratio = MODE == kBiased ? slope / a.scale_log2 : 0.f;
 
   f32x16v acc[ND];

@@ -52,7 +52,6 @@ __device__ __forceinline__ int32_t scalar_at(const int32_t* p, long long i) {
 }
 
 constexpr int kStep = 32;      // keys a step
-constexpr int kMinSteps = 1;   // least steps of a run
 
 struct PagedArgs {
   const uint16_t* q;
@@ -111,7 +110,7 @@ __device__ __forceinline__ StepScan scan_steps(const PagedArgs& a, int lane) {
 
 __device__ __forceinline__ int run_steps(long long total, int runs) {
   const long long q = (total + runs - 1) / runs;
-  return static_cast<int>(q > kMinSteps ? q : kMinSteps);
+  return static_cast<int>(q > 1 ? q : 1);
 }
 
 template <int N>
@@ -203,7 +202,8 @@ void paged_attn_kernel(const PagedArgs a) {
     run_at = static_cast<long long>(blockIdx.x) * run_q;
     if (run_at >= total) return;
     count = static_cast<int>(min(static_cast<long long>(run_q), total - run_at));
-    const int blk = __ffsll(static_cast<unsigned long long>(__ballot(static_cast<long long>(sc.upto) * units > run_at))) - 1;
+    const uint64_t past = __ballot(static_cast<long long>(sc.upto) * units > run_at);
+    const int blk = __ffsll(static_cast<unsigned long long>(past)) - 1;
     long long at = __builtin_amdgcn_readlane(sc.before, blk);
     b = blk * sc.per;
     for (;; ++b) {  // ends: the block's sum passes run_at
@@ -305,7 +305,7 @@ void paged_attn_kernel(const PagedArgs a) {
         const int d0 = F8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
         qf[t] = *reinterpret_cast<const uint4*>(qp + d0);
       }
-      if (a.slopes) slope = a.slopes[h0 + min(col, heads - 1)] * 1.4426950408889634f;
+      if (a.slopes) slope = slope_log2(a.slopes[h0 + min(col, heads - 1)], kMaxSlope);
       m_run = -INFINITY;
       l_run = 0.f;
 #pragma unroll
@@ -602,7 +602,8 @@ inline bool paged_plan(int B, int Hq, int Hkv, int hd, int width, int page, int 
                   : 2ll * p->runs * p->GT * (hd + 2) * 4 + (static_cast<long long>(B) + 1) * 4;
   // all steps, a run's steps and the grids are 32-bit
   const double steps = static_cast<double>(B) * (p->cap_len / kStep + 1);
-  return steps < 2147483647. && p->groups < (1ll << 31) &&
+  return steps < 2147483647. &&
+         (p->wide || steps * Hkv * p->HT / p->runs < 2147483647.) && p->groups < (1ll << 31) &&
          static_cast<long long>(B) * Hq < (1ll << 31);
 }
 

@@ -28,6 +28,14 @@ inline bool scale_ok(float scale, float softcap) {
          (softcap == 0.f || 4.f * scale / softcap < inf);
 }
 
+// A distance bias a position, in log2 units.  Cut off at kMaxSlope, where a neighbour's
+// weight is e^-1024: a larger one times a distance could pass fp32, and 0 times it is NaN.
+constexpr float kMaxSlope = 1024.f;
+
+__device__ __forceinline__ float slope_log2(float slope, float most) {
+  return (fabsf(slope) > most ? copysignf(most, slope) : slope) * 1.4426950408889634f;
+}
+
 // Elements from the first to the last of strided rows [n, H, hd].
 inline int64_t rows_extent(int64_t row, int64_t head, int32_t n, int32_t H, int32_t hd) {
   return (n - 1) * row + (H - 1) * head + hd;

@@ -453,7 +453,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
         raise ValueError("q_norm and q_out go with q")
     _lib.call("llmy_paged_kv_append", pk, kr, kh, pv, vr, vh, k_cache.data_ptr(),
               v_cache.data_ptr(), kind, k_scale, v_scale, pt, pr, pp, pf, half, wk, eps,
-              interleaved, pq, qr, qh, wq, po, por, poh, N, Hq, Hkv, hd, B, width, page, pages, _stream())
+              interleaved, pq, qr, qh, wq, po, por, poh, N, Hq, Hkv, hd, B, width, page, pages,
+              _stream())
     return q_out
 
 
@@ -466,7 +467,7 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     """One new token per sequence, q [B,Hq,hd] bf16, over the first lengths[b] (int32)
     positions of page_table[b] in the caches [pages,Hkv,page,hd] (see
     llmy_paged_attn_decode): scores scale q.k, capped to softcap tanh(z / softcap), less
-    slopes[h] (fp32 [Hq]) a position of distance, over the last ``window`` positions (0:
+    slopes[h] (fp32 [Hq], cut off at 1024) a position of distance, over the last ``window`` positions (0:
     all).  Returns out [B,Hq,hd] bf16, zeros where nothing is visible.  ``workspace``: a
     buffer of llmy_paged_attn_workspace_bytes that no overlapping call uses."""
     B, Hq, hd = q.shape
@@ -491,8 +492,8 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         workspace = q.new_empty((nbytes + 1) // 2)  # bf16 words
         pw, have = workspace.data_ptr(), nbytes
     _lib.call("llmy_paged_attn_decode", pq, qr, qh, k_cache.data_ptr(), v_cache.data_ptr(), kind,
-              k_scale, v_scale, pt, pl, ps, out.data_ptr(), pw, have, B, Hq, Hkv, hd, width, page, pages,
-              window, hd ** -0.5 if scale is None else scale, softcap, _stream())
+              k_scale, v_scale, pt, pl, ps, out.data_ptr(), pw, have, B, Hq, Hkv, hd, width, page,
+              pages, window, hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 
 
@@ -519,8 +520,8 @@ def packed_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     pc = _vec(cu_seqlens, "cu_seqlens", _I32, docs + 1, dev)
     px, ps = _vec(prefix, "prefix", _I32, docs, dev), _vec(slopes, "slopes", _F32, Hq, dev)
     out = _out(out, q, dev)
-    _lib.call("llmy_packed_attn_prefill_bf16", pq, qr, qh, pk, kr, kh, pv, vr, vh, pc, px, ps, out.data_ptr(), N, docs, Hq, Hkv, hd, window,
-              hd ** -0.5 if scale is None else scale, softcap, _stream())
+    _lib.call("llmy_packed_attn_prefill_bf16", pq, qr, qh, pk, kr, kh, pv, vr, vh, pc, px, ps,
+              out.data_ptr(), N, docs, Hq, Hkv, hd, window, hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
 
 

@@ -188,14 +188,15 @@ int32_t llmy_banded_attn_decode_parts_bf16(const float* parts, int32_t nparts,
  * A paged cache is [pages, Hkv, page, head_dim], page 16, 32, 64, 128 or 256 tokens;
  * position p of a sequence is slot p % page of page page_table[row][p / page]
  * (page_table [B, width] int32).  cache_type 0: bf16; 1: OCP e4m3, standing for the
- * value times k_scale or v_scale (> 0; both 1 for bf16).  Page ids outside [0, pages) name no page. */
+ * value times k_scale or v_scale (> 0; both 1 for bf16).  Page ids outside [0, pages)
+ * name no page. */
 
 /* Per-head RMSNorm and position rotation of q [N, Hq, head_dim] and k [N, Hkv,
  * head_dim] in one pass: y = x rsqrt(mean(x^2) + eps) norm (q_norm / k_norm [head_dim]
  * fp32, NULL: no norm), then for the pairs (i, i + half) -- interleaved: (2i, 2i + 1) --
  * of the first 2 half dims (y_a cos t - y_b sin t, y_b cos t + y_a sin t) with
- * t = positions[n] * inv_freq[i] (fp32 [half]; the product in 64 bits), rounded once.  eps >= 0.
- * half % 4 == 0, 2 half <= head_dim; half 0: norm only.  A row of negative position is
+ * t = positions[n] * inv_freq[i] (fp32 [half]; the product in 64 bits), rounded once.
+ * eps >= 0, half % 4 == 0, 2 half <= head_dim; half 0: norm only.  A row of negative position is
  * padding: its outputs stay as they were.  Outputs may be the inputs themselves (same
  * pointer and strides).  Rows 8-byte aligned, strides multiples of 4, norms 16-byte
  * aligned. */
@@ -213,9 +214,9 @@ int32_t llmy_qk_norm_rope_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head
  * row n).  A token whose position is negative or past width * page, whose row is
  * outside [0, B) or whose page is named by no entry is not stored.  e4m3 stores
  * x / scale, saturated at 448, to nearest even.  The caches must not overlap; two tokens of
- * one call must not name one slot.  With Hq > 0 the tokens' queries are normed and rotated in the same pass
- * into q_out (negative positions: left as they were); q, q_norm, q_out NULL with
- * Hq 0. */
+ * one call must not name one slot.  With Hq > 0 the tokens' queries are normed and
+ * rotated in the same pass into q_out (negative positions: left as they were); q, q_norm,
+ * q_out NULL with Hq 0. */
 int32_t llmy_paged_kv_append(const llmy_bf16* k, int64_t k_row, int64_t k_head,
                              const llmy_bf16* v, int64_t v_row, int64_t v_head, void* k_cache,
                              void* v_cache, int32_t cache_type, float k_scale, float v_scale,
@@ -238,7 +239,7 @@ int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int3
  *   z_j = scale q . k_j; softcap c > 0: c tanh(z_j / c); slopes [Hq] or NULL:
  *   z_j -= slopes[h] (len - 1 - j); out = sum_j softmax(z)_j v_j
  * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
- * zeros where there is none.  Lengths below 0 count as 0, past width * page as that.
+ * zeros where there is none.  Slopes past +-1024 count as +-1024.  Lengths below 0 count as 0, past width * page as that.
  * What the other slots of a page hold, NaN included, has no effect.  out [B, Hq,
  * head_dim] bf16, not within the range of q.  scale >= 0, softcap <= 1024.  fp32 scores
  * and sums; weights as two bf16 in their product. */
@@ -258,9 +259,10 @@ int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head
  * with i - j < window).  Scores as in llmy_paged_attn_decode with slopes[h] |i - j|.
  * q [N, Hq, head_dim], k, v [N, Hkv, head_dim] strided rows (strides multiples of 8,
  * 16-byte aligned, k and v rows under 2^22 apart); out [N, Hq, head_dim] bf16, which
- * must not overlap the range of q, k or v.  Rows of no document stay as they were, and what they or
- * other unseen rows hold, NaN included, has no effect.  scale >= 0, softcap <= 1024.  fp32
- * scores and sums; weights rounded to bf16 for the product and its sum. */
+ * must not overlap the range of q, k or v.  Rows of no document stay as they were, and
+ * what they or other unseen rows hold, NaN included, has no effect.  scale >= 0, softcap
+ * <= 1024; slopes past +-1024, or past 2^31 / N, count as that.  fp32 scores and sums;
+ * weights rounded to bf16 for the product and its sum. */
 int32_t llmy_packed_attn_prefill_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                       const llmy_bf16* k, int64_t k_row, int64_t k_head,
                                       const llmy_bf16* v, int64_t v_row, int64_t v_head,

@@ -97,7 +97,7 @@ def test_longer_prompt(hd):
 @pytest.mark.parametrize("kw", [{}, {"softcap": 10.0}, {"slopes": True, "window": 150},
                                 {"prefix": [100, 0, 150, 9, 400, 1]}], ids=str)
 def test_many_heads(kw, hd):
-    """Enough rows and heads for workgroups of 128 rows (fewer give 32-row ones)."""
+    """Enough rows and heads for workgroups of 64 rows (fewer give 32-row ones)."""
     g, (q, k, v) = _inputs(640, 64, 2, hd, 4)
     kw = dict(kw)
     if kw.pop("slopes", False):
@@ -105,6 +105,49 @@ def test_many_heads(kw, hd):
     if "prefix" in kw:
         kw["prefix"] = torch.tensor(kw["prefix"], dtype=torch.int32)
     _ok(*_both(q, k, v, _cu([130, 1, 200, 0, 290, 19]), **kw))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kw", [
+    {}, {"softcap": 10.0}, {"slopes": True}, {"slopes": True, "window": 150},
+    {"prefix": [100, 0, 150, 9, 400]}, {"window": 33},
+    {"slopes": True, "softcap": 8.0, "prefix": [3, 1, 650, 0, 7]}], ids=str)
+def test_rows_and_heads_for_whole_workgroups(kw, hd):
+    """Over two 128-row workgroups a compute unit, each wave takes its rows alone; rows
+    past the last document are left."""
+    g, (q, k, v) = _inputs(1170, 64, 2, hd, 14)
+    kw = dict(kw)
+    if kw.pop("slopes", False):
+        kw["slopes"] = torch.rand(64, generator=g) * 0.1
+    if "prefix" in kw:
+        kw["prefix"] = torch.tensor(kw["prefix"], dtype=torch.int32)
+    cu = _cu([130, 1, 700, 0, 290])
+    dev = {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
+    out = torch.full((1170, 64, hd), 9.0, dtype=BF16, device="cuda")
+    _ops().packed_attn_prefill(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), out=out, **dev)
+    heads = [0, 31, 32, 63]
+    if "slopes" in kw:
+        kw["slopes"] = kw["slopes"][heads]
+    want, spread = ref.packed_prefill(q[:1121, heads], k[:1121], v[:1121], cu, **kw)
+    _ok(out[:1121, heads].cpu(), want, spread)
+    assert (out[1121:] == 9.0).all()
+
+
+@pytest.mark.parametrize("heads", [8, 256])
+@pytest.mark.parametrize("kw", [{}, {"softcap": 20.0}, {"prefix": [40, 0]}], ids=str)
+def test_largest_slopes(kw, heads):
+    """Past 1024 they count as 1024: one key is left, the nearest or the farthest one."""
+    _, (q, k, v) = _inputs(300, heads, 2, 64, 15)
+    top = torch.finfo(torch.float32).max
+    slopes = torch.tensor([top, -top, 1e7, -1e7, 2048.0, -2000.0, 500.0, -0.25])
+    kw = {n: torch.tensor(x, dtype=torch.int32) if n == "prefix" else x for n, x in kw.items()}
+    cu = _cu([290, 10])
+    got = _ops().packed_attn_prefill(
+        q.cuda(), k.cuda(), v.cuda(), cu.cuda(), slopes=slopes.repeat(heads // 8).cuda(),
+        **{n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}).cpu()
+    at = list(range(4)) + list(range(heads - 4, heads))  # four heads of either key-value head
+    want, spread = ref.packed_prefill(q[:, at], k, v, cu, slopes=slopes.clamp(-1024, 1024), **kw)
+    _ok(got[:, at], want, spread)
 
 
 def test_more_documents_than_fit_the_table():
@@ -163,7 +206,12 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(bad, hd, heads
     _ok(torch.where(hit, want.to(BF16), got), want, spread)
 
 
-@pytest.mark.parametrize("heads", [1, 8, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_that_are_not_finite_in_whole_workgroups(bad):
+    test_values_that_are_not_finite_reach_only_rows_that_see_them(bad, 64, 300)
+
+
+@pytest.mark.parametrize("heads", [1, 8, 128, 180])
 def test_infinite_scores_stay_with_their_rows(heads):
     """A key of infinities makes the rows that see it NaN, in every split of the keys; rows
     before it are those of the finite keys."""
@@ -186,8 +234,8 @@ def test_nothing_to_do():
     out = torch.full((9, 2, 64), 3.0, dtype=BF16, device="cuda")
     zero = torch.zeros(1, dtype=torch.int32, device="cuda")
     _ops().packed_attn_prefill(q.cuda(), k.cuda(), v.cuda(), zero, out=out)
-    _ops().packed_attn_prefill(q.cuda(), k.cuda(), v.cuda(), torch.zeros(4, dtype=torch.int32).cuda(),
-                               out=out)
+    _ops().packed_attn_prefill(q.cuda(), k.cuda(), v.cuda(),
+                               torch.zeros(4, dtype=torch.int32).cuda(), out=out)
     assert (out == 3.0).all()
     e = q[:0].cuda()
     assert _ops().packed_attn_prefill(e, e, e, zero).shape == (0, 2, 64)

@@ -326,6 +326,18 @@ def test_decode_options(kw, hd, fp8):
     _attn_ok(got.cpu(), want, spread)
 
 
+@pytest.mark.parametrize("lens", [[300, 17], [5000, 40]])
+def test_decode_largest_slopes(lens):
+    """Past 1024 they count as 1024: one key is left, the nearest or the farthest one."""
+    g = torch.Generator().manual_seed(18)
+    case = _decode_case(2, 8, 2, 64, 16, lens, False, g)
+    top = torch.finfo(torch.float32).max
+    slopes = torch.tensor([top, -top, 1e7, -1e7, 2048.0, -2000.0, 500.0, -0.25])
+    got, _, _ = _decode_both(*case, slopes=slopes)
+    want, spread = ref.paged_decode(*case[:5], slopes=slopes.clamp(-1024, 1024))
+    _attn_ok(got.cpu(), want, spread)
+
+
 @pytest.mark.parametrize("B,lens", [
     (1, [20000]),                            # one sequence over many runs
     (3, [9000, 5, 6100]),                    # runs that end in one head and start in the next
