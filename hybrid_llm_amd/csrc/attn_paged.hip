@@ -25,7 +25,7 @@
 //     run that starts or ends inside a head's steps leaves (m, l, O) partials in the
 //     workspace, at most two, and a second kernel joins them; a head that lies in
 //     one run is stored by that wave.  64 sequences of up to 4096 tokens, 32 heads
-//     over 8 x 128: 97 us, 5.6 TB/s of the visible keys (all of 4096: 169 us, 6.1); four of
+//     over 8 x 128: 95-100 us, 5.6 TB/s of the visible keys (all of 4096: 169 us, 6.1); four of
 //     131072 in e4m3: 179 us, 5.9.
 //   * the page ids come by scalar loads (a page holds whole 16-key tiles, so they are
 //     the same for every lane of a DMA), which leaves the vector counter to the DMAs.
