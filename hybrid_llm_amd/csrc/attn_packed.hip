@@ -496,7 +496,7 @@ extern "C" int32_t llmy_packed_attn_prefill_bf16(
   LLMY_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16));
   for (const int64_t x : {q_row, q_head, k_row, k_head, v_row, v_head})
     LLMY_REQUIRE(x >= 0 && x % 8 == 0);
-  LLMY_REQUIRE(k_row < (1 << 22) && v_row < (1 << 22));  // 64-row offsets are 32-bit
+  LLMY_REQUIRE(k_row < (1 << 22) && v_row < (1 << 22));  // a tile's offsets are 32-bit
   // out is written while other workgroups still read
   const int64_t out_n = static_cast<int64_t>(N) * Hq * head_dim;
   LLMY_REQUIRE(apart(q, rows_extent(q_row, q_head, N, Hq, head_dim), out, out_n) &&
