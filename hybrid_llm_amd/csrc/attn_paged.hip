@@ -480,8 +480,8 @@ void paged_attn_kernel(const PagedArgs a) {
         const float2 ml = *reinterpret_cast<const float2*>(part + 16 * LD + 2 * h);
         const float4 x = *reinterpret_cast<const float4*>(part + h * LD + c);
         const float f = exp2_fast(ml.x - m_sub);
-        if (f == 0.f) continue;  // no weight beside the others
-        den = fmaf(ml.y, f, den);
+        den = fmaf(ml.y, f, den);  // NaN of a NaN score, whatever its part's weight
+        if (f == 0.f) continue;    // no weight beside the others
         sum.x = fmaf(x.x, f, sum.x);
         sum.y = fmaf(x.y, f, sum.y);
         sum.z = fmaf(x.z, f, sum.z);
@@ -496,8 +496,11 @@ void paged_attn_kernel(const PagedArgs a) {
 
 // Joins the partials of one (sequence, query head): o = sum_i 2^(m_i - m) O_i /
 // sum_i 2^(m_i - m) l_i, in the runs' order within each of T / (HD / 4) lane groups and
-// then over the groups, so the result does not depend on timing.  T threads: 64 where
-// the heads alone fill the chip, 512 where few heads have many partials each.
+// then over the groups, so the result does not depend on timing.  A part without weight adds
+// nothing to O, whose values may be infinite, but adds its l, which is finite or, of a
+// visible NaN score (no maximum sees one), NaN: then the row is NaN, however its head was
+// cut.  T threads: 64 where the heads alone fill the chip, 512 where few heads have many
+// partials each.
 template <int HD, int T>
 __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
   constexpr int LPP = HD / 4;       // lanes a partial
@@ -530,13 +533,13 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
     const float m_sub = m_new == -INFINITY ? 0.f : m_new;
     const float f = exp2_fast(m - m_sub), e = exp2_fast(ml.x - m_sub);
     m = m_new;
-    if (e == 0.f) continue;  // no weight beside the others
-    if (f == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f), l = 0.f;
+    l = fmaf(ml.y, e, l * f);  // NaN of a NaN score, whatever its part's weight
+    if (e == 0.f) continue;    // no weight beside the others
+    if (f == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
     o.x = fmaf(x.x, e, o.x * f);
     o.y = fmaf(x.y, e, o.y * f);
     o.z = fmaf(x.z, e, o.z * f);
     o.w = fmaf(x.w, e, o.w * f);
-    l = fmaf(ml.y, e, l * f);
   }
   *reinterpret_cast<float4*>(&so[grp][4 * c]) = o;
   if (c == 0) {
@@ -553,9 +556,9 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const float e = exp2_fast(sm[i] - m_sub);
+      den = fmaf(sl[i], e, den);
       if (e == 0.f) continue;
       num = fmaf(so[i][d], e, num);
-      den = fmaf(sl[i], e, den);
     }
     out[d] = f2bf(den > 0.f || den != den ? num * (a.v_scale / den) : 0.f);
   }
