@@ -414,8 +414,11 @@ void packed_attn_kernel(const PackedArgs a) {
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
       const float e = exp2_fast(sm[at + 32 * w] - mx);
-      if (e == 0.f) continue;  // no weight: its infinities, which the others have too, add NaN
+      // the sum of a part without weight is finite or, of a visible NaN score alone (no
+      // maximum sees one), NaN, and then the row's is; its infinities, which the others
+      // have too, would add NaN
       den = fmaf(sl[at + 32 * w], e, den);
+      if (e == 0.f) continue;
 #pragma unroll
       for (int i = 0; i < NO; i += 4) {
         const float4 v = *reinterpret_cast<const float4*>(so + (at + 32 * w) * LD + c0 + i);
