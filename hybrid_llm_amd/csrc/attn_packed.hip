@@ -272,15 +272,16 @@ void packed_attn_kernel(const PackedArgs a) {
 #pragma unroll
     for (int r = 1; r < 16; ++r) x = fmaxf(x, s[r]);
     if (MODE == kBiased) x = fmaf(x, a.scale_log2, lane_bias);
+    // the cap ascends, so the largest score is the largest capped one.  A visible -inf is
+    // capped to -cap, so whether there is a score says the mask (bits c(r)), not the value
+    if (MODE == kCapped)
+      x = seen & 0x0f0f0f0fu ? softcap_log2(x * a.cap_x2, a.cap_log2) : -INFINITY;
     {  // the other lane half's (lanes l and l ^ 32 hold one row)
       const auto sw =
           __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
       x = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     }
-    // the cap ascends, so the largest score is the largest capped one
     if (MODE == kPlain) x *= a.scale_log2;
-    if (MODE == kCapped)
-      x = x == -INFINITY ? x : softcap_log2(x * a.cap_x2, a.cap_log2);
     // the offset moves when some row's largest score passes it by 8 (log2), decided by
     // the wave, so most sub-tiles rescale nothing
     if (__ballot(x - 8.f > m)) {

@@ -56,3 +56,23 @@ def test_a_nan_key_that_a_window_begins_on(heads):
     want, spread = ref.packed_prefill(q[:, some], k, v, _cu([300]), window=25)
     _ok(got[:95, some], want[:95], spread[:95])
     _ok(got[120:, some], want[120:], spread[120:])
+
+
+# ------------------------------------------------------------------ a cap and infinite scores
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1000.0])
+@pytest.mark.parametrize("keys", [(0, 300), (0, 70), (40, 41), (64, 200)], ids=str)
+def test_capped_scores_of_minus_infinity(keys, cap, hd, heads):
+    """They are -cap: alone they weigh alike, beside others e^-cap.  Capped scores are off by
+    2^-23 of the cap and 2^-11, a weight by e^(2 of that) - 1."""
+    _, (q, k, v) = _inputs(300, heads, 1, hd, 18)
+    q[..., 0] = q[..., 0].abs() + 0.125
+    k[keys[0]:keys[1], :, 0] = -math.inf
+    cu = _cu([250, 50])
+    got = _prompt(q, k, v, cu, softcap=cap)
+    some = [0, heads // 2, heads - 1]
+    want, spread = ref.packed_prefill(q[:, some], k, v, cu, softcap=cap)
+    assert bool(want.isfinite().all())
+    # the oracle's own capped -inf scores weigh alike exactly, and so do the kernel's
+    _ok(got[:, some], want, spread)
