@@ -30,6 +30,13 @@
 // masked sub-tile): a workgroup that ends with an output that is not finite runs once
 // more, with such values zeroed in masked sub-tiles and given to the rows that do see
 // them at the end.
+//
+// An exponent s scale - m is one multiply-add, its product not rounded, while m is the
+// rounded product of the largest score: the weights are off by one factor 2^d, |d| half a
+// step of m.  It leaves with the division by their sum, as long as it stays inside the
+// exponent's range: d is 8 at most where |m| < 2^28.  A workgroup with an m past that
+// runs the second time too, which rounds the products first (a multiply a score, 2% of a
+// long prompt's time if all took it).
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "attn_tile.hpp"
@@ -40,6 +47,11 @@ namespace llmy {
 typedef float f32x16v __attribute__((ext_vector_type(16)));
 
 constexpr int kDocsInLds = 511;
+
+// A row's offset before its first score: every finite score reaches it.
+constexpr float kNoScore = -3.402823466e38f;
+// From here on (log2 units) a workgroup runs its second time: see below.
+constexpr float kFar = 0x1p28f;
 
 struct PackedArgs {
   const uint16_t *q, *k, *v;
@@ -208,6 +220,7 @@ void packed_attn_kernel(const PackedArgs a) {
     }
   }
   bool careful = false;  // the second run: see the top
+  float factor = a.scale_log2;  // of the scores that meet the offset; 1 in the second run
   auto sub_tile = [&](auto subc, int ks, uint32_t off) __attribute__((always_inline)) {
     constexpr int S = decltype(subc)::value * 32 * RB;
     if (ks >= whi || ks + 32 <= wlo) return;  // no row of this wave sees it
@@ -236,7 +249,7 @@ void packed_attn_kernel(const PackedArgs a) {
     // lane, plus a lane's own part, which joins the offset; in units of the raw scores the
     // first is one multiply-add by a constant
     const float dq = static_cast<float>(qi - ks - 4 * half);
-    const float lane_bias = MODE == kBiased ? -slope * dq : 0.f;
+    float lane_bias = MODE == kBiased ? -slope * dq : 0.f;
     if (MODE == kBiased) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = fmaf(ratio, (r & 3) + 8 * (r >> 2), s[r]);
@@ -268,10 +281,15 @@ void packed_attn_kernel(const PackedArgs a) {
             (&vf[0][0][0])[i][e] &= ~not_finite((&vf[0][0][0])[i][e]);
       }
     }
+    if ((MODE == kPlain || MODE == kBiased) && careful) {  // the products, rounded
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], a.scale_log2, lane_bias);
+      lane_bias = 0.f;
+    }
     float x = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) x = fmaxf(x, s[r]);
-    if (MODE == kBiased) x = fmaf(x, a.scale_log2, lane_bias);
+    if (MODE == kBiased) x = fmaf(x, factor, lane_bias);
     // the cap ascends, so the largest score is the largest capped one.  A visible -inf is
     // capped to -cap, so whether there is a score says the mask (bits c(r)), not the value
     if (MODE == kCapped)
@@ -281,7 +299,7 @@ void packed_attn_kernel(const PackedArgs a) {
           __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
       x = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     }
-    if (MODE == kPlain) x *= a.scale_log2;
+    if (MODE == kPlain) x *= factor;
     // the offset moves when some row's largest score passes it by 8 (log2), decided by
     // the wave, so most sub-tiles rescale nothing
     if (__ballot(x - 8.f > m)) {
@@ -298,9 +316,9 @@ void packed_attn_kernel(const PackedArgs a) {
     float p[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      if (MODE == kPlain) p[r] = exp2_fast(fmaf(s[r], a.scale_log2, -m));
+      if (MODE == kPlain) p[r] = exp2_fast(fmaf(s[r], factor, -m));
       if (MODE == kCapped) p[r] = exp2_fast(softcap_log2(s[r] * a.cap_x2, a.cap_log2) - m);
-      if (MODE == kBiased) p[r] = exp2_fast(fmaf(s[r], a.scale_log2, lane_bias - m));
+      if (MODE == kBiased) p[r] = exp2_fast(fmaf(s[r], factor, lane_bias - m));
       if (MODE == kAny) p[r] = exp2_fast(s[r] - m);
     }
     if (MODE == kCapped && !whole) {  // -inf is capped to -cap: out of the sum here
@@ -325,7 +343,7 @@ void packed_attn_kernel(const PackedArgs a) {
   };
 
   for (;;) {
-    m = -1e38f;
+    m = kNoScore;
     l = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -354,8 +372,11 @@ void packed_attn_kernel(const PackedArgs a) {
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) bad = fmaf(acc[d][r], 0.f, bad);
-    if (!__syncthreads_or(mine && bad != 0.f)) break;  // NaN: some value is not finite
+    // NaN: some value is not finite, or a weight overflowed
+    const bool far = (MODE == kPlain || MODE == kBiased) && m != kNoScore && !(fabsf(m) < kFar);
+    if (!__syncthreads_or(mine && (bad != 0.f || far))) break;
     careful = true;
+    factor = 1.f;
   }
   if (careful) {
     // the values left out, straight from memory: this lane's dims 8 e + 4 half .. + 3 of
