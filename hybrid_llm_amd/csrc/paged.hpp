@@ -20,11 +20,12 @@ inline int page_shift(int32_t page) {
   return -1;
 }
 
-// Scores: a scale of at least 0; a cap of 0 (none) or up to 1024, since the fp32 form of the
-// cap is off by 2^-23 of it, and not so small beside the scale that their ratio overflows.
+// Scores: a scale of at least 0 that is finite in log2 units too; a cap of 0 (none) or up to
+// 1024, since the fp32 form of the cap is off by 2^-23 of it, and not so small beside the
+// scale that their ratio overflows.
 inline bool scale_ok(float scale, float softcap) {
   const float inf = __builtin_inff();
-  return scale >= 0.f && scale < inf && softcap >= 0.f && softcap <= 1024.f &&
+  return scale >= 0.f && scale * 1.4426950408889634f < inf && softcap >= 0.f && softcap <= 1024.f &&
          (softcap == 0.f || 4.f * scale / softcap < inf);
 }
 
@@ -46,11 +47,12 @@ inline bool apart(const uint16_t* a, int64_t na, const uint16_t* b, int64_t nb) 
   return a + na <= b || b + nb <= a;
 }
 
-// An 8-bit cache holds x / scale; a bf16 one x itself.
+// An 8-bit cache holds x / scale, a bf16 one x itself.  From 2^-100 to 2^100 a scale's
+// reciprocal, its quotients' remainders and its share of a sum are ordinary fp32 numbers;
+// the reciprocal of one below 2^-128 is infinite, and 0 times that is NaN.
 inline bool scales_ok(int32_t cache_type, float k_scale, float v_scale) {
-  const float inf = __builtin_inff();
-  return cache_type == kCacheBf16 ? k_scale == 1.f && v_scale == 1.f
-                                  : k_scale > 0.f && v_scale > 0.f && k_scale < inf && v_scale < inf;
+  const auto ok = [](float s) { return s >= 0x1p-100f && s <= 0x1p100f; };
+  return cache_type == kCacheBf16 ? k_scale == 1.f && v_scale == 1.f : ok(k_scale) && ok(v_scale);
 }
 
 }  // namespace llmy

@@ -188,8 +188,8 @@ int32_t llmy_banded_attn_decode_parts_bf16(const float* parts, int32_t nparts,
  * A paged cache is [pages, Hkv, page, head_dim], page 16, 32, 64, 128 or 256 tokens;
  * position p of a sequence is slot p % page of page page_table[row][p / page]
  * (page_table [B, width] int32).  cache_type 0: bf16; 1: OCP e4m3, standing for the
- * value times k_scale or v_scale (> 0; both 1 for bf16).  Page ids outside [0, pages)
- * name no page. */
+ * value times k_scale or v_scale (2^-100 to 2^100; both 1 for bf16).  Page ids outside
+ * [0, pages) name no page. */
 
 /* Per-head RMSNorm and position rotation of q [N, Hq, head_dim] and k [N, Hkv,
  * head_dim] in one pass: y = x rsqrt(mean(x^2) + eps) norm (q_norm / k_norm [head_dim]
@@ -241,7 +241,8 @@ int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int3
  * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
  * zeros where there is none.  Slopes past +-1024 count as +-1024.  Lengths below 0 count as 0, past width * page as that.
  * What the other slots of a page hold, NaN included, has no effect.  out [B, Hq,
- * head_dim] bf16, not within the range of q.  scale >= 0, softcap <= 1024.  fp32 scores
+ * head_dim] bf16, not within the range of q.  scale >= 0, finite with k_scale and log2(e);
+ * softcap <= 1024.  fp32 scores
  * and sums; weights as two bf16 in their product. */
 int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                const void* k_cache, const void* v_cache, int32_t cache_type,
