@@ -67,6 +67,25 @@ __device__ __forceinline__ uint32_t pack4_e4m3(const float* v, float scale, floa
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], r, true));
 }
 
+// The mean square of a row, of which this lane has y.
+template <int HD>
+__device__ __forceinline__ float mean_square(const float* y) {
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+  ss += dpp_f<kDppXor1>(ss);
+  ss += dpp_f<kDppXor2>(ss);
+  ss += dpp_f<kDppHalfMirror>(ss);
+  if (HD == 128) ss += dpp_f<kDppMirror>(ss);
+  return ss * (1.f / HD);
+}
+
+// Below this mean square the squares may have lost bits to fp32's end; such rows, all under
+// 2^-41, are raised so that bf16's smallest squares to a normal number.  Rows whose
+// squares overflowed reach past 2^60 and are lowered; what that takes below the
+// smallest normal is under 2^-100 of the row.
+constexpr float kLeastMean = 0x1p-90f, kRaise = 0x1p100f, kLower = 0x1p-70f;
+
 template <int HD, int IT, bool CACHE, bool F8>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
   constexpr int LPR = HD / 8;   // lanes a row
@@ -129,6 +148,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
     *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(&trig[wave][1][4 * c]);
   }
 
+  const bool normed = a.w[0] || a.w[1];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const int r = first + i * RPI + g;
@@ -138,16 +158,19 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
     unpack4(x0[i], y);
     unpack4(x1[i], y + 4);
     const float* w = kind == 0 ? a.w[0] : kind == 1 ? a.w[1] : nullptr;
-    float ss = 0.f;
+    float mean = mean_square<HD>(y) + a.eps;
+    // rows whose squares overflow, or vanish with an eps that does too: times a power of
+    // two, which the norm takes out (1 for the other rows of such a wave)
+    const bool odd = w && r < a.heads && !(mean >= kLeastMean && mean < INFINITY);
+    if (normed && __ballot(odd)) {
+      const float by = !odd ? 1.f : mean < 1.f ? kRaise : kLower;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
-    ss += dpp_f<kDppXor1>(ss);
-    ss += dpp_f<kDppXor2>(ss);
-    ss += dpp_f<kDppHalfMirror>(ss);
-    if (LPR == 16) ss += dpp_f<kDppMirror>(ss);
+      for (int j = 0; j < 8; ++j) y[j] *= by;
+      mean = mean_square<HD>(y) + a.eps * by * by;
+    }
     if (r >= a.heads) continue;
     if (w) {
-      const float rs = rsqrtf(ss * (1.f / HD) + a.eps);
+      const float rs = rsqrtf(mean);
       const float4 w0 = *reinterpret_cast<const float4*>(w + d0);
       const float4 w1 = *reinterpret_cast<const float4*>(w + d1);
       y[0] *= rs * w0.x; y[1] *= rs * w0.y; y[2] *= rs * w0.z; y[3] *= rs * w0.w;
