@@ -42,6 +42,84 @@ inline int64_t rows_extent(int64_t row, int64_t head, int32_t n, int32_t H, int3
   return (n - 1) * row + (H - 1) * head + hd;
 }
 
+// Strided rows of 16-bit words [n, H, hd], whose memory may interleave with other rows' (the
+// q and k of a fused projection), so that only an exact look tells whether they meet.
+struct Rows {
+  const void* p;
+  int64_t row, head;  // strides, in elements
+  int32_t n, H, hd;
+
+  // Elements to the end of the last; a double, since strides are any 63-bit number.
+  double extent() const {
+    return static_cast<double>(n - 1) * row + static_cast<double>(H - 1) * head + hd;
+  }
+  bool same(const Rows& o) const {
+    return p == o.p && (n == 1 || row == o.row) && (H == 1 || head == o.head);
+  }
+};
+
+// Whether the blocks of hd elements at d + i r, -n < i < n, miss the one at 0 (i = 0 left
+// out where `others`).
+inline bool misses(int64_t d, int64_t r, int32_t n, int32_t hd, bool others = false) {
+  const auto miss = [&](int64_t i) {
+    const int64_t at = d + i * r;
+    return i <= -n || i >= n || (others && i == 0) || at >= hd || at <= -hd;
+  };
+  // the blocks next to 0, among them the nearest
+  const int64_t most = n - 1, i = r == 0 ? 0 : -d / r < -most ? -most : -d / r > most ? most : -d / r;
+  return miss(i - 1) && miss(i) && miss(i + 1);
+}
+
+constexpr double kMaxExtent = 0x1p52;  // past any memory; the sums below stay exact
+
+// Whether no block of one is touched by a block of the other, of as many rows.
+inline bool rows_apart(const Rows& a, const Rows& b) {
+  if (a.extent() > kMaxExtent || b.extent() > kMaxExtent) return false;
+  const int64_t ea = static_cast<int64_t>(a.extent()), eb = static_cast<int64_t>(b.extent());
+  const int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p) -
+                                         reinterpret_cast<uintptr_t>(a.p)) / 2;
+  if (d >= ea || d <= -eb) return true;
+  const int64_t r = a.n == 1 ? 0 : a.row;
+  if (a.n > 1 && a.row != b.row) return false;  // entwined at two pitches: not looked into
+  const int64_t sa = (a.H - 1) * a.head + a.hd, sb = (b.H - 1) * b.head + b.hd;
+  if (r > 0 && sa <= r && sb <= r) {  // beside each other in one wider row
+    const int64_t at = (d % r + r) % r;
+    if (at >= sa && at + sb <= r) return true;
+  }
+  if (a.H == 1 || b.H == 1 || a.head == b.head) {
+    const int64_t s = a.H == 1 ? b.head : a.head;
+    for (int64_t h = 1 - a.H; h < b.H; ++h)
+      if (!misses(d + h * s, r, a.n, a.hd)) return false;
+    return true;
+  }
+  for (int64_t i = 0; i < a.H; ++i)
+    for (int64_t j = 0; j < b.H; ++j)
+      if (!misses(d + j * b.head - i * a.head, r, a.n, a.hd)) return false;
+  return true;
+}
+
+// Whether no two blocks of rows that are written share an element.
+inline bool rows_apart(const Rows& a) {
+  if (a.extent() > kMaxExtent) return false;
+  const int64_t r = a.n == 1 ? 0 : a.row;
+  if (a.n > 1 && !misses(0, r, a.n, a.hd, true)) return false;
+  if ((a.H - 1) * a.head + a.hd <= r || (a.H > 1 && (a.n - 1) * r + a.hd <= a.head)) return true;
+  for (int64_t h = 1; h < a.H; ++h)
+    if (!misses(h * a.head, r, a.n, a.hd)) return false;
+  return true;
+}
+
+// Whether strided rows lie apart from a range of bytes.
+inline bool rows_apart(const Rows& a, const void* p, int64_t bytes) {
+  const double x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(p);
+  return bytes == 0 || y + bytes <= x || y >= x + 2. * a.extent();
+}
+
+// Rows written in place of others are exactly those, or apart from them.
+inline bool in_place_or_apart(const Rows& out, const Rows& in) {
+  return out.same(in) || rows_apart(out, in);
+}
+
 // Whether two ranges of 16-bit words lie apart.
 inline bool apart(const uint16_t* a, int64_t na, const uint16_t* b, int64_t nb) {
   return a + na <= b || b + nb <= a;

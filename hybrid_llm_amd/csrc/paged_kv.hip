@@ -268,7 +268,12 @@ extern "C" int32_t llmy_qk_norm_rope_bf16(
                rows_ok(q_out, qo_row, qo_head, Hq, head_dim) &&
                rows_ok(k_out, ko_row, ko_head, Hkv, head_dim));
   LLMY_REQUIRE(aligned(q_norm, 16) && aligned(k_norm, 16));
-  LLMY_REQUIRE(N == 1 || (qo_row >= head_dim && ko_row >= head_dim));  // rows written apart
+  // rows are written while other waves still read theirs
+  const Rows qi{q, q_row, q_head, N, Hq, head_dim}, ki{k, k_row, k_head, N, Hkv, head_dim},
+      qo{q_out, qo_row, qo_head, N, Hq, head_dim}, ko{k_out, ko_row, ko_head, N, Hkv, head_dim};
+  LLMY_REQUIRE(rows_apart(qo) && rows_apart(ko) && rows_apart(qo, ko) &&
+               in_place_or_apart(qo, qi) && in_place_or_apart(ko, ki) && rows_apart(qo, ki) &&
+               rows_apart(ko, qi));
   RopeArgs a{};
   a.x[0] = q; a.xr[0] = q_row; a.xh[0] = q_head;
   a.x[1] = k; a.xr[1] = k_row; a.xh[1] = k_head;
@@ -306,9 +311,18 @@ extern "C" int32_t llmy_paged_kv_append(
   LLMY_REQUIRE(apart(static_cast<uint16_t*>(k_cache), cache_words,
                      static_cast<uint16_t*>(v_cache), cache_words));
   LLMY_REQUIRE(aligned(q_norm, 16) && aligned(k_norm, 16));
-  LLMY_REQUIRE(Hq == 0 || (rows_ok(q, q_row, q_head, Hq, head_dim) &&
-                           rows_ok(q_out, qo_row, qo_head, Hq, head_dim) &&
-                           (N == 1 || qo_row >= head_dim)));
+  if (Hq > 0) {
+    LLMY_REQUIRE(rows_ok(q, q_row, q_head, Hq, head_dim) &&
+                 rows_ok(q_out, qo_row, qo_head, Hq, head_dim));
+    // rows are written while other waves still read theirs
+    const Rows qo{q_out, qo_row, qo_head, N, Hq, head_dim};
+    LLMY_REQUIRE(rows_apart(qo) &&
+                 in_place_or_apart(qo, Rows{q, q_row, q_head, N, Hq, head_dim}) &&
+                 rows_apart(qo, Rows{k, k_row, k_head, N, Hkv, head_dim}) &&
+                 rows_apart(qo, Rows{v, v_row, v_head, N, Hkv, head_dim}) &&
+                 rows_apart(qo, k_cache, 2 * cache_words) &&
+                 rows_apart(qo, v_cache, 2 * cache_words));
+  }
   RopeArgs a{};
   a.x[0] = q; a.xr[0] = q_row; a.xh[0] = q_head;
   a.x[1] = k; a.xr[1] = k_row; a.xh[1] = k_head;

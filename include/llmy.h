@@ -197,9 +197,10 @@ int32_t llmy_banded_attn_decode_parts_bf16(const float* parts, int32_t nparts,
  * of the first 2 half dims (y_a cos t - y_b sin t, y_b cos t + y_a sin t) with
  * t = positions[n] * inv_freq[i] (fp32 [half]; the product in 64 bits), rounded once.
  * eps >= 0, half % 4 == 0, 2 half <= head_dim; half 0: norm only.  A row of negative position is
- * padding: its outputs stay as they were.  Outputs may be the inputs themselves (same
- * pointer and strides).  Rows 8-byte aligned, strides multiples of 4, norms 16-byte
- * aligned. */
+ * padding: its outputs stay as they were.  An output may be its own input (same pointer and
+ * strides); else no row of it may touch a row of q, k or the other output (rows that
+ * interleave with theirs may, at one row stride), and no two of its rows touch.  Rows
+ * 8-byte aligned, strides multiples of 4, norms 16-byte aligned. */
 int32_t llmy_qk_norm_rope_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                const llmy_bf16* k, int64_t k_row, int64_t k_head,
                                const int32_t* positions, const float* inv_freq, int32_t half,
@@ -213,10 +214,10 @@ int32_t llmy_qk_norm_rope_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head
  * paged cache: token n goes to position positions[n] of page-table row rows[n] (NULL:
  * row n).  A token whose position is negative or past width * page, whose row is
  * outside [0, B) or whose page is named by no entry is not stored.  e4m3 stores
- * x / scale, saturated at 448, to nearest even.  The caches must not overlap; two tokens of
- * one call must not name one slot.  With Hq > 0 the tokens' queries are normed and
- * rotated in the same pass into q_out (negative positions: left as they were); q, q_norm,
- * q_out NULL with Hq 0. */
+ * x / scale in fp32, saturated at 448, to nearest even.  The caches must not overlap; two
+ * tokens of one call must not name one slot, nor k and v lie in slots that it writes.  With Hq > 0 the tokens' queries are normed and
+ * rotated in the same pass into q_out (negative positions: left as they were; q itself or
+ * apart from q, k, v and the caches, as above); q, q_norm, q_out NULL with Hq 0. */
 int32_t llmy_paged_kv_append(const llmy_bf16* k, int64_t k_row, int64_t k_head,
                              const llmy_bf16* v, int64_t v_row, int64_t v_head, void* k_cache,
                              void* v_cache, int32_t cache_type, float k_scale, float v_scale,
