@@ -656,6 +656,16 @@ extern "C" int32_t llmy_paged_attn_decode(
   // with no page at all every length counts as 0
   LLMY_REQUIRE(pages == 0 || (k_cache && v_cache && aligned(k_cache, 16) && aligned(v_cache, 16)));
   LLMY_REQUIRE(p.ws == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= p.ws));
+  // out and the workspace are written while other workgroups still read
+  const int64_t out_bytes = 2ll * B * Hq * head_dim;
+  const int64_t cache_bytes = static_cast<int64_t>(pages) * Hkv * page * head_dim *
+                              (cache_type == kCacheE4m3 ? 1 : 2);
+  LLMY_REQUIRE(bytes_apart(out, out_bytes, k_cache, cache_bytes) &&
+               bytes_apart(out, out_bytes, v_cache, cache_bytes) &&
+               bytes_apart(workspace, p.ws, k_cache, cache_bytes) &&
+               bytes_apart(workspace, p.ws, v_cache, cache_bytes) &&
+               bytes_apart(workspace, p.ws, out, out_bytes) &&
+               rows_apart(Rows{q, q_row, q_head, B, Hq, head_dim}, workspace, p.ws));
   PagedArgs a{};
   a.q = q; a.qb = q_row; a.qh = q_head;
   a.kc = static_cast<const uint8_t*>(k_cache);

@@ -109,6 +109,12 @@ inline bool rows_apart(const Rows& a) {
   return true;
 }
 
+// Whether two ranges of bytes lie apart; an empty one always does.
+inline bool bytes_apart(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na == 0 || nb == 0 || x + na <= y || y + nb <= x;
+}
+
 // Whether strided rows lie apart from a range of bytes.
 inline bool rows_apart(const Rows& a, const void* p, int64_t bytes) {
   const double x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(p);

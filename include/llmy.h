@@ -241,10 +241,10 @@ int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int3
  *   z_j -= slopes[h] (len - 1 - j); out = sum_j softmax(z)_j v_j
  * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
  * zeros where there is none.  Slopes past +-1024 count as +-1024.  Lengths below 0 count as 0, past width * page as that.
- * What the other slots of a page hold, NaN included, has no effect.  out [B, Hq,
- * head_dim] bf16, not within the range of q.  scale >= 0, finite with k_scale and log2(e);
- * softcap <= 1024.  fp32 scores
- * and sums; weights as two bf16 in their product. */
+ * What the other slots of a page hold, NaN included, has no effect; a NaN score makes its
+ * row NaN.  out [B, Hq, head_dim] bf16.  out and the workspace lie apart from each other,
+ * from q and from the caches.  scale >= 0, finite times k_scale and log2(e); softcap <=
+ * 1024.  fp32 scores and sums; weights as two bf16 in their product. */
 int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                const void* k_cache, const void* v_cache, int32_t cache_type,
                                float k_scale, float v_scale, const int32_t* page_table,
