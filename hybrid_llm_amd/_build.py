@@ -42,12 +42,11 @@ def sources() -> list[Path]:
     return sorted(list(CSRC.glob("*.hip")) + list(CSRC.glob("*.cpp")))
 
 
-# Per-source additions.  attn_prefill, attn_packed: the output accumulators are
-# rescaled by VALU between MFMAs, so they stay in VGPRs (the default AGPR form moves
-# every one out and back; measured 12% faster, same results).
+# Per-source additions.  attn_prefill: the output accumulators are rescaled by
+# VALU between MFMAs, so they stay in VGPRs (the default AGPR form moves every
+# one out and back; measured 12% faster, same results).
 FILE_FLAGS = {
     "attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-    "attn_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 
