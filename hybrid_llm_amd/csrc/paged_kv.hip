@@ -221,8 +221,10 @@ int32_t launch_norm_rope(RopeArgs a, int head_dim, hipStream_t s) {
   const int rpi = 512 / head_dim;
   // Four iterations a wave read at the rate of a copy (16384 tokens x 40 rows of 128: 65 us,
   // 5.2 TB/s; one iteration 91 us), one spreads a small call over more waves (1003 x 18: 4.8
-  // us against 5.2; 8191 x 4 into an e4m3 cache: 6.3 against 6.9; but 4096 x 20 rows of 64: 8.3
-  // against 7.0).
+  // us against 5.2) and leaves none of a token's last wave idle, since a wave stays with
+  // its token (8191 x 4 into an e4m3 cache, 12 of 16 row slots empty: 6.3 against 6.9); but
+  // 4096 x 20 rows of 64: 8.3 against 7.0.  The border lies somewhere between 33 and 82
+  // thousand rows; nothing in between was measured, nor rows of both widths at one size.
   const int it = static_cast<long long>(a.N) * a.heads >= 65536 ? 4 : 1;
   a.chunks = (a.heads + it * rpi - 1) / (it * rpi);
   const long long wgs = (static_cast<long long>(a.N) * a.chunks + 3) / 4;

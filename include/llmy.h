@@ -263,8 +263,8 @@ int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head
  * 16-byte aligned, k and v rows under 2^22 apart); out [N, Hq, head_dim] bf16, which
  * must not overlap the range of q, k or v.  Rows of no document stay as they were, and
  * what they or other unseen rows hold, NaN included, has no effect.  scale >= 0, softcap
- * <= 1024; slopes past +-1024, or past 2^31 / N, count as that.  fp32 scores and sums;
- * weights rounded to bf16 for the product and its sum. */
+ * <= 1024, the scale finite times log2(e); slopes past +-1024, or past 2^31 / N, count as
+ * that.  fp32 scores and sums; weights rounded to bf16 for the product and its sum. */
 int32_t llmy_packed_attn_prefill_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                       const llmy_bf16* k, int64_t k_row, int64_t k_head,
                                       const llmy_bf16* v, int64_t v_row, int64_t v_head,
