@@ -52,6 +52,7 @@ __device__ __forceinline__ int32_t scalar_at(const int32_t* p, long long i) {
 }
 
 constexpr int kStep = 32;      // keys a step
+constexpr float kLowest = -3.402823466e38f;
 
 struct PagedArgs {
   const uint16_t* q;
@@ -361,7 +362,13 @@ void paged_attn_kernel(const PagedArgs a) {
       }
     }
     float z[8];
-    float mloc = -INFINITY;
+    // a step with a visible key lifts the maximum to the lowest finite number, also if they
+    // all score -inf: softmax over such alone is NaN, over no key it gives zeros
+    const auto shows = [&](int h) {
+      const int first = key0 + 16 * h;
+      return !((hole >> h) & 1u) && max(first, cur.lo) < min(first + 16, cur.len);
+    };
+    float mloc = !edge || shows(0) || shows(1) ? kLowest : -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float x = sc[j >> 2][j & 3];
@@ -426,7 +433,7 @@ void paged_attn_kernel(const PagedArgs a) {
       // whole: the head's first step lies in this run too
       const bool whole = head_end && i >= s - cur.s0;
       if (whole) {
-        const float f = l > 0.f || l != l ? a.v_scale / l : 0.f;
+        const float f = m_run == -INFINITY && l == 0.f ? 0.f : a.v_scale / l;
         uint16_t* o = a.out + (static_cast<long long>(b) * a.hq + h0 + col) * HD + 4 * g;
         if (col < heads)
 #pragma unroll
@@ -487,7 +494,7 @@ void paged_attn_kernel(const PagedArgs a) {
         sum.z = fmaf(x.z, f, sum.z);
         sum.w = fmaf(x.w, f, sum.w);
       }
-      const float r = den > 0.f || den != den ? a.v_scale / den : 0.f;
+      const float r = mx == -INFINITY && den == 0.f ? 0.f : a.v_scale / den;
       *reinterpret_cast<uint2*>(o + h * HD + c) =
           make_uint2(pack_bf2(sum.x * r, sum.y * r), pack_bf2(sum.z * r, sum.w * r));
     }
@@ -560,7 +567,7 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
       if (e == 0.f) continue;
       num = fmaf(so[i][d], e, num);
     }
-    out[d] = f2bf(den > 0.f || den != den ? num * (a.v_scale / den) : 0.f);
+    out[d] = f2bf(mx == -INFINITY && den == 0.f ? 0.f : num * (a.v_scale / den));
   }
 }
 

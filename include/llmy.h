@@ -242,7 +242,7 @@ int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int3
  * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
  * zeros where there is none.  Slopes past +-1024 count as +-1024.  Lengths below 0 count as 0, past width * page as that.
  * What the other slots of a page hold, NaN included, has no effect; a NaN score makes its
- * row NaN.  out [B, Hq, head_dim] bf16.  out and the workspace lie apart from each other,
+ * row NaN, and so do scores that are -inf throughout.  out [B, Hq, head_dim] bf16.  out and the workspace lie apart from each other,
  * from q and from the caches.  scale >= 0, finite times k_scale and log2(e); softcap <=
  * 1024.  fp32 scores and sums; weights as two bf16 in their product. */
 int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head,

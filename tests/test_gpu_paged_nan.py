@@ -70,3 +70,32 @@ def test_a_nan_key_beside_far_larger_scores(pos, heads):
     got = _step(case[0], kc, *case[2:], scale=64.0)
     assert got[0, :heads // 2].isnan().all()
     assert not got[0, heads // 2:].isnan().any() and not got[1].isnan().any()
+
+
+@pytest.mark.parametrize("longest", TABLES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("keys", ["all", "but the last", "a whole step"])
+def test_scores_of_minus_infinity(keys, hd, longest):
+    """Beside a finite score they have no weight; alone their softmax is 0 / 0, as in a prompt's
+    rows, where a sequence without a visible key gives zeros."""
+    g = torch.Generator().manual_seed(hd + longest)
+    q, kc, vc, table, lens, ks, vs = _decode_case(4, 8, 2, hd, 16, [77, longest, 0, 90], False, g)
+    table[3] = -1
+    q[..., 0] = q[..., 0].abs() + 0.125
+    for t in range(77):
+        if keys == "all" or keys == "but the last" and t < 76 or keys == "a whole step" and t < 32:
+            kc[int(table[0, t // 16]), 1, t % 16, 0] = -math.inf
+    want, spread = ref.paged_decode(q, kc, vc, table, lens)
+    got = _step(q, kc, vc, table, lens, ks, vs)
+    assert bool(want[0, 4:].isnan().all()) == (keys == "all")
+    assert bool((got[2:] == 0).all())
+    if keys == "all":
+        assert got[0, 4:].isnan().all()
+        prompt = _ops().packed_attn_prefill(
+            q[:1].cuda(), kc[int(table[0, 0]), :, :1].transpose(0, 1).cuda(),
+            torch.ones(1, 2, hd, dtype=q.dtype).cuda(),
+            torch.tensor([0, 1], dtype=torch.int32).cuda()).cpu()
+        assert prompt[0, 4:].isnan().all() and not prompt[0, :4].isnan().any()
+        got[0, 4:] = 0
+        want[0, 4:] = spread[0, 4:] = 0
+    _attn_ok(got, want, spread)
