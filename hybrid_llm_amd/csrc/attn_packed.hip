@@ -26,11 +26,11 @@
 // Blocks run from the last rows to the first, the longest ones of a document first; the
 // query heads of a key-value head run side by side on one XCD and share its L2.
 //
-// What a masked place holds, NaN and infinities included, must reach no row, and 0 * inf
-// is NaN in the product.  The values are not looked at as they pass (96 instructions a
-// masked sub-tile): a workgroup that ends with an output that is not finite runs once
-// more, with such values zeroed in masked sub-tiles and given to the rows that do see
-// them at the end.
+// What a masked place holds, NaN and infinities included, must reach no row, what a visible
+// one holds every row that sees it, however small its weight, and 0 * inf is NaN in the
+// product.  The values are not looked at as they pass (96 instructions a sub-tile): a
+// workgroup that ends with an output that is not finite runs once more, with such values
+// zeroed and given to the rows that see them at the end.
 //
 // An exponent s scale - m is one multiply-add, its product not rounded, while m is the
 // rounded product of the largest score: the weights are off by one factor 2^d, |d| half a
@@ -274,13 +274,13 @@ void packed_attn_kernel(const PackedArgs a) {
         const uint32_t v = __builtin_amdgcn_sbfe(seen, (r & 3) + 8 * (r >> 2), 1);
         s[r] = __uint_as_float((v & __float_as_uint(s[r])) | (~v & 0xff800000u));  // else -inf
       }
-      if (careful) {
+    }
+    if (careful) {
 #pragma unroll
-        for (int i = 0; i < 4 * ND; ++i)
+      for (int i = 0; i < 4 * ND; ++i)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            (&vf[0][0][0])[i][e] &= ~not_finite((&vf[0][0][0])[i][e]);
-      }
+        for (int e = 0; e < 2; ++e)
+          (&vf[0][0][0])[i][e] &= ~not_finite((&vf[0][0][0])[i][e]);
     }
     if ((MODE == kPlain || MODE == kBiased) && careful) {  // the products, rounded
 #pragma unroll
@@ -384,7 +384,7 @@ void packed_attn_kernel(const PackedArgs a) {
   }
   if (careful) {
     // the values left out, straight from memory: this lane's dims 8 e + 4 half .. + 3 of
-    // every key that its row sees (one that was added before adds nothing new: inf + inf)
+    // every key that its row sees
     for (int key = wlo; key < whi; key += 4) {
 #pragma unroll
       for (int e = 0; e < 4 * ND; ++e) {
