@@ -114,6 +114,18 @@ __device__ __forceinline__ int run_steps(long long total, int runs) {
   return static_cast<int>(q > 1 ? q : 1);
 }
 
+// What turns a row's sum of weighted values into its output: scale / sum of weights; without
+// a visible key (m -inf) 0, with only scores of -inf NaN.
+__device__ __forceinline__ float share(float m, float l, float scale) {
+  return l != 0.f ? scale / l : m == -INFINITY ? 0.f : NAN;
+}
+
+// A part's sum under its weight beside the others, which may have vanished: infinities and
+// NaN, those of visible values, stay all the same.
+__device__ __forceinline__ float weighted(float x, float f) {
+  return f != 0.f ? x * f : fabsf(x) < INFINITY ? 0.f : x;
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -292,6 +304,46 @@ void paged_attn_kernel(const PagedArgs a) {
   float m_run = -INFINITY, l_run = 0.f, slope = 0.f;
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // After a part, the steps from `from` to `to` of a head: a visible value that is not finite
+  // is what its dim becomes for every head, but left NaN there under a weight that had
+  // vanished.  Seen by the sums, then looked up in memory, but for rows that are NaN as a
+  // whole (l, their sum of weights).  (e4m3 has no infinities.)
+  auto settle = [&](int from, int to, float l) __attribute__((always_inline)) {
+    if (F8) return;
+    float bad = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bad = fmaf(acc[d][r], 0.f, bad);
+    if (!__ballot(bad != 0.f && l == l)) return;  // bad: NaN of an infinity or a NaN
+    const long long row = static_cast<long long>(b) * a.width;
+    const int kvh = u / a.HT;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma nounroll
+      for (int at = from; at <= to; at += W) {
+        const int first = max(at * kStep, cur.lo), end = min((at + 1) * kStep, cur.len);
+#pragma nounroll
+        for (int key = first; key < end; ++key) {
+          const int page = scalar_at(a.table, row + (key >> a.shift));
+          if (page < 0 || page >= a.pages) continue;
+          const long long slot = ((static_cast<long long>(page) * a.hkv + kvh) << a.shift) +
+                                 (key & ((1 << a.shift) - 1));
+          const uint2 w = *reinterpret_cast<const uint2*>(a.vc + slot * RB + 32 * d + 8 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t half = r < 2 ? w.x : w.y;
+            const float v = __uint_as_float(r & 1 ? half & 0xffff0000u : half << 16);
+            if (!(fabsf(v) < INFINITY)) t[r] += v;
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!(fabsf(t[r]) < INFINITY)) acc[d][r] = t[r];
+    }
+  };
   bool fresh = true;
   int st = 0;
   for (int i = 0; i < count; ++i) {
@@ -432,8 +484,9 @@ void paged_attn_kernel(const PagedArgs a) {
       l += __shfl_xor(l, 32, kWave);
       // whole: the head's first step lies in this run too
       const bool whole = head_end && i >= s - cur.s0;
+      settle(max(cur.s0, s - i), s, l);
       if (whole) {
-        const float f = m_run == -INFINITY && l == 0.f ? 0.f : a.v_scale / l;
+        const float f = share(m_run, l, a.v_scale);
         uint16_t* o = a.out + (static_cast<long long>(b) * a.hq + h0 + col) * HD + 4 * g;
         if (col < heads)
 #pragma unroll
@@ -464,6 +517,7 @@ void paged_attn_kernel(const PagedArgs a) {
     const int heads = min(16, a.G - 16 * ht);
     float l = l_run + __shfl_xor(l_run, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
+    settle(cur.s0 + wave, cur.s1 - 1, l);
     float* const so = reinterpret_cast<float*>(mem);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -488,13 +542,12 @@ void paged_attn_kernel(const PagedArgs a) {
         const float4 x = *reinterpret_cast<const float4*>(part + h * LD + c);
         const float f = exp2_fast(ml.x - m_sub);
         den = fmaf(ml.y, f, den);  // NaN of a NaN score, whatever its part's weight
-        if (f == 0.f) continue;    // no weight beside the others
-        sum.x = fmaf(x.x, f, sum.x);
-        sum.y = fmaf(x.y, f, sum.y);
-        sum.z = fmaf(x.z, f, sum.z);
-        sum.w = fmaf(x.w, f, sum.w);
+        sum.x += weighted(x.x, f);
+        sum.y += weighted(x.y, f);
+        sum.z += weighted(x.z, f);
+        sum.w += weighted(x.w, f);
       }
-      const float r = mx == -INFINITY && den == 0.f ? 0.f : a.v_scale / den;
+      const float r = share(mx, den, a.v_scale);
       *reinterpret_cast<uint2*>(o + h * HD + c) =
           make_uint2(pack_bf2(sum.x * r, sum.y * r), pack_bf2(sum.z * r, sum.w * r));
     }
@@ -503,10 +556,9 @@ void paged_attn_kernel(const PagedArgs a) {
 
 // Joins the partials of one (sequence, query head): o = sum_i 2^(m_i - m) O_i /
 // sum_i 2^(m_i - m) l_i, in the runs' order within each of T / (HD / 4) lane groups and
-// then over the groups, so the result does not depend on timing.  A part without weight adds
-// nothing to O, whose values may be infinite, but adds its l, which is finite or, of a
-// visible NaN score (no maximum sees one), NaN: then the row is NaN, however its head was
-// cut.  T threads: 64 where the heads alone fill the chip, 512 where few heads have many
+// then over the groups, so the result does not depend on timing.  A part without weight still
+// adds its infinities, and its l, which is finite or, of a visible NaN score (no maximum
+// sees one), NaN: then the row is NaN, however its head was cut.  T threads: 64 where the heads alone fill the chip, 512 where few heads have many
 // partials each.
 template <int HD, int T>
 __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
@@ -541,12 +593,10 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
     const float f = exp2_fast(m - m_sub), e = exp2_fast(ml.x - m_sub);
     m = m_new;
     l = fmaf(ml.y, e, l * f);  // NaN of a NaN score, whatever its part's weight
-    if (e == 0.f) continue;    // no weight beside the others
-    if (f == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-    o.x = fmaf(x.x, e, o.x * f);
-    o.y = fmaf(x.y, e, o.y * f);
-    o.z = fmaf(x.z, e, o.z * f);
-    o.w = fmaf(x.w, e, o.w * f);
+    o.x = weighted(x.x, e) + weighted(o.x, f);
+    o.y = weighted(x.y, e) + weighted(o.y, f);
+    o.z = weighted(x.z, e) + weighted(o.z, f);
+    o.w = weighted(x.w, e) + weighted(o.w, f);
   }
   *reinterpret_cast<float4*>(&so[grp][4 * c]) = o;
   if (c == 0) {
@@ -564,10 +614,9 @@ __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
     for (int i = 0; i < NG; ++i) {
       const float e = exp2_fast(sm[i] - m_sub);
       den = fmaf(sl[i], e, den);
-      if (e == 0.f) continue;
-      num = fmaf(so[i][d], e, num);
+      num += weighted(so[i][d], e);
     }
-    out[d] = f2bf(mx == -INFINITY && den == 0.f ? 0.f : num * (a.v_scale / den));
+    out[d] = f2bf(num * share(mx, den, a.v_scale));
   }
 }
 

@@ -1,13 +1,14 @@
 """Infinite and NaN values that a row sees under a weight below fp32's range: the row's dim is
 that value, as in 64 bits, whatever waves or runs the keys are cut into.  Tolerance of the
-other dims: that of tests/test_gpu_packed_attention.py."""
+other dims: that of tests/test_gpu_paged.py and tests/test_gpu_packed_attention.py."""
 import math
 
 import pytest
 import torch
 
 from oracle import paged as ref
-from test_gpu_packed_attention import _cu, _inputs, _ok, _ops
+from test_gpu_packed_attention import _cu, _inputs, _ok
+from test_gpu_paged import _attn_ok, _decode_case, _ops
 
 pytestmark = pytest.mark.gpu
 
@@ -24,6 +25,37 @@ def _aside(got, want, ok, rows):
         got[..., d] = 0
         want[..., d] = 0
     ok(got, want)
+
+
+@pytest.mark.parametrize("longest", [100, 5000])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("far", [0, 40, 76])
+@pytest.mark.parametrize("by", [-160.0, 100.0])
+def test_a_step_over_a_value_without_weight(by, far, hd, longest):
+    """The far key's score is 160 below the others, or the last one's 100 above (and the far key's
+    60 below the rest)."""
+    g = torch.Generator().manual_seed(hd + far)
+    q, kc, vc, table, lens, ks, vs = _decode_case(2, 8, 2, hd, 16, [78, longest], False, g, std=0.5)
+    q[..., 0] = 1.0
+    kc[..., 0] = 0
+
+    def at(c, t):
+        return c[int(table[0, t // 16]), :, t % 16]
+
+    at(kc, far)[:, 0] = -160.0 if by < 0 else -60.0
+    if by > 0:
+        at(kc, 77)[:, 0] = by
+    want, spread = ref.paged_decode(q, kc, vc, table, lens, scale=1.0)
+    for d, x in BAD.items():
+        at(vc, far)[:, d] = x
+    exact, _ = ref.paged_decode(q, kc, vc, table, lens, scale=1.0)
+    assert exact[0, :, 3].eq(math.inf).all() and exact[0, :, 5].eq(-math.inf).all()
+    got = _ops().paged_attn_decode(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), lens.cuda(),
+                                   scale=1.0).cpu()
+    spread = spread.clone()
+    spread[..., list(BAD)] = 0
+    _aside(got[:1], want[:1], lambda a, b: _attn_ok(a, b, spread[:1]), slice(None))
+    _attn_ok(got[1:], want[1:], ref.paged_decode(q, kc, vc, table, lens, scale=1.0)[1][1:])
 
 
 @pytest.mark.parametrize("heads", [8, 128, 180])
