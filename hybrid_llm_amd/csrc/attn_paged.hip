@@ -556,10 +556,10 @@ void paged_attn_kernel(const PagedArgs a) {
 
 // Joins the partials of one (sequence, query head): o = sum_i 2^(m_i - m) O_i /
 // sum_i 2^(m_i - m) l_i, in the runs' order within each of T / (HD / 4) lane groups and
-// then over the groups, so the result does not depend on timing.  A part without weight still
-// adds its infinities, and its l, which is finite or, of a visible NaN score (no maximum
-// sees one), NaN: then the row is NaN, however its head was cut.  T threads: 64 where the heads alone fill the chip, 512 where few heads have many
-// partials each.
+// then over the groups, so the result does not depend on timing.  A part without weight
+// still adds its infinities, and its l, which is finite or, of a visible NaN score (no
+// maximum sees one), NaN: then the row is NaN, however its head was cut.  T threads: 64
+// where the heads alone fill the chip, 512 where few heads have many partials each.
 template <int HD, int T>
 __global__ __launch_bounds__(T) void paged_join_kernel(const PagedArgs a) {
   constexpr int LPP = HD / 4;       // lanes a partial

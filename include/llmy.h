@@ -240,11 +240,13 @@ int64_t llmy_paged_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int3
  *   z_j = scale q . k_j; softcap c > 0: c tanh(z_j / c); slopes [Hq] or NULL:
  *   z_j -= slopes[h] (len - 1 - j); out = sum_j softmax(z)_j v_j
  * over j in [max(0, len - window), len) (window 0: all) whose page the table names;
- * zeros where there is none.  Slopes past +-1024 count as +-1024.  Lengths below 0 count as 0, past width * page as that.
- * What the other slots of a page hold, NaN included, has no effect; a NaN score makes its
- * row NaN, and so do scores that are -inf throughout.  out [B, Hq, head_dim] bf16.  out and the workspace lie apart from each other,
- * from q and from the caches.  scale >= 0, finite times k_scale and log2(e); softcap <=
- * 1024.  fp32 scores and sums; weights as two bf16 in their product. */
+ * zeros where there is none.  Slopes past +-1024 count as +-1024.  Lengths below 0 count
+ * as 0, past width * page as that.  What the other slots of a page hold, NaN included, has
+ * no effect; an infinite or NaN value that is seen is its dim's result, whatever its
+ * weight; a NaN score, or scores that are -inf throughout, make the row NaN.  out [B, Hq,
+ * head_dim] bf16; it and the workspace lie apart from each other, from q and from the
+ * caches.  scale >= 0, finite times k_scale and log2(e); softcap <= 1024.  fp32 scores and
+ * sums (of weights up to 2^8 times values); weights as two bf16 in their product. */
 int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                const void* k_cache, const void* v_cache, int32_t cache_type,
                                float k_scale, float v_scale, const int32_t* page_table,
@@ -262,9 +264,11 @@ int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head
  * q [N, Hq, head_dim], k, v [N, Hkv, head_dim] strided rows (strides multiples of 8,
  * 16-byte aligned, k and v rows under 2^22 apart); out [N, Hq, head_dim] bf16, which
  * must not overlap the range of q, k or v.  Rows of no document stay as they were, and
- * what they or other unseen rows hold, NaN included, has no effect.  scale >= 0, softcap
- * <= 1024, the scale finite times log2(e); slopes past +-1024, or past 2^31 / N, count as
- * that.  fp32 scores and sums; weights rounded to bf16 for the product and its sum. */
+ * what they or other unseen rows hold, NaN included, has no effect; infinite and NaN values
+ * and scores that are seen as in llmy_paged_attn_decode.  scale >= 0, softcap <= 1024, the
+ * scale finite times log2(e); slopes past +-1024, or past 2^31 / N, count as that.  fp32
+ * scores and sums (of weights up to 2^8 times values); weights rounded to bf16 for the
+ * product and its sum. */
 int32_t llmy_packed_attn_prefill_bf16(const llmy_bf16* q, int64_t q_row, int64_t q_head,
                                       const llmy_bf16* k, int64_t k_row, int64_t k_head,
                                       const llmy_bf16* v, int64_t v_row, int64_t v_head,

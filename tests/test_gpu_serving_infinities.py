@@ -80,3 +80,23 @@ def test_a_prompt_over_a_value_without_weight(kw, far, hd, heads):
     spread = spread.clone()
     spread[..., list(BAD)] = 0
     _aside(got[far:], want[far:], lambda a, b: _ok(a, b, spread[far:]), slice(None))
+
+
+@pytest.mark.parametrize("longest", [100, 5000])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_an_8_bit_nan_without_weight(hd, longest):
+    g = torch.Generator().manual_seed(hd)
+    q, kc, vc, table, lens, ks, vs = _decode_case(2, 8, 2, hd, 16, [78, longest], True, g)
+    q[..., 0] = 8.0
+    k, v = kc.float(), vc.float()
+    k[..., 0] = 0
+    k[int(table[0, 2]), :, 8, 0] = -448.0
+    kc = k.to(kc.dtype)
+    want, spread = ref.paged_decode(q, kc, vc, table, lens, scale=2.0, k_scale=ks, v_scale=vs)
+    v[int(table[0, 2]), :, 8, 11] = math.nan
+    got = _ops().paged_attn_decode(q.cuda(), kc.cuda(), v.to(vc.dtype).cuda(), table.cuda(),
+                                   lens.cuda(), scale=2.0, k_scale=ks, v_scale=vs).cpu()
+    assert got[0, :, 11].isnan().all()
+    got[0, :, 11] = 0
+    want[0, :, 11] = spread[0, :, 11] = 0
+    _attn_ok(got, want, spread)
