@@ -14,6 +14,7 @@ from pathlib import Path
 _P = C.c_void_p
 _I = C.c_int32
 _F = C.c_float
+_D = C.c_double
 _I64 = C.c_int64
 _U64P = C.POINTER(C.c_uint64)
 
@@ -47,6 +48,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "llmy_paged_attn_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
     "llmy_paged_attn_decode": (_I, [_P, _I64, _I64, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P, _I64,
                                     _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "llmy_paged_kv_append_mx4": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P,
+                                      _P, _I, _P, _F, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _I,
+                                      _I, _I, _I, _I, _I, _I, _I, _P]),
+    "llmy_paged_kv_read_mx4": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
+                                    _I, _P]),
+    "llmy_paged_attn_mx4_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
+    "llmy_paged_attn_mx4": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64,
+                                 _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "llmy_paged_plan_workspace_bytes": (_I64, [_I, _I]),
+    "llmy_paged_plan": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I,
+                             _I, _P]),
+    "llmy_verify_drafts_workspace_bytes": (_I64, [_I, _I, _I]),
+    "llmy_verify_drafts_f32": (_I, [_P, _P, _P, _P, _P, _D, _P, _P, _P, _I64, _I, _I, _I, _P]),
     "llmy_packed_attn_prefill_bf16": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P,
                                            _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
     "llmy_gdn_prefill_workspace_bytes": (C.c_int64, [_I, _I, _I, _I, _I]),

@@ -38,6 +38,17 @@ __device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 
+// 8 codes of a 4-bit cache under their block's scale byte as bf16 (exact).
+__device__ __forceinline__ uint4 mx4_to_bf16(uint32_t w, uint32_t byte) {
+  const float step = __uint_as_float(byte << 23);
+  uint4 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, step, 0));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, step, 1));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, step, 2));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, step, 3));
+  return r;
+}
+
 // Unpack 8 bf16 held in a 16-byte vector into fp32.
 __device__ __forceinline__ void unpack8(const uint4& v, float* out) {
   out[0] = __uint_as_float(v.x << 16);
@@ -81,6 +92,12 @@ constexpr int kDppMirror = 0x140;     // row_mirror
 template <int CTRL>
 __device__ __forceinline__ float dpp_f(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
 }
 
 template <int CTRL>

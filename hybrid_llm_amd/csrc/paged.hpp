@@ -10,6 +10,7 @@
 namespace llmy {
 
 constexpr int32_t kCacheBf16 = 0, kCacheE4m3 = 1;
+constexpr int32_t kCacheMx4 = 2;  // entry points of their own: scales are tensors
 constexpr int32_t kMaxHeads = 1024;
 
 // log2 of a page's tokens, or -1 where the kernels do not take that size: 16 rows, the
@@ -138,5 +139,28 @@ inline bool scales_ok(int32_t cache_type, float k_scale, float v_scale) {
   const auto ok = [](float s) { return s >= 0x1p-100f && s <= 0x1p100f; };
   return cache_type == kCacheBf16 ? k_scale == 1.f && v_scale == 1.f : ok(k_scale) && ok(v_scale);
 }
+
+// A 4-bit cache: codes [pages, Hkv, page, head_dim / 2], two 4-bit floats a byte, the lower
+// dim in the low bits, and scale bytes [pages, Hkv, page, head_dim / 32], one a block of 32
+// dims: a code counts 2^(byte - 127) times, byte 255 makes its block NaN.
+struct Mx4Cache {
+  void *k, *v, *ks, *vs;
+
+  void* part(int i) const { return i == 0 ? k : i == 1 ? v : i == 2 ? ks : vs; }
+  static int64_t bytes(int i, int64_t slots, int32_t hd) { return slots * hd / (i < 2 ? 2 : 32); }
+  // rows of codes are read by 16 bytes, a row's scales together
+  bool ok(int64_t slots, int32_t hd) const {
+    const auto on = [](const void* p, uintptr_t a) {
+      return p && reinterpret_cast<uintptr_t>(p) % a == 0;
+    };
+    return slots == 0 || (on(k, 16) && on(v, 16) && on(ks, hd / 32) && on(vs, hd / 32));
+  }
+  bool apart(int64_t slots, int32_t hd) const {
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < i; ++j)
+        if (!bytes_apart(part(i), bytes(i, slots, hd), part(j), bytes(j, slots, hd))) return false;
+    return true;
+  }
+};
 
 }  // namespace llmy

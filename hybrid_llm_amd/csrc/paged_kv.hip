@@ -18,6 +18,11 @@
 // used.  A lane holds 4 dims of each half of its pairs, dims 4c.. and half + 4c..,
 // so a pair never crosses lanes; lane l forms the cosine and sine of pair l once
 // and hands them round through LDS.
+//
+// A 4-bit cache (kCacheMx4) stores blocks of 32 dims: the smallest power of two of which 7
+// cover the block's largest magnitude, and each value over it as a 4-bit float, to nearest
+// even.  7 and not 6, the largest code: what lies between is off by no more than half of
+// the code's last step, like the values under 6, and the finer scale serves the other 31.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "paged.hpp"
@@ -35,6 +40,7 @@ struct RopeArgs {
   const int32_t* rows;           // page-table row of token n, or null: n
   const int32_t* table;
   void *kc, *vc;
+  uint8_t *ks, *vs;              // a 4-bit cache's block scales
   float eps, scale[2], inv[2];   // of an 8-bit cache: k's and v's scale, 1 / it
   int half, interleaved;
   int N, hq, hkv, heads;         // heads: rows of one token (q, k and, with a cache, v)
@@ -86,11 +92,38 @@ __device__ __forceinline__ float mean_square(const float* y) {
 // smallest normal is under 2^-100 of the row.
 constexpr float kLeastMean = 0x1p-90f, kRaise = 0x1p100f, kLower = 0x1p-70f;
 
-template <int HD, int IT, bool CACHE, bool F8>
+// 8 values under a block scale 2^(byte - 127), byte 1 to 254, as 4-bit floats in order from
+// the lowest bits; magnitudes past 6 steps become 6.
+__device__ __forceinline__ uint32_t pack8_mx4(const float* v, uint32_t byte) {
+  const float step = __uint_as_float(byte << 23);
+  uint32_t r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], step, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], step, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], step, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], step, 3);
+}
+
+// The scale byte of a block of 32 dims, 8 on each of four neighbouring lanes: 255 where one
+// is not finite.  Magnitudes compare as integers, NaN past infinity; adding all but 1 of a
+// quarter of the mantissa's range carries into the exponent past 1.75, 7 / 4.  Largest
+// magnitudes over 1.5 x 2^127 count as that, or their code would stand for 2^128.
+__device__ __forceinline__ uint32_t mx4_scale(const float* y) {
+  uint32_t most = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(y[j]) & 0x7fffffffu);
+  most = max(most, dpp_u<kDppXor1>(most));
+  most = max(most, dpp_u<kDppXor2>(most));
+  if (most >= 0x7f800000u) return 255u;
+  const uint32_t e = (min(most, 0x7f400000u) + 0x1fffffu) >> 23;
+  return max(e, 3u) - 2u;
+}
+
+template <int HD, int IT, bool CACHE, int CT>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
+  constexpr bool F8 = CT == kCacheE4m3, M4 = CT == kCacheMx4;
   constexpr int LPR = HD / 8;   // lanes a row
   constexpr int RPI = 64 / LPR; // rows an iteration
   __shared__ __align__(16) float trig[4][2][64];
+  __shared__ __align__(16) float turn[M4 ? 4 : 1][M4 ? 512 : 4];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const uint32_t task = blockIdx.x * 4u + wave;
@@ -168,7 +201,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
       for (int j = 0; j < 8; ++j) y[j] *= by;
       mean = mean_square<HD>(y) + a.eps * by * by;
     }
-    if (r >= a.heads) continue;
+    if (!M4 && r >= a.heads) continue;  // (4 bits: all lanes meet again below)
     if (w) {
       const float rs = rsqrtf(mean);
       const float4 w0 = *reinterpret_cast<const float4*>(w + d0);
@@ -193,6 +226,26 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
         }
       }
     }
+    if (M4) {
+      // blocks are of neighbouring dims: each row's values in order through LDS
+      float z[8];
+      float* const own = turn[M4 ? wave : 0] + g * HD;
+      wave_lds_order();  // behind the last iteration's reads
+      *reinterpret_cast<float4*>(own + d0) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(own + d1) = make_float4(y[4], y[5], y[6], y[7]);
+      wave_lds_order();
+      *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(own + 8 * c);
+      *reinterpret_cast<float4*>(z + 4) = *reinterpret_cast<const float4*>(own + 8 * c + 4);
+      const uint32_t byte = mx4_scale(z);
+      if (kind != 0 && r < a.heads && slot >= 0) {
+        const long long row = slot / HD + (static_cast<long long>(h) << a.shift);
+        const uint32_t codes = byte == 255u ? 0u : pack8_mx4(z, byte);
+        uint8_t* const to = static_cast<uint8_t*>(kind == 1 ? a.kc : a.vc);
+        *reinterpret_cast<uint32_t*>(to + row * (HD / 2) + 4 * c) = codes;
+        if ((c & 3) == 0) (kind == 1 ? a.ks : a.vs)[row * (HD / 32) + (c >> 2)] = byte;
+      }
+      if (kind != 0 || r >= a.heads) continue;
+    }
     if (CACHE && kind != 0) {
       if (slot < 0) continue;
       const long long at = slot + (static_cast<long long>(h) << a.shift) * HD;
@@ -216,7 +269,42 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
   }
 }
 
-template <bool CACHE, bool F8>
+// Stored rows back as bf16, which holds each of them exactly (a code has two significant
+// bits); zeros for a token without a slot.  8 dims a lane: 4 bytes in, 16 out; bound by the
+// writes.
+struct ReadArgs {
+  const uint8_t *kc, *vc, *ks, *vs;
+  const int32_t *table, *rows, *pos;
+  uint16_t *k, *v;               // [N, Hkv, HD]
+  int N, hkv, B, width, shift, pages;
+};
+
+template <int HD>
+__global__ __launch_bounds__(256) void mx4_read_kernel(const ReadArgs a) {
+  constexpr int LPR = HD / 8;
+  const long long at = blockIdx.x * 256ll + threadIdx.x;
+  const int c = static_cast<int>(at % LPR);
+  long long row = at / LPR;  // token, k or v, head
+  const int h = static_cast<int>(row % a.hkv);
+  row /= a.hkv;
+  const bool is_v = row & 1;
+  row >>= 1;
+  if (row >= a.N) return;
+  const int n = static_cast<int>(row), p = a.pos[n], r = a.rows ? a.rows[n] : n;
+  uint4 out = uint4{0u, 0u, 0u, 0u};
+  if (p >= 0 && r >= 0 && r < a.B && (p >> a.shift) < a.width) {
+    const int page = a.table[static_cast<long long>(r) * a.width + (p >> a.shift)];
+    if (page >= 0 && page < a.pages) {
+      const long long s = ((static_cast<long long>(page) * a.hkv + h) << a.shift) +
+                          (p & ((1 << a.shift) - 1));
+      const uint32_t w = *reinterpret_cast<const uint32_t*>((is_v ? a.vc : a.kc) + s * (HD / 2) + 4 * c);
+      out = mx4_to_bf16(w, (is_v ? a.vs : a.ks)[s * (HD / 32) + (c >> 2)]);
+    }
+  }
+  *reinterpret_cast<uint4*>((is_v ? a.v : a.k) + (static_cast<long long>(n) * a.hkv + h) * HD + 8 * c) = out;
+}
+
+template <bool CACHE, int CT>
 int32_t launch_norm_rope(RopeArgs a, int head_dim, hipStream_t s) {
   const int rpi = 512 / head_dim;
   // Four iterations a wave read at the rate of a copy (16384 tokens x 40 rows of 128: 65 us,
@@ -232,14 +320,14 @@ int32_t launch_norm_rope(RopeArgs a, int head_dim, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(wgs));
   if (head_dim == 64) {
     if (it == 1)
-      hipLaunchKernelGGL((norm_rope_kernel<64, 1, CACHE, F8>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((norm_rope_kernel<64, 1, CACHE, CT>), grid, dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((norm_rope_kernel<64, 4, CACHE, F8>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((norm_rope_kernel<64, 4, CACHE, CT>), grid, dim3(256), 0, s, a);
   } else {
     if (it == 1)
-      hipLaunchKernelGGL((norm_rope_kernel<128, 1, CACHE, F8>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((norm_rope_kernel<128, 1, CACHE, CT>), grid, dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((norm_rope_kernel<128, 4, CACHE, F8>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((norm_rope_kernel<128, 4, CACHE, CT>), grid, dim3(256), 0, s, a);
   }
   return launch_status();
 }
@@ -285,7 +373,7 @@ extern "C" int32_t llmy_qk_norm_rope_bf16(
   a.pos = positions; a.inv_freq = inv_freq; a.eps = eps;
   a.half = half; a.interleaved = interleaved != 0;
   a.N = N; a.hq = Hq; a.hkv = Hkv; a.heads = Hq + Hkv;
-  return launch_norm_rope<false, false>(a, head_dim, as_stream(stream));
+  return launch_norm_rope<false, kCacheBf16>(a, head_dim, as_stream(stream));
 }
 
 extern "C" int32_t llmy_paged_kv_append(
@@ -338,6 +426,96 @@ extern "C" int32_t llmy_paged_kv_append(
   a.inv[0] = 1.f / k_scale; a.inv[1] = 1.f / v_scale;
   a.N = N; a.hq = Hq; a.hkv = Hkv; a.heads = Hq + 2 * Hkv;
   a.B = B; a.width = width; a.shift = page_shift(page); a.pages = pages;
-  return cache_type == kCacheE4m3 ? launch_norm_rope<true, true>(a, head_dim, as_stream(stream))
-                                  : launch_norm_rope<true, false>(a, head_dim, as_stream(stream));
+  return cache_type == kCacheE4m3
+             ? launch_norm_rope<true, kCacheE4m3>(a, head_dim, as_stream(stream))
+             : launch_norm_rope<true, kCacheBf16>(a, head_dim, as_stream(stream));
+}
+
+extern "C" int32_t llmy_paged_kv_append_mx4(
+    const llmy_bf16* k, int64_t k_row, int64_t k_head, const llmy_bf16* v, int64_t v_row,
+    int64_t v_head, void* k_cache, void* v_cache, void* k_scales, void* v_scales,
+    const int32_t* page_table, const int32_t* rows, const int32_t* positions,
+    const float* inv_freq, int32_t half, const float* k_norm, float eps, int32_t interleaved,
+    const llmy_bf16* q, int64_t q_row, int64_t q_head, const float* q_norm, llmy_bf16* q_out,
+    int64_t qo_row, int64_t qo_head, int32_t N, int32_t Hq, int32_t Hkv, int32_t head_dim,
+    int32_t B, int32_t width, int32_t page, int32_t pages, void* stream) {
+  LLMY_REQUIRE(N >= 0 && Hq >= 0 && Hkv > 0 && Hq <= kMaxHeads && Hkv <= kMaxHeads);
+  LLMY_REQUIRE(head_dim == 64 || head_dim == 128);
+  LLMY_REQUIRE(half >= 0 && half % 4 == 0 && 2 * half <= head_dim && (half == 0 || inv_freq));
+  LLMY_REQUIRE(eps >= 0.f);
+  LLMY_REQUIRE(B >= 0 && width >= 0 && pages >= 0 && page_shift(page) > 0);
+  if (N == 0) return 0;
+  LLMY_REQUIRE(positions && rows_ok(k, k_row, k_head, Hkv, head_dim) &&
+               rows_ok(v, v_row, v_head, Hkv, head_dim));
+  const Mx4Cache c{k_cache, v_cache, k_scales, v_scales};
+  const int64_t slots = static_cast<int64_t>(pages) * Hkv * page;
+  LLMY_REQUIRE((B == 0 || width == 0 || page_table) && c.ok(slots, head_dim) &&
+               c.apart(slots, head_dim));
+  LLMY_REQUIRE(aligned(q_norm, 16) && aligned(k_norm, 16));
+  // the caches are written while other waves still read rows and weights
+  for (int i = 0; i < 4; ++i)
+    LLMY_REQUIRE(rows_apart(Rows{k, k_row, k_head, N, Hkv, head_dim}, c.part(i),
+                            c.bytes(i, slots, head_dim)) &&
+                 rows_apart(Rows{v, v_row, v_head, N, Hkv, head_dim}, c.part(i),
+                            c.bytes(i, slots, head_dim)));
+  if (Hq > 0) {
+    LLMY_REQUIRE(rows_ok(q, q_row, q_head, Hq, head_dim) &&
+                 rows_ok(q_out, qo_row, qo_head, Hq, head_dim));
+    const Rows qi{q, q_row, q_head, N, Hq, head_dim}, qo{q_out, qo_row, qo_head, N, Hq, head_dim};
+    LLMY_REQUIRE(rows_apart(qo) && in_place_or_apart(qo, qi) &&
+                 rows_apart(qo, Rows{k, k_row, k_head, N, Hkv, head_dim}) &&
+                 rows_apart(qo, Rows{v, v_row, v_head, N, Hkv, head_dim}));
+    for (int i = 0; i < 4; ++i)
+      LLMY_REQUIRE(rows_apart(qo, c.part(i), c.bytes(i, slots, head_dim)) &&
+                   rows_apart(qi, c.part(i), c.bytes(i, slots, head_dim)));
+  }
+  RopeArgs a{};
+  a.x[0] = q; a.xr[0] = q_row; a.xh[0] = q_head;
+  a.x[1] = k; a.xr[1] = k_row; a.xh[1] = k_head;
+  a.x[2] = v; a.xr[2] = v_row; a.xh[2] = v_head;
+  a.o[0] = q_out; a.orow[0] = qo_row; a.ohead[0] = qo_head;
+  a.w[0] = q_norm; a.w[1] = k_norm;
+  a.pos = positions; a.inv_freq = inv_freq; a.eps = eps;
+  a.half = half; a.interleaved = interleaved != 0;
+  a.rows = rows; a.table = page_table; a.kc = k_cache; a.vc = v_cache;
+  a.ks = static_cast<uint8_t*>(k_scales); a.vs = static_cast<uint8_t*>(v_scales);
+  a.N = N; a.hq = Hq; a.hkv = Hkv; a.heads = Hq + 2 * Hkv;
+  a.B = B; a.width = width; a.shift = page_shift(page); a.pages = pages;
+  return launch_norm_rope<true, kCacheMx4>(a, head_dim, as_stream(stream));
+}
+
+extern "C" int32_t llmy_paged_kv_read_mx4(const void* k_cache, const void* v_cache,
+                                          const void* k_scales, const void* v_scales,
+                                          const int32_t* page_table, const int32_t* rows,
+                                          const int32_t* positions, llmy_bf16* k, llmy_bf16* v,
+                                          int32_t N, int32_t Hkv, int32_t head_dim, int32_t B,
+                                          int32_t width, int32_t page, int32_t pages,
+                                          void* stream) {
+  LLMY_REQUIRE(N >= 0 && Hkv > 0 && Hkv <= kMaxHeads && (head_dim == 64 || head_dim == 128));
+  LLMY_REQUIRE(B >= 0 && width >= 0 && pages >= 0 && page_shift(page) > 0);
+  if (N == 0) return 0;
+  const Mx4Cache c{const_cast<void*>(k_cache), const_cast<void*>(v_cache),
+                   const_cast<void*>(k_scales), const_cast<void*>(v_scales)};
+  const int64_t slots = static_cast<int64_t>(pages) * Hkv * page;
+  LLMY_REQUIRE(positions && k && v && aligned(k, 16) && aligned(v, 16) &&
+               (B == 0 || width == 0 || page_table) && c.ok(slots, head_dim));
+  const int64_t bytes = 2ll * N * Hkv * head_dim;
+  LLMY_REQUIRE(bytes_apart(k, bytes, v, bytes));
+  for (int i = 0; i < 4; ++i)
+    LLMY_REQUIRE(bytes_apart(k, bytes, c.part(i), c.bytes(i, slots, head_dim)) &&
+                 bytes_apart(v, bytes, c.part(i), c.bytes(i, slots, head_dim)));
+  ReadArgs a{};
+  a.kc = static_cast<const uint8_t*>(k_cache); a.vc = static_cast<const uint8_t*>(v_cache);
+  a.ks = static_cast<const uint8_t*>(k_scales); a.vs = static_cast<const uint8_t*>(v_scales);
+  a.table = page_table; a.rows = rows; a.pos = positions; a.k = k; a.v = v;
+  a.N = N; a.hkv = Hkv; a.B = B; a.width = width; a.shift = page_shift(page); a.pages = pages;
+  const long long lanes = static_cast<long long>(N) * Hkv * 2 * (head_dim / 8);
+  LLMY_REQUIRE(lanes < (1ll << 38));  // workgroups are 31-bit
+  const dim3 grid(static_cast<unsigned>((lanes + 255) / 256));
+  const hipStream_t s = as_stream(stream);
+  if (head_dim == 64)
+    hipLaunchKernelGGL(mx4_read_kernel<64>, grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(mx4_read_kernel<128>, grid, dim3(256), 0, s, a);
+  return launch_status();
 }

@@ -121,6 +121,34 @@ def repetition_penalty_(logits: torch.Tensor, recent: torch.Tensor, penalty: flo
     return logits
 
 
+def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, u: torch.Tensor | None = None,
+                  temperature: float = 1.0, draft_probs: torch.Tensor | None = None,
+                  counts: torch.Tensor | None = None, workspace: torch.Tensor | None = None
+                  ) -> tuple:
+    """(tokens [B,K+1], accepted [B]) int32: K drafted tokens per sequence, draft_tokens [B,K]
+    int32, against the target's logits [B,K+1,V] fp32 with the uniforms u [B,K+1] (see
+    llmy_verify_drafts_f32): kept while u q < p, then a token from max(p - q, 0), or p behind
+    the last; -1 after it.  draft_probs [B,K,V] fp32 are the drafts' distributions (None:
+    certain of the draft), counts [B] int32 the drafts there are (None: K).  temperature <= 0
+    is greedy and takes no u.  ``workspace``: a buffer of llmy_verify_drafts_workspace_bytes
+    that no overlapping call uses."""
+    B, K = draft_tokens.shape
+    V = logits.shape[-1]
+    dev = _device()
+    if tuple(logits.shape) != (B, K + 1, V):
+        raise ValueError(f"logits must be [{B}, {K + 1}, V], got {tuple(logits.shape)}")
+    pl = _vec(logits, "logits", _F32, B * (K + 1) * V, dev)
+    pd = _vec(draft_tokens, "draft_tokens", _I32, B * K, dev)
+    pq = _vec(draft_probs, "draft_probs", _F32, B * K * V, dev)
+    pc, pu = _vec(counts, "counts", _I32, B, dev), _vec(u, "u", _F32, B * (K + 1), dev)
+    tokens, accepted = draft_tokens.new_empty(B, K + 1), draft_tokens.new_empty(B)
+    nbytes = _lib.load().llmy_verify_drafts_workspace_bytes(B, K, V)
+    workspace, pw, have = _workspace(workspace, nbytes, draft_tokens, dev)
+    _lib.call("llmy_verify_drafts_f32", pl, pd, pq, pc, pu, float(temperature), tokens.data_ptr(),
+              accepted.data_ptr(), pw, have, B, K, V, _stream())
+    return tokens, accepted
+
+
 # --------------------------------------------------------------------------- projections
 EPI_STORE_BF16, EPI_STORE_F32, EPI_RESID_ADD, EPI_RESID_GATED = 0, 1, 2, 3
 # per-256-wide-K-block partial products [K/256, M, N] fp32 (M <= 64), folded by
@@ -315,6 +343,7 @@ def banded_attn_decode_parts(parts: torch.Tensor, k_off: int, v_off: int, k_cach
 # ---------------------------------------------- full-length attention over a paged cache
 CACHE_BF16, CACHE_E4M3 = 0, 1
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_FP4, _E8M0 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu  # a 4-bit cache's codes and scales
 _CACHE_TYPES = {torch.bfloat16: CACHE_BF16, torch.float8_e4m3fn: CACHE_E4M3}
 # One test a tensor, its message formed only where it fails: these calls take 3 us on the
 # GPU at their smallest, less than checks that name each property in turn.
@@ -495,6 +524,179 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
               k_scale, v_scale, pt, pl, ps, out.data_ptr(), pw, have, B, Hq, Hkv, hd, width, page,
               pages, window, hd ** -0.5 if scale is None else scale, softcap, _stream())
     return out
+
+
+def _mx4(k_cache, v_cache, k_scales, v_scales, Hkv: int, hd: int, dev: int) -> tuple:
+    """(pages, page) and the addresses of a 4-bit cache's codes [pages, Hkv, page, hd / 2] and
+    scales [pages, Hkv, page, hd / 32]."""
+    shape = k_cache.shape
+    if len(shape) == 4:
+        scales = (shape[0], Hkv, shape[2], hd // 32)
+        if (k_cache.dtype is _FP4 and v_cache.dtype is _FP4 and k_scales.dtype is _E8M0
+                and v_scales.dtype is _E8M0 and shape[1] == Hkv and shape[3] == hd // 2
+                and v_cache.shape == shape and k_scales.shape == scales
+                and v_scales.shape == scales
+                and all(t.is_contiguous() and t.get_device() == dev
+                        for t in (k_cache, v_cache, k_scales, v_scales))):
+            return (shape[0], shape[2], k_cache.data_ptr(), v_cache.data_ptr(),
+                    k_scales.data_ptr(), v_scales.data_ptr())
+    raise ValueError(
+        f"a 4-bit cache is contiguous codes [pages, {Hkv}, page, {hd // 2}] of {_FP4} and scales "
+        f"[pages, {Hkv}, page, {hd // 32}] of {_E8M0} on cuda:{dev}, the current device; got "
+        + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.device}"
+                    for t in (k_cache, v_cache, k_scales, v_scales)))
+
+
+def mx4_cache(pages: int, Hkv: int, page: int, hd: int, device="cuda") -> tuple:
+    """An empty 4-bit cache: (k_cache, v_cache, k_scales, v_scales), every value zero."""
+    codes, scales = (pages, Hkv, page, hd // 2), (pages, Hkv, page, hd // 32)
+    return tuple(torch.zeros(s, dtype=torch.uint8, device=device).view(t)
+                 for s, t in ((codes, _FP4), (codes, _FP4), (scales, _E8M0), (scales, _E8M0)))
+
+
+def _table(page_table: torch.Tensor, dev: int) -> tuple:
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    B, width = page_table.shape
+    return B, width, _vec(page_table, "page_table", _I32, B * width, dev)
+
+
+def _workspace(workspace, nbytes: int, like: torch.Tensor, dev: int) -> tuple:
+    """(buffer, its address, its bytes): the given one, checked, or one made here."""
+    if workspace is not None:
+        at = _vec(workspace, "workspace", workspace.dtype, workspace.numel(), dev)
+        have = workspace.numel() * workspace.element_size()
+        if have < nbytes:
+            raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
+        return workspace, at, have
+    if nbytes <= 0:  # none needed, or sizes that the call refuses
+        return None, None, 0
+    workspace = like.new_empty((nbytes + 7) // 8, dtype=torch.int64)
+    return workspace, workspace.data_ptr(), nbytes
+
+
+def paged_kv_append_mx4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                        v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                        page_table: torch.Tensor, positions: torch.Tensor,
+                        rows: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
+                        k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                        interleaved: bool = False, q: torch.Tensor | None = None,
+                        q_norm: torch.Tensor | None = None, q_out: torch.Tensor | None = None
+                        ) -> torch.Tensor | None:
+    """paged_kv_append into a cache held in 4 bits (mx4_cache): codes k_cache, v_cache
+    [pages,Hkv,page,hd/2] float4_e2m1fn_x2 and scales k_scales, v_scales [pages,Hkv,page,hd/32]
+    float8_e8m0fnu, one for each 32 dims of a row (see llmy_paged_kv_append_mx4).  Returns
+    q_out."""
+    N, Hkv, hd = k.shape
+    dev = _device()
+    pk, kr, kh = _heads(k, "k", (N, Hkv, hd), dev)
+    pv, vr, vh = _heads(v, "v", (N, Hkv, hd), dev)
+    pages, page, *cache = _mx4(k_cache, v_cache, k_scales, v_scales, Hkv, hd, dev)
+    B, width, pt = _table(page_table, dev)
+    if rows is None and N > B:
+        raise ValueError(f"{N} tokens and {B} page-table rows: name each token's row")
+    pp, pr = _vec(positions, "positions", _I32, N, dev), _vec(rows, "rows", _I32, N, dev)
+    half = 0 if inv_freq is None else inv_freq.numel()
+    pf = _vec(inv_freq, "inv_freq", _F32, half, dev)
+    wk = _vec(k_norm, "k_norm", _F32, hd, dev)
+    Hq, pq, qr, qh, po, por, poh, wq = 0, None, 0, 0, None, 0, 0, None
+    if q is not None:
+        Hq = q.shape[1]
+        pq, qr, qh = _heads(q, "q", (N, Hq, hd), dev)
+        wq = _vec(q_norm, "q_norm", _F32, hd, dev)
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            po, por, poh = q_out.data_ptr(), Hq * hd, hd
+        else:
+            po, por, poh = _heads(q_out, "q_out", (N, Hq, hd), dev)
+    elif q_norm is not None or q_out is not None:
+        raise ValueError("q_norm and q_out go with q")
+    _lib.call("llmy_paged_kv_append_mx4", pk, kr, kh, pv, vr, vh, *cache, pt, pr, pp, pf, half, wk,
+              eps, interleaved, pq, qr, qh, wq, po, por, poh, N, Hq, Hkv, hd, B, width, page,
+              pages, _stream())
+    return q_out
+
+
+def paged_kv_read_mx4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                      v_scales: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor,
+                      rows: torch.Tensor | None = None) -> tuple:
+    """(k, v) [N,Hkv,hd] bf16: what a 4-bit cache holds for N tokens, named as in
+    paged_kv_append_mx4; zeros for one without a slot (see llmy_paged_kv_read_mx4)."""
+    Hkv, hd, N = k_cache.shape[1], 2 * k_cache.shape[-1], positions.numel()
+    dev = _device()
+    pages, page, *cache = _mx4(k_cache, v_cache, k_scales, v_scales, Hkv, hd, dev)
+    B, width, pt = _table(page_table, dev)
+    if rows is None and N > B:
+        raise ValueError(f"{N} tokens and {B} page-table rows: name each token's row")
+    pp, pr = _vec(positions, "positions", _I32, N, dev), _vec(rows, "rows", _I32, N, dev)
+    k, v = (torch.empty(N, Hkv, hd, dtype=_BF16, device=k_cache.device) for _ in range(2))
+    _lib.call("llmy_paged_kv_read_mx4", *cache, pt, pr, pp, k.data_ptr(), v.data_ptr(), N, Hkv,
+              hd, B, width, page, pages, _stream())
+    return k, v
+
+
+def paged_attn_mx4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
+                   lengths: torch.Tensor, scale: float | None = None, window: int = 0,
+                   softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None, workspace: torch.Tensor | None = None
+                   ) -> torch.Tensor:
+    """The last token of each sequence, q [B,Hq,hd] bf16, or its last T, q [B,T,Hq,hd] (a token
+    and its drafts, T <= 64), over the first lengths[b] (int32) positions of page_table[b] in a
+    4-bit cache that holds them already (see llmy_paged_attn_mx4): token t sees the positions
+    up to its own, lengths[b] - T + t.  scale, window, softcap, slopes, out and workspace (of
+    llmy_paged_attn_mx4_workspace_bytes) as in paged_attn_decode."""
+    shape = q.shape
+    B, T, Hq, hd = shape if len(shape) == 4 else (shape[0], 1, *shape[1:])
+    Hkv = k_cache.shape[1]
+    dev = _device()
+    st = q.stride()
+    if q.dtype is not _BF16 or st[-1] != 1 or q.get_device() != dev:
+        raise ValueError(f"q must be torch.bfloat16 with contiguous dims on cuda:{dev}, the "
+                         f"current device; got {q.dtype} {tuple(shape)}, strides {st}, {q.device}")
+    pages, page, *cache = _mx4(k_cache, v_cache, k_scales, v_scales, Hkv, hd, dev)
+    rows, width, pt = _table(page_table, dev)
+    if rows != B:
+        raise ValueError(f"page_table must be [{B}, pages], got {tuple(page_table.shape)}")
+    pl, ps = _vec(lengths, "lengths", _I32, B, dev), _vec(slopes, "slopes", _F32, Hq, dev)
+    out = _out(out, q, dev)
+    nbytes = _lib.load().llmy_paged_attn_mx4_workspace_bytes(B, T, Hq, Hkv, hd, width, page)
+    workspace, pw, have = _workspace(workspace, nbytes, q, dev)
+    _lib.call("llmy_paged_attn_mx4", q.data_ptr(), st[0], st[1] if len(shape) == 4 else 0, st[-2],
+              *cache, pt, pl, ps, out.data_ptr(), pw, have, B, T, Hq, Hkv, hd, width, page, pages,
+              window, hd ** -0.5 if scale is None else scale, softcap, _stream())
+    return out
+
+
+def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, page_table: torch.Tensor,
+               held: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, page: int,
+               tokens: int, reset: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> tuple:
+    """Pages and slots for the new tokens of B sequences (see llmy_paged_plan), all int32 and
+    decided on the GPU: sequence b has lengths[b] tokens on held[b] pages of page_table[b] and
+    gets new_tokens[b] behind them, after giving its pages back and starting over where
+    reset[b] is not 0.  page_table [B,width], held [B], free_pages (a stack of page ids) and
+    n_free [1] (its height) are updated in place.  Returns (cu_seqlens [B+1], rows [tokens],
+    positions [tokens], lengths [B]) for the packed new tokens, of which ``tokens`` bounds the
+    number; a token whose sequence got no pages has position -1, entries behind the last row
+    and position -1.  ``workspace``: a buffer of llmy_paged_plan_workspace_bytes that no
+    overlapping call uses."""
+    dev = _device()
+    B, width, pt = _table(page_table, dev)
+    pl, pn = _vec(lengths, "lengths", _I32, B, dev), _vec(new_tokens, "new_tokens", _I32, B, dev)
+    ph, pr = _vec(held, "held", _I32, B, dev), _vec(reset, "reset", _I32, B, dev)
+    pf = _vec(free_pages, "free_pages", _I32, free_pages.numel(), dev)
+    p1 = _vec(n_free, "n_free", _I32, 1, dev)
+    if tokens < 0:
+        raise ValueError(f"tokens must not be negative, got {tokens}")
+    cu = lengths.new_empty(B + 1)
+    rows, positions, out = lengths.new_empty(tokens), lengths.new_empty(tokens), lengths.new_empty(B)
+    nbytes = _lib.load().llmy_paged_plan_workspace_bytes(B, tokens)
+    workspace, pw, have = _workspace(workspace, nbytes, lengths, dev)
+    _lib.call("llmy_paged_plan", pl, pn, pr, pt, ph, pf, p1, cu.data_ptr(), rows.data_ptr(),
+              positions.data_ptr(), out.data_ptr(), pw, have, B, width, page, free_pages.numel(),
+              tokens, _stream())
+    return cu, rows, positions, out
 
 
 def packed_attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,

@@ -256,6 +256,92 @@ int32_t llmy_paged_attn_decode(const llmy_bf16* q, int64_t q_row, int64_t q_head
                                int32_t pages, int32_t window, float scale, float softcap,
                                void* stream);
 
+/* A cache held in 4 bits (OCP microscaling, MXFP4): codes k_cache / v_cache [pages, Hkv,
+ * page, head_dim / 2], a 4-bit float (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) for each
+ * dim, the lower dim in a byte's low bits; scales k_scales / v_scales [pages, Hkv, page,
+ * head_dim / 32], one byte for each 32 dims of a row: a code counts 2^(byte - 127) times,
+ * byte 255 makes its block NaN (253 and 254, under which codes pass fp32, are not stored;
+ * the attention takes a block of v under them as NaN).  Codes 16-byte aligned, scales by
+ * head_dim / 32.
+ *
+ * Appends as llmy_paged_kv_append does.  A block's scale is the smallest power of two, 2^-126
+ * or more, of which 7 cover its largest magnitude; each value over it goes to the nearest
+ * code, ties to the even one (past 6: to 6, off by at most 1 as between 4 and 6).
+ * Magnitudes past 1.5 x 2^127 are stored as that; a block that holds a NaN or an infinity
+ * is NaN.  The four parts of the cache lie apart from each other and from all rows. */
+int32_t llmy_paged_kv_append_mx4(const llmy_bf16* k, int64_t k_row, int64_t k_head,
+                                 const llmy_bf16* v, int64_t v_row, int64_t v_head,
+                                 void* k_cache, void* v_cache, void* k_scales, void* v_scales,
+                                 const int32_t* page_table, const int32_t* rows,
+                                 const int32_t* positions, const float* inv_freq, int32_t half,
+                                 const float* k_norm, float eps, int32_t interleaved,
+                                 const llmy_bf16* q, int64_t q_row, int64_t q_head,
+                                 const float* q_norm, llmy_bf16* q_out, int64_t qo_row,
+                                 int64_t qo_head, int32_t N, int32_t Hq, int32_t Hkv,
+                                 int32_t head_dim, int32_t B, int32_t width, int32_t page,
+                                 int32_t pages, void* stream);
+
+/* The stored keys and values of N tokens, named as in the append, as bf16 rows k, v [N, Hkv,
+ * head_dim] (16-byte aligned, apart from each other and the cache): exactly what the cache
+ * holds (past 3.39e38, under bytes 253 and 254, infinity), zeros for a token without a slot. */
+int32_t llmy_paged_kv_read_mx4(const void* k_cache, const void* v_cache, const void* k_scales,
+                               const void* v_scales, const int32_t* page_table,
+                               const int32_t* rows, const int32_t* positions, llmy_bf16* k,
+                               llmy_bf16* v, int32_t N, int32_t Hkv, int32_t head_dim, int32_t B,
+                               int32_t width, int32_t page, int32_t pages, void* stream);
+
+/* Workspace (bytes) of llmy_paged_attn_mx4 for these sizes; -1 where that call refuses them,
+ * 0 where it takes none.  No two calls that may overlap share one. */
+int64_t llmy_paged_attn_mx4_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
+                                            int32_t head_dim, int32_t width, int32_t page);
+
+/* Attention of the last T tokens (1 to 64) of each sequence over a 4-bit cache that holds
+ * them already: q [B, T, Hq, head_dim] (strides in elements, multiples of 8, 16-byte aligned),
+ * out [B, T, Hq, head_dim] bf16.  Token t stands at position lengths[b] - T + t and sees the
+ * positions up to its own, as llmy_paged_attn_decode of that length does: window, softcap,
+ * slopes, lengths, pages without a name, rows that see nothing and NaN or -inf scores as
+ * there (a token at a negative position sees nothing).  A NaN block of v that is seen makes
+ * its dims NaN for the rows that see it, whatever its weight; what unseen slots hold has no
+ * effect.  out and the workspace lie apart from each other, from the range of q and from the
+ * cache.  scale >= 0, finite times log2(e); softcap <= 1024.  fp32 scores and sums (of
+ * weights up to 2^8 times values); weights as two bf16 in their product. */
+int32_t llmy_paged_attn_mx4(const llmy_bf16* q, int64_t q_seq, int64_t q_row, int64_t q_head,
+                            const void* k_cache, const void* v_cache, const void* k_scales,
+                            const void* v_scales, const int32_t* page_table,
+                            const int32_t* lengths, const float* slopes, llmy_bf16* out,
+                            void* workspace, int64_t workspace_bytes, int32_t B, int32_t T,
+                            int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t width,
+                            int32_t page, int32_t pages, int32_t window, float scale,
+                            float softcap, void* stream);
+
+/* Workspace (bytes) of llmy_paged_plan; -1 where that call refuses the sizes. */
+int64_t llmy_paged_plan_workspace_bytes(int32_t B, int32_t capacity);
+
+/* Pages and slots for the new tokens of B sequences (at most 4096), from their lengths.
+ * Sequence b holds held[b] pages (page_table[b][0 .. held[b])) and lengths[b] tokens, and
+ * gets new_tokens[b] more behind them (negative numbers count as 0); where reset [B] (or
+ * NULL) is not 0 its pages go back first and its length counts as 0.  free_pages
+ * [free_capacity] is a stack of page ids, its top n_free[0] entries from the bottom in use.
+ * In place:
+ *   - the pages of sequences that start over are pushed, in the sequences' order and the
+ *     pages' (beyond free_capacity: dropped);
+ *   - then each sequence in order that has new tokens gets the pages that ceil((length +
+ *     new) / page) lacks, from the top of the stack down, held[b] onward in its row.  One
+ *     that would need more than are left gets none, nor does any after it that needs some;
+ *     nor does one that passes width * page, or whose packed tokens pass `capacity`.
+ * held, free_pages, n_free and page_table are updated; entries of page_table from held[b] on
+ * and of free_pages from n_free on hold what they held.  Out: cu_seqlens [B + 1], the packed
+ * tokens' bounds (sums of new_tokens, at most capacity); rows, positions [capacity]: each
+ * packed token's sequence and position, both as the append takes them: position -1 where its
+ * sequence got no place, row and position -1 behind the last token; lengths_out [B], with
+ * the new tokens of those that did.  No range that the call writes may touch another. */
+int32_t llmy_paged_plan(const int32_t* lengths, const int32_t* new_tokens, const int32_t* reset,
+                        int32_t* page_table, int32_t* held, int32_t* free_pages, int32_t* n_free,
+                        int32_t* cu_seqlens, int32_t* rows, int32_t* positions,
+                        int32_t* lengths_out, void* workspace, int64_t workspace_bytes, int32_t B,
+                        int32_t width, int32_t page, int32_t free_capacity, int32_t capacity,
+                        void* stream);
+
 /* Attention over N packed rows of `docs` documents: rows cu_seqlens[d] .. cu_seqlens[d + 1]
  * (device int32 [docs + 1], ascending) are document d.  Row i of a document that starts
  * at a sees its rows j <= i with i - j < window (0: all) and, with prefix [docs] (int32 or
@@ -732,6 +818,29 @@ int32_t llmy_sample_top_p_f32(const float* logits, int32_t rows, int32_t V,
 int32_t llmy_repetition_penalty_f32(float* logits, int32_t rows, int32_t V,
                                     const int32_t* recent, int32_t n_recent,
                                     float penalty, void* stream);
+
+/* Workspace (bytes) of llmy_verify_drafts_f32; -1 where that call refuses the sizes. */
+int64_t llmy_verify_drafts_workspace_bytes(int32_t B, int32_t K, int32_t V);
+
+/* Verification of K drafted tokens (1 to 63) per sequence against the target's logits [B,
+ * K + 1, V] fp32, row t behind t of its drafts; p_t = softmax(logits_t / temperature).
+ * draft_tokens [B, K]; draft_probs [B, K, V] fp32, the distributions q_t that they were drawn
+ * from, or NULL: q_t is 1 at the draft; counts [B] or NULL: drafts there are (0 to K; else K);
+ * u [B, K + 1] fp32 in [0, 1).  Draft x_t is kept while u_t q_t(x_t) < p_t(x_t) (one outside
+ * [0, V) is not); the first that is not is replaced by a draw from max(p_t - q_t, 0) (where
+ * nothing is left, from p_t), and behind the last comes a draw from that row's p: the first
+ * id, in order, whose running sum passes u[b][K] times the whole.  tokens [B, K + 1]: the
+ * kept drafts, the drawn id, then -1; accepted [B]: drafts kept.  temperature <= 0: a draft
+ * is kept while it is its row's first largest id, and that id follows; u is not read.  A
+ * row with no finite largest logit (NaN counts as larger) is certain of its first largest
+ * id.  Exponentials and sums in 64 bits.  V <= 2^30.  Outputs and the workspace (8-byte
+ * aligned) lie apart from each other and from the inputs; no two calls that may overlap
+ * share a workspace.  The reference has no drafts. */
+int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* draft_tokens,
+                               const float* draft_probs, const int32_t* counts, const float* u,
+                               double temperature, int32_t* tokens, int32_t* accepted,
+                               void* workspace, int64_t workspace_bytes, int32_t B, int32_t K,
+                               int32_t V, void* stream);
 
 /* --- Engine handles (llmy_cuda/include/llmy.h:27-72) ----------------------
  * The reference engine API with the same signatures and meaning; the model
