@@ -53,7 +53,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                       _I, _I, _I, _I, _I, _I, _I, _P]),
     "llmy_paged_kv_read_mx4": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
                                     _I, _P]),
-    "llmy_paged_attn_mx4_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
+    "llmy_paged_attn_mx4_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "llmy_paged_attn_mx4": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64,
                                  _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
     "llmy_paged_plan_workspace_bytes": (_I64, [_I, _I]),

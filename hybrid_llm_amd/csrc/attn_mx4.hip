@@ -43,7 +43,9 @@ __device__ __forceinline__ int32_t uniform_at(const int32_t* p, long long i) {
 }
 
 constexpr int kMxStep = 32;      // keys a step
-constexpr int kMxAhead = 3;      // steps in registers
+constexpr int kMxAhead = 2;      // steps in registers
+constexpr int kMxPad = 8;        // steps that a head tile costs besides
+constexpr int kMxLeast = 16;     // places of a run at the least
 constexpr float kMxLowest = -3.402823466e38f;
 constexpr uint32_t kMxOne = 127u;   // the scale byte of 1
 constexpr uint32_t kMxLost = 253u;  // from here on codes pass fp32, or the block is NaN
@@ -55,16 +57,21 @@ struct Mx4Args {
   const int32_t *table, *lengths;
   uint16_t* out;               // [B, T, Hq, HD]
   float *po, *pml;             // partials: O [2 runs, GT, HD] and (m, l) [2 runs, GT, 2]
-  int32_t* starts;             // [B + 1]: steps of the sequences before each, and of all
+  int32_t* starts;             // [B + 1]: places of the sequences before each, and of all
   const float* slopes;
   float scale_log2, cap_log2, cap_x2;
   int B, T, hq, hkv, G, HT, GT;  // T G columns in HT tiles of GT <= 16 NT
   int width, shift, pages, window, cap_len;
+  uint32_t page_bytes;         // of a page's codes
   int runs;
 };
 
 struct MxSeq {
   int len, lo, s0, s1;         // positions [lo, len) seen by any token, steps [s0, s1)
+
+  // A head tile's places on the flat list: kMxPad for what it costs beside its steps (its
+  // queries, the waves' join, the round that its last steps do not fill), then they.
+  __device__ __forceinline__ int places() const { return s1 > s0 ? s1 - s0 + kMxPad : 0; }
 };
 
 __device__ __forceinline__ MxSeq mx_seq(int len, const Mx4Args& a) {
@@ -76,7 +83,7 @@ __device__ __forceinline__ MxSeq mx_seq(int len, const Mx4Args& a) {
   return s;
 }
 
-// Steps of all sequences (the host sees to it that they fit 31 bits), as sums over 64
+// Places of all sequences (the host sees to it that they fit 31 bits), as sums over 64
 // blocks of `per` sequences, one per lane.
 struct MxScan {
   int before, upto, total;  // this lane's block: exclusive and inclusive sums
@@ -89,8 +96,7 @@ __device__ __forceinline__ MxScan mx_scan(const Mx4Args& a, int lane) {
   int n = 0;
   const int b1 = min(a.B, (lane + 1) * r.per);
   for (int b = lane * r.per; b < b1; ++b) {
-    const MxSeq s = mx_seq(a.lengths[b], a);
-    n += s.s1 - s.s0;
+    n += mx_seq(a.lengths[b], a).places();
   }
   r.upto = n;
 #pragma unroll
@@ -105,7 +111,7 @@ __device__ __forceinline__ MxScan mx_scan(const Mx4Args& a, int lane) {
 
 __device__ __forceinline__ int mx_run(long long total, int runs) {
   const long long q = (total + runs - 1) / runs;
-  return static_cast<int>(q > 1 ? q : 1);
+  return static_cast<int>(q > kMxLeast ? q : kMxLeast);
 }
 
 // 1 over a row's sum of weights; without a visible key (m -inf) 0, with only scores of -inf
@@ -135,9 +141,44 @@ struct MxStage {
   uint32_t vs[NV];
 };
 
-// W waves: 1: a run of the flat list; more: a head tile, each wave every W-th of its steps.
+// Waves a SIMD: as many as the registers of each form take.
+constexpr int mx4_waves(int hd, int nt) { return hd == 64 ? (nt == 1 ? 3 : 2) : nt == 1 ? 3 : 2; }
+
+// A place in a workgroup's run: steps [begin, end) of one head tile, `it` of its rounds (a
+// step for each wave) done, and `left` steps of the run behind this tile's.
+struct MxPlace {
+  int b, kvh, ht, len, lo, begin, end, it, left;
+
+  // its sequence's page ids, and the last that its keys reach: those past the length stay there
+  const int32_t* table;
+  int last;
+
+  __device__ __forceinline__ void sequence(const Mx4Args& a, int n, int first) {
+    len = n;
+    lo = first;
+    table = a.table + static_cast<long long>(b) * a.width;
+    last = (n - 1) >> a.shift;
+  }
+};
+
+// A global address from an SGPR pair and a lane's 32-bit offset: kept from being folded into
+// one 64-bit address a lane, which costs an addition each time.
+typedef const uint8_t __attribute__((address_space(1)))* global_u8;
+
+__device__ __forceinline__ global_u8 mx_base(const uint8_t* p, uint64_t off) {
+  uint64_t at = reinterpret_cast<uint64_t>(p) + off;
+  asm("" : "+s"(at));
+  return reinterpret_cast<global_u8>(at);
+}
+
+template <class T>
+__device__ __forceinline__ T mx_load(global_u8 p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const T __attribute__((address_space(1)))*>(p));
+}
+
+// W waves: a run of the flat list (runs > 0), or a whole head tile.
 template <int HD, int NT, int W>
-__global__ __launch_bounds__(64 * W, W > 1 ? W / 4 : NT == 1 ? 2 : 1)
+__global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : mx4_waves(HD, NT))
 void mx4_attn_kernel(const Mx4Args a) {
   constexpr int RB = 2 * HD;                  // bytes of a V row in LDS
   constexpr int CB = HD / 2, SB = HD / 32;    // bytes of a stored row: codes, scales
@@ -146,55 +187,101 @@ void mx4_attn_kernel(const Mx4Args a) {
   constexpr int NV = MxStage<HD>::NV;
   constexpr int CPR = HD / 32;                // 16-byte chunks of a stored row
   constexpr int LD = HD + 4;                  // of a column's part in the waves' join
-  constexpr int TILE = kMxStep * RB, JOIN = W > 1 ? 16 * NT * (LD + 2) * 4 : 0;
+  constexpr int TILE = kMxStep * RB, JOIN = 16 * NT * (LD + 2) * 4;
   constexpr int LDS = TILE > JOIN ? TILE : JOIN;
+  static_assert(LDS % 128 == 0, "the waves' rows start on one bank");
   __shared__ __align__(1024) uint8_t smem[W * LDS];
 
   const int lane = threadIdx.x & 63;
-  const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const int units = a.hkv * a.HT, TG = a.T * a.G;
 
-  // this wave's run: `count` steps from step s of head tile u of sequence b on
-  int b, u, s, count, run_q = 0;
-  long long run_at = 0;
-  MxSeq cur;
-  if (W > 1) {
-    b = blockIdx.x / units;
-    u = blockIdx.x - b * units;
-    cur = mx_seq(uniform_at(a.lengths, b), a);
-    s = cur.s0 + wave;
-    count = max(0, (cur.s1 - s + W - 1) / W);
-  } else {
-    const MxScan sc = mx_scan(a, lane);
-    if (blockIdx.x == 0) {  // where each sequence's steps begin, for the join
-      int at = sc.before;
-      const int b1 = min(a.B, (lane + 1) * sc.per);
-      for (int i = lane * sc.per; i < b1; ++i) {
-        a.starts[i] = at;
-        const MxSeq q = mx_seq(a.lengths[i], a);
-        at += q.s1 - q.s0;
+  MxPlace at;  // where this workgroup's run starts
+  {
+    MxSeq cur;
+    int u;
+    at.it = 0;
+    if (a.runs == 0) {
+      at.b = blockIdx.x / units;
+      u = blockIdx.x - at.b * units;
+      cur = mx_seq(uniform_at(a.lengths, at.b), a);
+      at.begin = cur.s0;
+      at.end = cur.s1;
+      at.left = 0;
+    } else {
+      const MxScan sc = mx_scan(a, lane);
+      if (blockIdx.x == 0 && wave == 0) {  // where each sequence's places begin, for the join
+        int x = sc.before;
+        const int b1 = min(a.B, (lane + 1) * sc.per);
+        for (int i = lane * sc.per; i < b1; ++i) {
+          a.starts[i] = x;
+          x += mx_seq(a.lengths[i], a).places();
+        }
+        if (lane == 0) a.starts[a.B] = sc.total;
       }
-      if (lane == 0) a.starts[a.B] = sc.total;
+      const long long total = static_cast<long long>(sc.total) * units;
+      const int run_q = mx_run(total, a.runs);
+      const long long run_at = static_cast<long long>(blockIdx.x) * run_q;
+      if (run_at >= total) return;
+      const int count = static_cast<int>(min(static_cast<long long>(run_q), total - run_at));
+      const uint64_t past = __ballot(static_cast<long long>(sc.upto) * units > run_at);
+      const int blk = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      long long before = __builtin_amdgcn_readlane(sc.before, blk);
+      at.b = blk * sc.per;
+      for (;; ++at.b) {  // ends: the block's sum passes run_at
+        cur = mx_seq(uniform_at(a.lengths, at.b), a);
+        if ((before + cur.places()) * units > run_at) break;
+        before += cur.places();
+      }
+      const long long rem = run_at - before * units;
+      u = static_cast<int>(rem / cur.places());
+      const int p0 = static_cast<int>(rem - static_cast<long long>(u) * cur.places());
+      const int p1 = min(cur.places(), p0 + count);
+      at.begin = cur.s0 + max(0, p0 - kMxPad);
+      at.end = cur.s0 + max(0, p1 - kMxPad);
+      at.left = count - (p1 - p0);
+      if (at.end == at.begin) return;  // the pad alone: its steps begin the next run
     }
-    const long long total = static_cast<long long>(sc.total) * units;
-    run_q = mx_run(total, a.runs);
-    run_at = static_cast<long long>(blockIdx.x) * run_q;
-    if (run_at >= total) return;
-    count = static_cast<int>(min(static_cast<long long>(run_q), total - run_at));
-    const uint64_t past = __ballot(static_cast<long long>(sc.upto) * units > run_at);
-    const int blk = __ffsll(static_cast<unsigned long long>(past)) - 1;
-    long long at = __builtin_amdgcn_readlane(sc.before, blk);
-    b = blk * sc.per;
-    for (;; ++b) {  // ends: the block's sum passes run_at
-      cur = mx_seq(uniform_at(a.lengths, b), a);
-      if ((at + cur.s1 - cur.s0) * units > run_at) break;
-      at += cur.s1 - cur.s0;
+    at.sequence(a, cur.len, cur.lo);
+    if (at.begin == at.end) {  // nothing to see (a whole tile): zeros
+      const int kvh = u / a.HT, ht = u - kvh * a.HT;
+      const int cols = min(16 * NT, TG - 16 * NT * ht);
+      for (int e = threadIdx.x; e < cols * (HD / 4); e += 64 * W) {
+        const int ci = 16 * NT * ht + e / (HD / 4), t = ci / a.G;
+        *reinterpret_cast<uint2*>(a.out + ((static_cast<long long>(at.b) * a.T + t) * a.hq +
+                                           kvh * a.G + ci - t * a.G) * HD + 4 * (e % (HD / 4))) =
+            make_uint2(0u, 0u);
+      }
+      return;
     }
-    const long long rem = run_at - at * units;
-    u = static_cast<int>(rem / (cur.s1 - cur.s0));
-    s = cur.s0 + static_cast<int>(rem - static_cast<long long>(u) * (cur.s1 - cur.s0));
+    at.kvh = u / a.HT;
+    at.ht = u - at.kvh * a.HT;
   }
+
+  // one round on; false behind the run's last
+  const auto advance = [&](MxPlace& p) __attribute__((always_inline)) {
+    ++p.it;
+    if (p.begin + p.it * W < p.end) return true;
+    if (p.left <= kMxPad) return false;  // no step of the next tile
+    p.it = 0;
+    if (++p.ht == a.HT) {
+      p.ht = 0;
+      if (++p.kvh == a.hkv) {
+        p.kvh = 0;
+        MxSeq q;
+        do {
+          q = mx_seq(uniform_at(a.lengths, ++p.b), a);
+        } while (q.s0 == q.s1);
+        p.sequence(a, q.len, q.lo);
+      }
+    }
+    p.begin = p.lo / kMxStep;
+    const int all = (p.len + kMxStep - 1) / kMxStep - p.begin;
+    p.end = p.begin + min(all, p.left - kMxPad);
+    p.left = max(0, p.left - kMxPad - all);
+    return true;
+  };
 
   // byte offsets of this lane's loads from its tile's first row
   const uint32_t k_at = col * CB + g * (CB / 4), ks_at = col * SB + g * SB / 4;
@@ -202,118 +289,115 @@ void mx4_attn_kernel(const Mx4Args a) {
   uint8_t* const mem = smem + wave * LDS;
   const uint32_t base = lds_addr(mem);
 
-  int ib = b, iu = u, is = s;
-  MxSeq icur = cur;
-  auto next = [&](int& nb, int& nu, int& ns, MxSeq& q) {  // the step after; the caller counts
-    ns += W;
-    if (W > 1 || ns < q.s1) return;
-    if (++nu == units) {
-      nu = 0;
-      do {
-        q = mx_seq(uniform_at(a.lengths, ++nb), a);
-      } while (q.s0 == q.s1);
-    }
-    ns = q.s0;
+  // The round that is loaded next, and its page ids.  Every wave loads something every round,
+  // its tile's last step where it has none of its own, so that the compiler can count the
+  // loads that are in flight: past a branch around them it would wait for all.
+  MxPlace to = at;
+  bool more = true;
+  int ipage[2], istep;
+  const auto look = [&]() __attribute__((always_inline)) {
+    istep = min(to.begin + to.it * W + wave, to.end - 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      ipage[h] = uniform_at(to.table, min((istep * kMxStep + 16 * h) >> a.shift, to.last));
   };
-  unsigned holes[kMxAhead];  // of each stage: its 16-key tiles whose page the table does not name
+  // of each stage: its 16-key tiles that are not there, no step's or in a page without a name
+  unsigned holes[kMxAhead];
   MxStage<HD> stage[kMxAhead];
-  auto issue = [&](int d) __attribute__((always_inline)) {
-    const int kvh = iu / a.HT;
-    const long long row = static_cast<long long>(ib) * a.width;
-    const int last = (icur.len - 1) >> a.shift;  // keys past the length stay in its page
-    long long at[2];
-    holes[d] = 0;
+  const auto issue = [&](int d) __attribute__((always_inline)) {
+    holes[d] = !more || to.begin + to.it * W + wave >= to.end ? 3u : 0u;
+    global_u8 kp[2], vp[2], ksp[2], vsp[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = is * kMxStep + 16 * h;
-      const int page = uniform_at(a.table, row + min(key >> a.shift, last));
-      const bool ok = page >= 0 && page < a.pages;
+      const int key = istep * kMxStep + 16 * h;
+      const bool ok = ipage[h] >= 0 && ipage[h] < a.pages;
       if (!ok) holes[d] |= 1u << h;
-      at[h] = ((static_cast<long long>(ok ? page : 0) * a.hkv + kvh) << a.shift) +
-              (key & ((1 << a.shift) - 1));
-      const uint8_t* kp = a.kc + at[h] * CB + k_at;
+      const uint64_t off = static_cast<uint64_t>(ok ? ipage[h] : 0) * a.page_bytes +
+                           static_cast<uint32_t>((to.kvh << a.shift) + (key & ((1 << a.shift) - 1))) * CB;
+      static_assert(CB == 16 * SB, "scales lie as the codes do");
+      kp[h] = mx_base(a.kc, off);
+      vp[h] = mx_base(a.vc, off);
+      ksp[h] = mx_base(a.ks, off / 16);
+      vsp[h] = mx_base(a.vs, off / 16);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       if constexpr (HD == 128) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
+        const u32x4 w = mx_load<u32x4>(kp[h] + k_at);
         stage[d].k[h][0] = w.x; stage[d].k[h][1] = w.y;
         stage[d].k[h][2] = w.z; stage[d].k[h][3] = w.w;
       } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
+        const u32x2 w = mx_load<u32x2>(kp[h] + k_at);
         stage[d].k[h][0] = w.x; stage[d].k[h][1] = w.y;
       }
-      stage[d].ks[h] = a.ks[at[h] * SB + ks_at];
+      stage[d].ks[h] = ksp[h][ks_at];
     }
     if constexpr (HD == 128) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        stage[d].v[j] = *reinterpret_cast<const u32x4*>(a.vc + at[j] * CB + v_at);
-        stage[d].vs[j] = a.vs[at[j] * SB + vs_at];
+        stage[d].v[j] = mx_load<u32x4>(vp[j] + v_at);
+        stage[d].vs[j] = vsp[j][vs_at];
       }
     } else {
-      const long long mine = lane < 32 ? at[0] : at[1];
-      stage[d].v[0] = *reinterpret_cast<const u32x4*>(a.vc + mine * CB + v_at);
-      stage[d].vs[0] = a.vs[mine * SB + vs_at];
+      stage[d].v[0] = mx_load<u32x4>((lane < 32 ? vp[0] : vp[1]) + v_at);
+      stage[d].vs[0] = (lane < 32 ? vsp[0] : vsp[1])[vs_at];
     }
+    more = more && advance(to);
+    look();
   };
 
   // LDS offsets: this lane's V row(s) and its transposing reads
-  const int v_row = lane / CPR, v_ch = 4 * (lane % CPR);
-  uint32_t vput[4], voff[ND];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) vput[i] = v_row * RB + 16 * ((v_ch + i) ^ mx_swz(v_row));
-#pragma unroll
-  for (int d = 0; d < ND; ++d) {
-    const int row = 4 * g + (col >> 2), dim = 16 * d + 4 * (col & 3);
-    voff[d] = row * RB + 16 * ((dim >> 3) ^ mx_swz(row)) + 2 * (dim & 7);
-  }
-
-  int issued = 0;
-#pragma unroll
-  for (int d = 0; d < kMxAhead; ++d)
-    if (d < count) {
-      if (d) next(ib, iu, is, icur);
-      issue(d);
-      ++issued;
-    }
+  // (chunk c of a row lies at c ^ swz, which the bits of c over and under split)
+  const int v_row = lane / CPR, v_ch = 4 * (lane % CPR), t_row = 4 * g + (col >> 2);
+  const uint32_t vput = v_row * RB + 16 * (v_ch ^ mx_swz(v_row));
+  const uint32_t vget = base + t_row * RB + 16 * (((col >> 1) & 1) ^ mx_swz(t_row)) + 8 * (col & 1);
 
   uint4 qf[NT][NS];
   f32x4 acc[NT][ND];
   float m_run[NT], l_run[NT], slope[NT];
   int lo[NT], end[NT];  // what each column sees
-  bool fresh = true;
+  bool rough[NT];       // some column's offset is as large as below
+  const auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m_run[n] = -INFINITY;
-    l_run[n] = slope[n] = 0.f;
-    lo[n] = end[n] = 0;
+    for (int n = 0; n < NT; ++n) {
+      const int c = min(16 * (NT * at.ht + n) + col, TG - 1), t = a.T == 1 ? 0 : c / a.G;
+      const int h = at.kvh * a.G + c - t * a.G;
+      end[n] = at.len - (a.T - 1 - t);
+      lo[n] = a.window > 0 ? max(0, end[n] - a.window) : 0;
+      const uint16_t* qp = a.q + at.b * a.qb + t * a.qt + h * a.qh + g * (HD / 4);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  auto step = [&](int d, int i) __attribute__((always_inline)) {
-    const int kvh = u / a.HT, ht = u - kvh * a.HT;
-    if (fresh) {
-      fresh = false;
+      for (int x = 0; x < NS; ++x) qf[n][x] = *reinterpret_cast<const uint4*>(qp + 8 * x);
+      slope[n] = a.slopes ? slope_log2(a.slopes[h], kMaxSlope) : 0.f;
+      m_run[n] = -INFINITY;
+      l_run[n] = 0.f;
+      rough[n] = true;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int c = min(16 * (NT * ht + n) + col, TG - 1), t = c / a.G;
-        const int h = kvh * a.G + c - t * a.G;
-        end[n] = cur.len - (a.T - 1 - t);
-        lo[n] = a.window > 0 ? max(0, end[n] - a.window) : 0;
-        const uint16_t* qp = a.q + b * a.qb + t * a.qt + h * a.qh + g * (HD / 4);
-#pragma unroll
-        for (int x = 0; x < NS; ++x) qf[n][x] = *reinterpret_cast<const uint4*>(qp + 8 * x);
-        if (a.slopes) slope[n] = slope_log2(a.slopes[h], kMaxSlope);
-        m_run[n] = -INFINITY;
-        l_run[n] = 0.f;
-#pragma unroll
-        for (int x = 0; x < ND; ++x) acc[n][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+      for (int x = 0; x < ND; ++x) acc[n][x] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+  };
+  // waited for before a tile's rounds: left pending, each of them would wait as its first does
+  const auto settle = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < NS; ++x)
+        asm volatile("" : "+v"(qf[n][x].x), "+v"(qf[n][x].y), "+v"(qf[n][x].z), "+v"(qf[n][x].w));
+      asm volatile("" : "+v"(slope[n]));
+    }
+  };
+  look();
+  begin();
+#pragma unroll
+  for (int d = 0; d < kMxAhead; ++d) issue(d);
+  settle();
+
+  const bool special = a.cap_x2 > 0.f || a.slopes;
+  const auto step = [&](int d, int s) __attribute__((always_inline)) {
     const int key0 = s * kMxStep;
     const unsigned hole = holes[d];
     // whether some column does not see some key of the step
-    const bool edge = (a.window > 0 && key0 < cur.len - a.window) ||
-                      key0 + kMxStep > cur.len - (a.T - 1) || hole;
+    const bool edge = (a.window > 0 && key0 < at.len - a.window) ||
+                      key0 + kMxStep > at.len - (a.T - 1) || hole;
     MxStage<HD>& st = stage[d];
 
     f32x4 sc[NT][2];
@@ -334,7 +418,7 @@ void mx4_attn_kernel(const Mx4Args a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int row = 16 * j + v_row, key = key0 + row;
-        if (key < cur.lo || key >= cur.len || ((hole >> (row >> 4)) & 1u)) {
+        if (key < at.lo || key >= at.len || ((hole >> (row >> 4)) & 1u)) {
           st.v[j] = u32x4{0u, 0u, 0u, 0u};
           st.vs[j] = kMxOne;
         }
@@ -369,41 +453,54 @@ void mx4_attn_kernel(const Mx4Args a) {
       const uint32_t w[4] = {st.v[j].x, st.v[j].y, st.v[j].z, st.v[j].w};
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        *reinterpret_cast<uint4*>(mem + 16 * j * RB + vput[x]) = mx4_to_bf16(w[x], st.vs[j]);
-    }
-    if (issued < count) {
-      next(ib, iu, is, icur);
-      issue(d);
-      ++issued;
+        *reinterpret_cast<uint4*>(mem + 16 * j * RB + (vput ^ (16 * x))) = mx4_to_bf16(w[x], st.vs[j]);
     }
     wave_lds_order();
-    u32x2 vf[2 * ND];
-#pragma unroll
-    for (int x = 0; x < ND; ++x) {
-      vf[2 * x] = lds_get_tr16(base + voff[x]);
-      vf[2 * x + 1] = lds_get_tr16(base + voff[x] + 16 * RB);
-    }
+    issue(d);
 
+    uint4 pb[NT], pl[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float z[8];
+      // scores: products to scale by `mul`, or, where more is done to them, in log2 units
+      float z[8], mul = a.scale_log2;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = sc[n][j >> 2][j & 3];
+      float least = kMxLowest;
+      if (special || edge) {
+        mul = 1.f;
+        if (a.cap_x2 > 0.f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) z[j] = softcap_log2(z[j] * a.cap_x2, a.cap_log2);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) z[j] *= a.scale_log2;
+        }
+        const int key = key0 + 4 * g;
+        if (a.slopes) {
+          const float far = static_cast<float>(end[n] - 1 - key);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            z[j] -= slope[n] * (far - static_cast<float>(16 * (j >> 2) + (j & 3)));
+        }
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int at_key = key + 16 * (j >> 2) + (j & 3);
+            const bool seen = at_key >= lo[n] && at_key < end[n] && !((hole >> (j >> 2)) & 1u);
+            z[j] = seen ? z[j] : -INFINITY;
+          }
+          const auto shows = [&](int h) {
+            const int from = key0 + 16 * h;
+            return !((hole >> h) & 1u) && max(from, lo[n]) < min(from + 16, end[n]);
+          };
+          least = shows(0) || shows(1) ? kMxLowest : -INFINITY;
+        }
+      }
       // a step with a visible key lifts the maximum to the lowest finite number, also if they
       // all score -inf: softmax over such alone is NaN, over no key it gives zeros
-      const auto shows = [&](int h) {
-        const int first = key0 + 16 * h;
-        return !((hole >> h) & 1u) && max(first, lo[n]) < min(first + 16, end[n]);
-      };
-      float mloc = !edge || shows(0) || shows(1) ? kMxLowest : -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float x = sc[n][j >> 2][j & 3];
-        x = a.cap_x2 > 0.f ? softcap_log2(x * a.cap_x2, a.cap_log2) : x * a.scale_log2;
-        const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-        if (a.slopes) x -= slope[n] * static_cast<float>(end[n] - 1 - key);
-        if (edge && (key < lo[n] || key >= end[n] || ((hole >> (j >> 2)) & 1u))) x = -INFINITY;
-        z[j] = x;
-        mloc = fmaxf(mloc, x);
-      }
+      float mloc = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])),
+                         fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+      mloc = fmaxf(mloc * mul, least);
       // the offset moves only when some score passes it by more than 8 (weights stay
       // below 2^8), decided by the wave; all four lanes of a column take the same one
       if (__ballot(!(mloc <= m_run[n] + 8.f))) {
@@ -412,76 +509,53 @@ void mx4_attn_kernel(const Mx4Args a) {
         const float m_new = fmaxf(m_run[n], mloc);
         const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m_run[n] - m_new);
         m_run[n] = m_new;
+        rough[n] = __ballot(!(fabsf(m_new) < 0x1p20f)) != 0;
         l_run[n] *= alpha;
 #pragma unroll
         for (int x = 0; x < ND; ++x) acc[n][x] *= alpha;
       }
-      const float m_sub = m_run[n] == -INFINITY ? 0.f : m_run[n];
+      // One rounding for product and difference, which leaves all weights the same factor from
+      // the offset's own; not so where that is 2^20 or more, and the factor any
+      if (rough[n]) {
+#pragma clang fp contract(off)
+        const float m_sub = m_run[n] == -INFINITY ? 0.f : m_run[n];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = z[j] * mul - m_sub;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = fmaf(z[j], mul, -m_run[n]);
+      }
       // the weights as a sum of two bf16, the first cut off
       uint32_t h8[8];
       float lo8[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float p = exp2_fast(z[j] - m_sub);
+        const float p = exp2_fast(z[j]);
         l_run[n] += p;
         h8[j] = __float_as_uint(p) & 0xffff0000u;
         lo8[j] = p - __uint_as_float(h8[j]);
       }
-      const uint4 pb = uint4{h8[0] >> 16 | h8[1], h8[2] >> 16 | h8[3], h8[4] >> 16 | h8[5],
-                             h8[6] >> 16 | h8[7]};
-      const uint4 pl = pack8_bf16(lo8);
-#pragma unroll
-      for (int x = 0; x < ND; ++x) {
-        const bf16x8 vv = as_bf16x8(uint4{vf[2 * x].x, vf[2 * x].y, vf[2 * x + 1].x, vf[2 * x + 1].y});
-        acc[n][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pb), acc[n][x], 0, 0, 0);
-        acc[n][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pl), acc[n][x], 0, 0, 0);
-      }
+      pb[n] = uint4{h8[0] >> 16 | h8[1], h8[2] >> 16 | h8[3], h8[4] >> 16 | h8[5],
+                    h8[6] >> 16 | h8[7]};
+      pl[n] = pack8_bf16(lo8);
     }
-
-    const bool head_end = s + 1 == cur.s1;
-    if (W == 1 && (head_end || i + 1 == count)) {
-      // whole: the head's first step lies in this run too
-      const bool whole = head_end && i >= s - cur.s0;
+#pragma unroll
+    for (int x = 0; x < ND; ++x) {
+      const uint32_t from = (vget ^ (32 * (x & 3))) + 128 * (x >> 2);
+      const u32x2 v0 = lds_get_tr16(from), v1 = lds_get_tr16(from + 16 * RB);
+      const bf16x8 vv = as_bf16x8(uint4{v0.x, v0.y, v1.x, v1.y});
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int c = 16 * (NT * ht + n) + col;
-        float l = l_run[n] + __shfl_xor(l_run[n], 16, kWave);
-        l += __shfl_xor(l, 32, kWave);
-        if (c >= TG) continue;
-        if (whole) {
-          const float f = mx_share(m_run[n], l);
-          const int t = c / a.G, h = kvh * a.G + c - t * a.G;
-          uint16_t* o = a.out + ((static_cast<long long>(b) * a.T + t) * a.hq + h) * HD + 4 * g;
-#pragma unroll
-          for (int x = 0; x < ND; ++x)
-            *reinterpret_cast<uint2*>(o + 16 * x) =
-                make_uint2(pack_bf2(acc[n][x][0] * f, acc[n][x][1] * f),
-                           pack_bf2(acc[n][x][2] * f, acc[n][x][3] * f));
-        } else {
-          // the run starts in this head (or at its first step): 0; else it ends in it: 1
-          const int part = i > s - cur.s0 ? 1 : 0;
-          const long long at = (2ll * blockIdx.x + part) * a.GT + c - 16 * NT * ht;
-          float* o = a.po + at * HD + 4 * g;
-#pragma unroll
-          for (int x = 0; x < ND; ++x)
-            *reinterpret_cast<float4*>(o + 16 * x) =
-                make_float4(acc[n][x][0], acc[n][x][1], acc[n][x][2], acc[n][x][3]);
-          if (g == 0) *reinterpret_cast<float2*>(a.pml + 2 * at) = make_float2(m_run[n], l);
-        }
+        acc[n][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pb[n]), acc[n][x], 0, 0, 0);
+        acc[n][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, as_bf16x8(pl[n]), acc[n][x], 0, 0, 0);
       }
-      fresh = true;
     }
-    if (i + 1 < count) next(b, u, s, cur);
   };
-  for (int i = 0; i < count; i += kMxAhead) {
-#pragma unroll
-    for (int d = 0; d < kMxAhead; ++d)
-      if (i + d < count) step(d, i + d);
-  }
 
-  if constexpr (W > 1) {
-    // the waves' (m, l, O) joined through each one's LDS, which it has done with
-    const int kvh = u / a.HT, ht = u - kvh * a.HT;
+  // The waves' (m, l, O) of a head tile joined through each one's LDS: to the output where the
+  // run has all of its steps, else to the workspace, where the run's first tile takes place 0
+  // and its last one place 1.
+  const auto join = [&](bool first) __attribute__((always_inline)) {
     wave_lds_order();
     float* const so = reinterpret_cast<float*>(mem);
 #pragma unroll
@@ -497,7 +571,8 @@ void mx4_attn_kernel(const Mx4Args a) {
             make_float2(m_run[n], l);
     }
     __syncthreads();
-    const int cols = min(16 * NT, TG - 16 * NT * ht);
+    const bool whole = at.begin == at.lo / kMxStep && at.end == (at.len + kMxStep - 1) / kMxStep;
+    const int cols = min(16 * NT, TG - 16 * NT * at.ht);
     for (int e = threadIdx.x; e < cols * (HD / 4); e += 64 * W) {
       const int c = e / (HD / 4), x = 4 * (e - c * (HD / 4));
       float mx = -INFINITY;
@@ -519,87 +594,132 @@ void mx4_attn_kernel(const Mx4Args a) {
         sum.z += mx_weighted(y.z, f);
         sum.w += mx_weighted(y.w, f);
       }
-      const float r = mx_share(mx, den);
-      const int ci = 16 * NT * ht + c, t = ci / a.G, h = kvh * a.G + ci - t * a.G;
-      *reinterpret_cast<uint2*>(a.out + ((static_cast<long long>(b) * a.T + t) * a.hq + h) * HD + x) =
-          make_uint2(pack_bf2(sum.x * r, sum.y * r), pack_bf2(sum.z * r, sum.w * r));
+      if (whole) {
+        const float r = mx_share(mx, den);
+        const int ci = 16 * NT * at.ht + c, t = a.T == 1 ? 0 : ci / a.G;
+        const int h = at.kvh * a.G + ci - t * a.G;
+        *reinterpret_cast<uint2*>(a.out + ((static_cast<long long>(at.b) * a.T + t) * a.hq + h) * HD + x) =
+            make_uint2(pack_bf2(sum.x * r, sum.y * r), pack_bf2(sum.z * r, sum.w * r));
+      } else {
+        const long long i = (2ll * blockIdx.x + (first ? 0 : 1)) * a.GT + c;
+        *reinterpret_cast<float4*>(a.po + i * HD + x) = sum;
+        if (x == 0) *reinterpret_cast<float2*>(a.pml + 2 * i) = make_float2(mx, den);
+      }
     }
+  };
+
+  // A tile's rounds by twos, so that each stage keeps its registers, in a loop of one exit: past
+  // a second one the compiler would again wait for all loads.  An odd round leaves the stages
+  // in the other order.
+  static_assert(kMxAhead == 2, "the loop below");
+  for (bool first = true;; first = false) {
+    const int rounds = (at.end - at.begin + W - 1) / W;
+    int s = at.begin + wave;
+    for (int r = rounds >> 1; r > 0; --r, s += 2 * W) {
+      step(0, s);
+      step(1, s + W);
+    }
+    if (rounds & 1) step(0, s);
+    join(first);
+    at.it = rounds - 1;
+    if (!advance(at)) break;
+    if (rounds & 1) {
+      const MxStage<HD> later = stage[0];
+      stage[0] = stage[1];
+      stage[1] = later;
+      const unsigned hole = holes[0];
+      holes[0] = holes[1];
+      holes[1] = hole;
+    }
+    __syncthreads();  // before its parts are written over
+    begin();
+    settle();
   }
 }
 
-// Joins the partials of one (sequence, token, query head): o = sum_i 2^(m_i - m) O_i /
-// sum_i 2^(m_i - m) l_i, in the runs' order within each of T / (HD / 4) lane groups and
-// then over the groups, so the result does not depend on timing.
-template <int HD, int TH>
-__global__ __launch_bounds__(TH) void mx4_join_kernel(const Mx4Args a, int cols) {
-  constexpr int LPP = HD / 4;       // lanes a partial
-  constexpr int NG = TH / LPP;
-  __shared__ __align__(16) float so[NG][HD];
-  __shared__ float sm[NG], sl[NG];
-  const int grp = threadIdx.x / LPP, c = threadIdx.x % LPP;
-  const int bt = blockIdx.x / a.hq, h = blockIdx.x - bt * a.hq;
-  const int b = bt / a.T, t = bt - b * a.T;
-  const int kvh = h / a.G, ci = t * a.G + h - kvh * a.G, ht = ci / cols, row = ci - ht * cols;
-  const int units = a.hkv * a.HT, u = kvh * a.HT + ht;
-  uint16_t* out = a.out + static_cast<long long>(blockIdx.x) * HD;
+// Joins the partials of one (sequence, head tile): o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i -
+// m) l_i, for kMxJoinCols of its columns a workgroup, in the runs' order within each of a number
+// of lane groups and then over the groups, so the result does not depend on timing.
+constexpr int kMxJoin = 512, kMxJoinCols = 8;
 
+template <int HD>
+__global__ __launch_bounds__(kMxJoin) void mx4_join_kernel(const Mx4Args a, int cols, int parts) {
+  constexpr int LPP = HD / 4;                       // lanes a column
+  constexpr int ITEMS = kMxJoinCols * LPP, GROUPS = kMxJoin / ITEMS;
+  __shared__ __align__(16) float so[kMxJoin][4];
+  __shared__ float2 sml[kMxJoin];
+  const int units = a.hkv * a.HT;
+  const int tile = blockIdx.x / parts, row = (blockIdx.x - tile * parts) * kMxJoinCols +
+                                             threadIdx.x % ITEMS / LPP;
+  const int b = tile / units, u = tile - b * units;
+  const int kvh = u / a.HT, ht = u - kvh * a.HT;
   const int start = uniform_at(a.starts, b), n = uniform_at(a.starts, b + 1) - start;
-  if (n == 0) {  // nothing visible: zeros
-    if (threadIdx.x < LPP) *reinterpret_cast<uint2*>(out + 4 * c) = make_uint2(0u, 0u);
-    return;
-  }
   const int q = mx_run(static_cast<long long>(uniform_at(a.starts, a.B)) * units, a.runs);
   const long long first = static_cast<long long>(start) * units + static_cast<long long>(u) * n;
-  const int w0 = static_cast<int>(first / q), w1 = static_cast<int>((first + n - 1) / q);
+  // the runs of its first and last step
+  const int w0 = static_cast<int>((first + kMxPad) / q);
+  const int w1 = n ? static_cast<int>((first + n - 1) / q) : -1;
   if (w0 == w1) return;  // stored by its run
+  const int ci = cols * ht + row, c = threadIdx.x % LPP, grp = threadIdx.x / ITEMS;
+  const bool here = row < cols && ci < a.T * a.G;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int w = w0 + grp; w <= w1; w += NG) {
-    const int part = w == w0 && first != static_cast<long long>(w0) * q ? 1 : 0;
-    const long long i = (2ll * w + part) * a.GT + row;
-    const float2 ml = *reinterpret_cast<const float2*>(a.pml + 2 * i);
-    const float4 x = *reinterpret_cast<const float4*>(a.po + i * HD + 4 * c);
-    const float m_new = fmaxf(m, ml.x);
-    const float m_sub = m_new == -INFINITY ? 0.f : m_new;
-    const float f = exp2_fast(m - m_sub), e = exp2_fast(ml.x - m_sub);
-    m = m_new;
-    l = fmaf(ml.y, e, l * f);  // NaN of a NaN score, whatever its part's weight
-    o.x = mx_weighted(x.x, e) + mx_weighted(o.x, f);
-    o.y = mx_weighted(x.y, e) + mx_weighted(o.y, f);
-    o.z = mx_weighted(x.z, e) + mx_weighted(o.z, f);
-    o.w = mx_weighted(x.w, e) + mx_weighted(o.w, f);
-  }
-  *reinterpret_cast<float4*>(&so[grp][4 * c]) = o;
-  if (c == 0) {
-    sm[grp] = m;
-    sl[grp] = l;
-  }
-  __syncthreads();
-  float mx = sm[0];
-#pragma unroll
-  for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[i]);
-  const float m_sub = mx == -INFINITY ? 0.f : mx;
-  for (int d = threadIdx.x; d < HD; d += TH) {
-    float num = 0.f, den = 0.f;
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const float e = exp2_fast(sm[i] - m_sub);
-      den = fmaf(sl[i], e, den);
-      num += mx_weighted(so[i][d], e);
+  if (here) {
+#pragma unroll 4
+    for (int w = w0 + grp; w <= w1; w += GROUPS) {
+      const int part = w == w0 && first > static_cast<long long>(w0) * q ? 1 : 0;
+      const long long i = (2ll * w + part) * a.GT + row;
+      const float2 ml = *reinterpret_cast<const float2*>(a.pml + 2 * i);
+      const float4 x = *reinterpret_cast<const float4*>(a.po + i * HD + 4 * c);
+      const float m_new = fmaxf(m, ml.x);
+      const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+      const float f = exp2_fast(m - m_sub), y = exp2_fast(ml.x - m_sub);
+      m = m_new;
+      l = fmaf(ml.y, y, l * f);  // NaN of a NaN score, whatever its part's weight
+      o.x = mx_weighted(x.x, y) + mx_weighted(o.x, f);
+      o.y = mx_weighted(x.y, y) + mx_weighted(o.y, f);
+      o.z = mx_weighted(x.z, y) + mx_weighted(o.z, f);
+      o.w = mx_weighted(x.w, y) + mx_weighted(o.w, f);
     }
-    out[d] = f2bf(num * mx_share(mx, den));
   }
+  *reinterpret_cast<float4*>(so[threadIdx.x]) = o;
+  sml[threadIdx.x] = make_float2(m, l);
+  __syncthreads();
+  if (grp > 0 || !here) return;
+  float mx = m;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) mx = fmaxf(mx, sml[threadIdx.x + i * ITEMS].x);
+  const float m_sub = mx == -INFINITY ? 0.f : mx, f = exp2_fast(m - m_sub);
+  l *= f;
+  o = make_float4(mx_weighted(o.x, f), mx_weighted(o.y, f), mx_weighted(o.z, f),
+                  mx_weighted(o.w, f));
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) {
+    const float2 ml = sml[threadIdx.x + i * ITEMS];
+    const float4 x = *reinterpret_cast<const float4*>(so[threadIdx.x + i * ITEMS]);
+    const float y = exp2_fast(ml.x - m_sub);
+    l = fmaf(ml.y, y, l);
+    o.x += mx_weighted(x.x, y);
+    o.y += mx_weighted(x.y, y);
+    o.z += mx_weighted(x.z, y);
+    o.w += mx_weighted(x.w, y);
+  }
+  const float r = mx_share(mx, l);  // (without a part, a sequence of length 0: zeros)
+  const int t = ci / a.G, h = kvh * a.G + ci - t * a.G;
+  *reinterpret_cast<uint2*>(a.out + ((static_cast<long long>(b) * a.T + t) * a.hq + h) * HD + 4 * c) =
+      make_uint2(pack_bf2(o.x * r, o.y * r), pack_bf2(o.z * r, o.w * r));
 }
 
 struct Mx4Plan {
   int G, HT, GT, NT, runs;
-  bool wide;  // a workgroup a head tile, its waves every 8th (4th) step; else runs and their join
+  int W;  // waves of a workgroup: of a whole head tile (runs 0), or of a run, whose parts are joined
   long long cap_len, groups, ws;
 };
 
-inline bool mx4_plan(int B, int T, int Hq, int Hkv, int hd, int width, int page, Mx4Plan* p) {
+inline bool mx4_plan(int B, int T, int Hq, int Hkv, int hd, int width, int page, int window,
+                     Mx4Plan* p) {
   if (B < 0 || T < 1 || T > 64 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > kMaxHeads ||
-      (hd != 64 && hd != 128) || width < 0 || page_shift(page) < 0)
+      (hd != 64 && hd != 128) || width < 0 || page_shift(page) < 0 || window < 0)
     return false;
   p->G = Hq / Hkv;
   const int tg = T * p->G;
@@ -609,35 +729,54 @@ inline bool mx4_plan(int B, int T, int Hq, int Hkv, int hd, int width, int page,
   p->GT = tg < cols ? tg : cols;
   p->cap_len = static_cast<long long>(width) * page;
   if (p->cap_len >= (1ll << 31) - kMxStep) return false;  // positions are 32-bit
-  const long long units = static_cast<long long>(B) * Hkv * p->HT;
-  const int W = p->NT == 1 ? 8 : 4;
-  const long long deep = (p->cap_len + kMxStep * W - 1) / (kMxStep * W);
-  p->wide = deep <= 4 || (W == 8 && deep <= 8 && 2 * units >= compute_units());
-  p->runs = p->wide ? 0 : compute_units() * (p->NT == 1 ? 8 : 4);
-  p->groups = p->wide ? units : p->runs;
-  p->ws = p->wide ? 0
-                  : 2ll * p->runs * p->GT * (hd + 2) * 4 + (static_cast<long long>(B) + 1) * 4;
+  const long long units = static_cast<long long>(B) * Hkv * p->HT, cus = compute_units();
+  // Whole head tiles by workgroups need one launch and no parts, but take as long as the longest
+  // of them.  By rounds of four waves that the table (or the window) can fill; us of four waves a
+  // tile / a CU's waves / runs, lengths even: 16 heads over 4 x 64, one sequence of 1000
+  // tokens 13 / 14 / 17, 2000 19 / 17 / 17, 4000 34 / 24 / 17; 64 of them 13 / 25 / 20, 21 /
+  // 29 / 23, 36 / 37 / 31; 32 heads over 8 x 128, 1 x 1000 16 / 14 / 17, 64 x 1000 22 / 33 /
+  // 31, 2000 35 / 46 / 42 (ragged 31 / 39 / 32), 4000 62 / 74 / 64 (ragged 54 / 58 / 44).
+  // Two column tiles a wave (8 tokens): 4 x 64, 16 x 1000 22 / 19 / 28, 2000 31 / 26 / 33, 4000
+  // 51 / 38 / 37; 8 x 128, 64 x 1000 31 / 40 / 46, 2000 50 / 58 / 64.
+  const long long seen = window > 0 && window + T < p->cap_len ? window + T : p->cap_len;
+  const long long rounds = (seen + 4 * kMxStep - 1) / (4 * kMxStep);
+  const int most = 4 * mx4_waves(hd, p->NT);
+  bool whole;
+  if (units >= cus && (p->NT == 1 || hd == 128)) {
+    whole = rounds <= 16;
+    p->W = 4;
+  } else if (p->NT == 1) {
+    whole = rounds <= 8;
+    p->W = hd == 64 || 2 * units > cus || rounds <= 4 ? 4 : most;
+  } else {
+    whole = rounds <= 16;
+    p->W = most;
+  }
+  if (!whole) p->W = 4;
+  p->runs = whole ? 0 : static_cast<int>(cus) * mx4_waves(hd, p->NT);
+  p->groups = whole ? units : p->runs;
+  p->ws = whole ? 0
+                : 2ll * p->runs * p->GT * (hd + 2) * 4 + (static_cast<long long>(B) + 1) * 4;
   // all steps, a run's steps and the grids are 32-bit
-  const double steps = static_cast<double>(B) * (p->cap_len / kMxStep + 1);
+  const double steps = static_cast<double>(B) * (p->cap_len / kMxStep + 1 + kMxPad);
   return steps < 2147483647. &&
-         (p->wide || steps * Hkv * p->HT / p->runs < 2147483647.) && p->groups < (1ll << 31) &&
-         static_cast<double>(B) * T * Hq < 2147483647.;
+         (whole || steps * Hkv * p->HT / p->runs < 2147483647.) && p->groups < (1ll << 31) &&
+         static_cast<double>(B) * T * Hq < 2147483647. && 4 * units < (1ll << 31);
 }
 
 template <int HD, int NT>
 int32_t launch_mx4(const Mx4Args& a, const Mx4Plan& p, hipStream_t s) {
-  constexpr int W = NT == 1 ? 8 : 4;
+  constexpr int MOST = 4 * mx4_waves(HD, NT);
   const dim3 grid(static_cast<unsigned>(p.groups));
-  if (p.wide) {
-    hipLaunchKernelGGL((mx4_attn_kernel<HD, NT, W>), grid, dim3(64 * W), 0, s, a);
-    return launch_status();
-  }
-  const dim3 heads(static_cast<unsigned>(a.B) * a.T * a.hq);
-  hipLaunchKernelGGL((mx4_attn_kernel<HD, NT, 1>), grid, dim3(64), 0, s, a);
-  if (heads.x >= 1024)
-    hipLaunchKernelGGL((mx4_join_kernel<HD, 64>), heads, dim3(64), 0, s, a, 16 * NT);
+  if (p.W == 4)
+    hipLaunchKernelGGL((mx4_attn_kernel<HD, NT, 4>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((mx4_join_kernel<HD, 512>), heads, dim3(512), 0, s, a, 16 * NT);
+    hipLaunchKernelGGL((mx4_attn_kernel<HD, NT, MOST>), grid, dim3(64 * MOST), 0, s, a);
+  if (p.runs == 0) return launch_status();
+  const int parts = (p.GT + kMxJoinCols - 1) / kMxJoinCols;
+  hipLaunchKernelGGL(mx4_join_kernel<HD>,
+                     dim3(static_cast<unsigned>(a.B) * a.hkv * a.HT * parts), dim3(kMxJoin), 0, s,
+                     a, 16 * NT, parts);
   return launch_status();
 }
 
@@ -647,9 +786,10 @@ using namespace llmy;
 
 extern "C" int64_t llmy_paged_attn_mx4_workspace_bytes(int32_t B, int32_t T, int32_t Hq,
                                                        int32_t Hkv, int32_t head_dim,
-                                                       int32_t width, int32_t page) {
+                                                       int32_t width, int32_t page,
+                                                       int32_t window) {
   Mx4Plan p;
-  return mx4_plan(B, T, Hq, Hkv, head_dim, width, page, &p) ? p.ws : -1;
+  return mx4_plan(B, T, Hq, Hkv, head_dim, width, page, window, &p) ? p.ws : -1;
 }
 
 extern "C" int32_t llmy_paged_attn_mx4(
@@ -660,8 +800,8 @@ extern "C" int32_t llmy_paged_attn_mx4(
     int32_t width, int32_t page, int32_t pages, int32_t window, float scale, float softcap,
     void* stream) {
   Mx4Plan p;
-  LLMY_REQUIRE(mx4_plan(B, T, Hq, Hkv, head_dim, width, page, &p));
-  LLMY_REQUIRE(pages >= 0 && window >= 0 && scale_ok(scale, softcap));
+  LLMY_REQUIRE(mx4_plan(B, T, Hq, Hkv, head_dim, width, page, window, &p));
+  LLMY_REQUIRE(pages >= 0 && scale_ok(scale, softcap));
   if (B == 0) return 0;
   LLMY_REQUIRE(q && out && lengths && aligned(q, 16) && aligned(out, 16));
   LLMY_REQUIRE(q_seq % 8 == 0 && q_row % 8 == 0 && q_head % 8 == 0 && q_seq >= 0 && q_row >= 0 &&
@@ -697,6 +837,7 @@ extern "C" int32_t llmy_paged_attn_mx4(
   a.B = B; a.T = T; a.hq = Hq; a.hkv = Hkv; a.G = p.G; a.HT = p.HT; a.GT = p.GT;
   a.width = width; a.shift = page_shift(page); a.pages = pages; a.window = window;
   a.cap_len = pages ? static_cast<int>(p.cap_len) : 0;
+  a.page_bytes = static_cast<uint32_t>(Hkv) * page * (head_dim / 2);
   a.runs = p.runs;
   const hipStream_t s = as_stream(stream);
   if (head_dim == 64)

@@ -660,7 +660,7 @@ def paged_attn_mx4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError(f"page_table must be [{B}, pages], got {tuple(page_table.shape)}")
     pl, ps = _vec(lengths, "lengths", _I32, B, dev), _vec(slopes, "slopes", _F32, Hq, dev)
     out = _out(out, q, dev)
-    nbytes = _lib.load().llmy_paged_attn_mx4_workspace_bytes(B, T, Hq, Hkv, hd, width, page)
+    nbytes = _lib.load().llmy_paged_attn_mx4_workspace_bytes(B, T, Hq, Hkv, hd, width, page, window)
     workspace, pw, have = _workspace(workspace, nbytes, q, dev)
     _lib.call("llmy_paged_attn_mx4", q.data_ptr(), st[0], st[1] if len(shape) == 4 else 0, st[-2],
               *cache, pt, pl, ps, out.data_ptr(), pw, have, B, T, Hq, Hkv, hd, width, page, pages,

@@ -293,7 +293,8 @@ int32_t llmy_paged_kv_read_mx4(const void* k_cache, const void* v_cache, const v
 /* Workspace (bytes) of llmy_paged_attn_mx4 for these sizes; -1 where that call refuses them,
  * 0 where it takes none.  No two calls that may overlap share one. */
 int64_t llmy_paged_attn_mx4_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
-                                            int32_t head_dim, int32_t width, int32_t page);
+                                            int32_t head_dim, int32_t width, int32_t page,
+                                            int32_t window);
 
 /* Attention of the last T tokens (1 to 64) of each sequence over a 4-bit cache that holds
  * them already: q [B, T, Hq, head_dim] (strides in elements, multiples of 8, 16-byte aligned),

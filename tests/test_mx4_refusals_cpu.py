@@ -95,10 +95,12 @@ def test_attention_refuses(lib, over):
 def test_attention_of_nothing_and_its_workspace(lib):
     assert attn(lib, B=0) == 0
     size = lib.llmy_paged_attn_mx4_workspace_bytes
-    assert size(2, 1, 4, 2, 64, 4, 16) == 0           # short: none
-    assert size(2, 1, 4, 2, 64, 1024, 16) > 0
-    assert size(2, 1, 4, 3, 64, 4, 16) == -1
-    assert size(2, 0, 4, 2, 64, 4, 16) == -1
+    assert size(2, 1, 4, 2, 64, 4, 16, 0) == 0           # short: none
+    assert size(2, 1, 4, 2, 64, 1024, 16, 0) > 0
+    assert size(2, 1, 4, 2, 64, 1024, 16, 64) == 0    # short by its window
+    assert size(2, 1, 4, 3, 64, 4, 16, 0) == -1
+    assert size(2, 0, 4, 2, 64, 4, 16, 0) == -1
+    assert size(2, 1, 4, 2, 64, 4, 16, -1) == -1
 
 
 def plan(lib, **over):
