@@ -132,6 +132,13 @@ __device__ __forceinline__ int mx_swz(int row) { return 2 * (row & 3) | ((row >>
 
 // What one step loads: a 16-key tile's codes (a lane: its key's quarter of the dims) and the
 // scale byte over them, twice; V's codes by 16 bytes with theirs.
+template <class T>
+__device__ __forceinline__ void mx_swap(T& a, T& b) {
+  const T t = a;
+  a = b;
+  b = t;
+}
+
 template <int HD>
 struct MxStage {
   static constexpr int NV = HD / 64;
@@ -139,10 +146,28 @@ struct MxStage {
   uint32_t ks[2];
   u32x4 v[NV];
   uint32_t vs[NV];
+
+  __device__ __forceinline__ void swap(MxStage& o) {  // (whole structures would go through memory)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) mx_swap(k[i][j], o.k[i][j]);
+      mx_swap(ks[i], o.ks[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      mx_swap(v[i], o.v[i]);
+      mx_swap(vs[i], o.vs[i]);
+    }
+  }
 };
 
 // Waves a SIMD: as many as the registers of each form take.
 constexpr int mx4_waves(int hd, int nt) { return hd == 64 ? (nt == 1 ? 3 : 2) : nt == 1 ? 3 : 2; }
+
+// Waves of the workgroups that take a head tile among few: what fits a CU without spilling, which
+// costs most where it is least work (28 bytes of scratch a lane: the first round 6 to 16 us).
+constexpr int mx4_most(int hd, int nt) { return hd == 64 && nt == 1 ? 12 : 8; }
 
 // A place in a workgroup's run: steps [begin, end) of one head tile, `it` of its rounds (a
 // step for each wave) done, and `left` steps of the run behind this tile's.
@@ -624,12 +649,8 @@ void mx4_attn_kernel(const Mx4Args a) {
     at.it = rounds - 1;
     if (!advance(at)) break;
     if (rounds & 1) {
-      const MxStage<HD> later = stage[0];
-      stage[0] = stage[1];
-      stage[1] = later;
-      const unsigned hole = holes[0];
-      holes[0] = holes[1];
-      holes[1] = hole;
+      stage[0].swap(stage[1]);
+      mx_swap(holes[0], holes[1]);
     }
     __syncthreads();  // before its parts are written over
     begin();
@@ -731,28 +752,25 @@ inline bool mx4_plan(int B, int T, int Hq, int Hkv, int hd, int width, int page,
   if (p->cap_len >= (1ll << 31) - kMxStep) return false;  // positions are 32-bit
   const long long units = static_cast<long long>(B) * Hkv * p->HT, cus = compute_units();
   // Whole head tiles by workgroups need one launch and no parts, but take as long as the longest
-  // of them.  By rounds of four waves that the table (or the window) can fill; us of four waves a
-  // tile / a CU's waves / runs, lengths even: 16 heads over 4 x 64, one sequence of 1000
-  // tokens 13 / 14 / 17, 2000 19 / 17 / 17, 4000 34 / 24 / 17; 64 of them 13 / 25 / 20, 21 /
-  // 29 / 23, 36 / 37 / 31; 32 heads over 8 x 128, 1 x 1000 16 / 14 / 17, 64 x 1000 22 / 33 /
-  // 31, 2000 35 / 46 / 42 (ragged 31 / 39 / 32), 4000 62 / 74 / 64 (ragged 54 / 58 / 44).
-  // Two column tiles a wave (8 tokens): 4 x 64, 16 x 1000 22 / 19 / 28, 2000 31 / 26 / 33, 4000
-  // 51 / 38 / 37; 8 x 128, 64 x 1000 31 / 40 / 46, 2000 50 / 58 / 64.
+  // of them; four waves share a CU with others, a CU's own serve few tiles.  By the rounds of
+  // four waves that the table (or the window) can fill; us of four waves a tile / of a CU's / of
+  // runs, lengths even: 16 heads over 4 x 64, one sequence of 1000 tokens 13 / 13 / 18, 2000 19
+  // / 16 / 19, 4000 34 / 23 / 18, 64 of 2000 21 / 17 / 22, 4000 36 / 26 / 30 (ragged 35 / 25 /
+  // 24); 32 heads over 8 x 128, 1 x 1000 16 / 13 / 16, 2000 25 / 19 / 16, 16 x 2000 26 / 19 / 22,
+  // 64 x 1000 22 / 27 / 30, 2000 36 / 41 / 42 (ragged 32 / 37 / 32), 4000 63 / 67 / 65 (ragged
+  // 55 / 60 / 44).  Two column tiles a wave (8 tokens): 4 x 64, 64 x 2000 29 / 22 / 33, 4000 51
+  // / 37 / 46; 8 x 128, 16 x 2000 35 / 28 / 32, 64 x 2000 51 / 58 / 67.
   const long long seen = window > 0 && window + T < p->cap_len ? window + T : p->cap_len;
   const long long rounds = (seen + 4 * kMxStep - 1) / (4 * kMxStep);
-  const int most = 4 * mx4_waves(hd, p->NT);
   bool whole;
-  if (units >= cus && (p->NT == 1 || hd == 128)) {
+  if (hd == 128 && units >= cus) {
     whole = rounds <= 16;
     p->W = 4;
-  } else if (p->NT == 1) {
-    whole = rounds <= 8;
-    p->W = hd == 64 || 2 * units > cus || rounds <= 4 ? 4 : most;
   } else {
-    whole = rounds <= 16;
-    p->W = most;
+    whole = rounds <= 8 || (rounds <= 16 && (hd == 64 || 4 * units >= cus)) ||
+            (rounds <= 32 && hd == 64 && units >= cus);
+    p->W = whole ? mx4_most(hd, p->NT) : 4;
   }
-  if (!whole) p->W = 4;
   p->runs = whole ? 0 : static_cast<int>(cus) * mx4_waves(hd, p->NT);
   p->groups = whole ? units : p->runs;
   p->ws = whole ? 0
@@ -766,7 +784,7 @@ inline bool mx4_plan(int B, int T, int Hq, int Hkv, int hd, int width, int page,
 
 template <int HD, int NT>
 int32_t launch_mx4(const Mx4Args& a, const Mx4Plan& p, hipStream_t s) {
-  constexpr int MOST = 4 * mx4_waves(HD, NT);
+  constexpr int MOST = mx4_most(HD, NT);
   const dim3 grid(static_cast<unsigned>(p.groups));
   if (p.W == 4)
     hipLaunchKernelGGL((mx4_attn_kernel<HD, NT, 4>), grid, dim3(256), 0, s, a);
