@@ -8,15 +8,14 @@
 //
 // The draw looks for a border among up to V of them, and sums in 32 bits move a border by
 // more than their distance at large V; so exponentials and sums are in 64 bits, which this
-// chip adds and multiplies at the rate of single 32-bit ones: 2^x of a reduced argument by
-// its Taylor sum.
+// chip adds and multiplies at the rate of single 32-bit ones.
 //
 // Bound by the read of the logits (then of one draft row a sequence).  Rows are cut into
 // chunks of 4096 ids, a workgroup each, so that one sequence's rows fill the chip too:
 //   1. each chunk's maximum and sum of exponentials under it;
-//   2. per (sequence, chunk): from those, which drafts are kept (few numbers, repeated by
-//      each chunk's workgroup), and the chunk's sum of the distribution to draw from;
-//   3. per sequence: the chunk in which the sum passes the threshold, and the id in it.
+//   2. per sequence: from those, which drafts are kept;
+//   3. per (sequence, chunk): its sum of the distribution to draw from;
+//   4. per sequence: the chunk in which the sum passes the threshold, and the id in it.
 // Greedy (T = 0): each row's first largest id, then the comparison: two launches.
 #include "common.hpp"
 #include "abi_util.hpp"
@@ -27,7 +26,7 @@ namespace llmy {
 constexpr int kVerThreads = 256, kVerPer = 16;
 constexpr int kVerChunk = kVerThreads * kVerPer;
 constexpr int kVerWaves = kVerThreads / kWave;
-constexpr int kMaxDrafts = 63;  // a wave looks at all rows of a sequence at once
+constexpr int kMaxDrafts = 63;  // rows of a sequence in LDS
 
 struct VerifyArgs {
   const float* logits;          // [B, K + 1, V]
@@ -36,35 +35,40 @@ struct VerifyArgs {
   const int32_t* counts;        // [B] or null: K
   const float* u;               // [B, K + 1]
   int32_t *tokens, *accepted;   // [B, K + 1], [B]
-  uint64_t* best;               // [B (K + 1), chunks]: largest (value, lowest id) of a chunk
-  double* sum;                  // [B (K + 1), chunks]: its sum under that maximum
+  uint64_t* best;               // [B (K + 1), parts]: largest (value, lowest id) of a part
+  double* sum;                  // [B (K + 1), parts]: its sum under that maximum
   double *rest, *plain;         // [B, chunks]: of max(e - q Z, 0) and e of the drawn row
-  double inv_t;
-  int B, K, V, chunks;
+  struct Decision* decided;     // [B]
+  double c;                     // log2(e) / T
+  int B, K, V;
+  int row_chunks, per_part, parts;  // chunks of a row, of a first workgroup, and those of a row
+  int chunks;                   // of a row that is drawn from
   bool vec4;
 };
 
-// e^x for x <= 0: 2^n sum_k r^k / k!, x = n ln 2 + r, |r| <= ln 2 / 2; the remainder
-// after k = 12 is under 2^-52 of it.  0 below -745, also for -inf.
-__device__ __forceinline__ double exp_neg(double x) {
-  x = fmax(x, -746.0);
-  const double n = rint(x * 1.4426950408889634);
-  double r = fma(n, -0.6931471805599453, x);  // ln 2 rounded to 64 bits, and what that left
-  r = fma(n, -2.3190468138462996e-17, r);
-  double s = 1.0 / 479001600.0;
-  s = fma(s, r, 1.0 / 39916800.0);
-  s = fma(s, r, 1.0 / 3628800.0);
-  s = fma(s, r, 1.0 / 362880.0);
-  s = fma(s, r, 1.0 / 40320.0);
-  s = fma(s, r, 1.0 / 5040.0);
-  s = fma(s, r, 1.0 / 720.0);
-  s = fma(s, r, 1.0 / 120.0);
-  s = fma(s, r, 1.0 / 24.0);
-  s = fma(s, r, 1.0 / 6.0);
-  s = fma(s, r, 0.5);
-  s = fma(s, r, 1.0);
-  s = fma(s, r, 1.0);
-  return ldexp(s, static_cast<int>(n));
+// 2^y for y up to about 0: 2^n 2^f, y = n + f, |f| <= 1/2, 2^f by the polynomial that meets it at
+// ten Chebyshev points: off by 2^-45 of it.  0 below 2^-1075, also for -inf.  Adding 1.5 x 2^52
+// rounds to a whole number and leaves it in the low word.
+__device__ __forceinline__ double exp2_neg(double y) {
+  y = fmax(y, -1100.0);
+  const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+  double s = 1.0212097549811005e-07;
+  s = fma(s, f, 1.3259945262689143e-06);
+  s = fma(s, f, 1.5252640059770786e-05);
+  s = fma(s, f, 0.00015403432339553542);
+  s = fma(s, f, 0.001333355825801874);
+  s = fma(s, f, 0.009618129195951041);
+  s = fma(s, f, 0.05550410866428854);
+  s = fma(s, f, 0.24022650695631514);
+  s = fma(s, f, 0.6931471805599526);
+  s = fma(s, f, 1.000000000000014);
+  return ldexp(s, static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t))));
+}
+
+// e^((x - top) / T) for x at most top, with shift = -top c: what that has been rounded by
+// is one factor for all weights under it.
+__device__ __forceinline__ double weight(float x, double c, double shift) {
+  return exp2_neg(fma(static_cast<double>(x), c, shift));
 }
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -79,60 +83,120 @@ __device__ __forceinline__ float key_value(uint64_t key) {
                           : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// This thread's 16 ids of a chunk of a row: the four from base + 1024 i + 4 t on, i < 4;
-// `none` past the row.
+// This thread's PER ids of a part of a row: the four from base + 1024 i + 4 t on, i < PER / 4;
+// `none` past the row.  (All loads of a part that lies in the row go out together; a test
+// around each would wait for the one before.)
+template <int PER>
 __device__ __forceinline__ void load_ids(const float* row, int V, int base, bool vec4, float none,
                                          float* v) {
+  const float* own = row + base + 4 * static_cast<int>(threadIdx.x);
+  if (vec4 && base + kVerThreads * PER <= V) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = base + 1024 * i + 4 * static_cast<int>(threadIdx.x);
-    if (vec4) {
-      float4 w = make_float4(none, none, none, none);
-      if (at < V) w = *reinterpret_cast<const float4*>(row + at);  // V % 4 == 0
+    for (int i = 0; i < PER / 4; ++i) {
+      const float4 w = *reinterpret_cast<const float4*>(own + 1024 * i);
       v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] = at + j < V ? row[at + j] : none;
     }
+    return;
+  }
+  // else every address lies in the row, and what is past it is put right afterwards
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = base + 1024 * (i >> 2) + 4 * static_cast<int>(threadIdx.x) + (i & 3);
+    v[i] = row[min(at, V - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = base + 1024 * (i >> 2) + 4 * static_cast<int>(threadIdx.x) + (i & 3);
+    v[i] = at < V ? v[i] : none;
   }
 }
 
+// The lowest id of this thread's largest value `most` among its ids of a chunk (NaN above all); none:
+// 2^31 - 1.  (A thread past the row's end has -inf, at ids behind it.)
+__device__ __forceinline__ uint64_t first_key(const float* v, float most, int base, int V) {
+  uint32_t at = 0x7fffffffu;
+#pragma unroll
+  for (int k = kVerPer - 1; k >= 0; --k) {
+    const bool same = v[k] == most || (v[k] != v[k] && most != most);
+    at = same ? base + 1024 * (k >> 2) + 4 * threadIdx.x + (k & 3) : at;
+  }
+  return at < static_cast<uint32_t>(V) ? value_index_key(most, at) : 0ull;
+}
+
+__device__ __forceinline__ float largest(const float* v) {
+  float most = v[0];
+#pragma unroll
+  for (int k = 1; k < kVerPer; ++k) most = __builtin_elementwise_maximum(most, v[k]);
+  return most;
+}
+
+// A part of a row: `per_part` chunks, the next one loaded under the present one's exponentials.
+// Each thread keeps a maximum and a sum under it; the workgroup's are formed once, at the end.
 template <bool GREEDY>
 __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(const VerifyArgs a) {
   __shared__ uint64_t keys[kVerWaves];
   __shared__ double sums[kVerWaves];
-  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
-  const int base = chunk * kVerChunk;
-  float v[kVerPer];
-  load_ids(a.logits + static_cast<long long>(row) * a.V, a.V, base, a.vec4, -INFINITY, v);
+  __shared__ float tops[kVerWaves];
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int c0 = part * a.per_part, c1 = min(a.row_chunks, c0 + a.per_part), wave = threadIdx.x >> 6;
+  const float* x = a.logits + static_cast<long long>(row) * a.V;
+  float v[kVerPer], next[kVerPer];
+  load_ids<kVerPer>(x, a.V, c0 * kVerChunk, a.vec4, -INFINITY, v);
+  float top = -INFINITY;
+  double s = 0;
   uint64_t key = 0;
+  for (int c = c0; c < c1; ++c) {
+    if (c + 1 < c1) load_ids<kVerPer>(x, a.V, (c + 1) * kVerChunk, a.vec4, -INFINITY, next);
+    const float most = largest(v);
+    if (GREEDY) {
+      key = umax64(key, first_key(v, most, c * kVerChunk, a.V));
+    } else {
+      const float old = top;
+      top = __builtin_elementwise_maximum(top, most);
+      // (under a row's first -inf alone the offset is the lowest number: weights 0)
+      const double shift = -static_cast<double>(fmaxf(top, -3.402823466e38f)) * a.c;
+      s *= weight(old, a.c, shift);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int id = base + 1024 * i + 4 * static_cast<int>(threadIdx.x) + j;
-      if (id < a.V) key = umax64(key, value_index_key(v[4 * i + j], id));
+      for (int k = 0; k < kVerPer; ++k) s += weight(v[k], a.c, shift);
     }
+#pragma unroll
+    for (int k = 0; k < kVerPer; ++k) v[k] = next[k];
+  }
+  if (!GREEDY) {
+    float all = top;
+    all = __builtin_elementwise_maximum(all, dpp_f<kDppXor1>(all));
+    all = __builtin_elementwise_maximum(all, dpp_f<kDppXor2>(all));
+    all = __builtin_elementwise_maximum(all, dpp_f<kDppHalfMirror>(all));
+    all = __builtin_elementwise_maximum(all, dpp_f<kDppMirror>(all));
+    all = __builtin_elementwise_maximum(
+        __builtin_elementwise_maximum(readlane_f(all, 0), readlane_f(all, 16)),
+        __builtin_elementwise_maximum(readlane_f(all, 32), readlane_f(all, 48)));
+    if ((threadIdx.x & 63) == 0) tops[wave] = all;
+    __syncthreads();
+    all = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[0], tops[1]),
+                                        __builtin_elementwise_maximum(tops[2], tops[3]));
+    if (fabsf(all) < INFINITY) {
+      s = wave_sum_d(s * weight(top, a.c, -static_cast<double>(all) * a.c));
+      if ((threadIdx.x & 63) == 0) sums[wave] = s;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        a.best[blockIdx.x] = value_index_key(all, 0u);
+        a.sum[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      }
+      return;
+    }
+    // no finite largest: its id is looked for after all
+    for (int c = c0; c < c1; ++c) {
+      load_ids<kVerPer>(x, a.V, c * kVerChunk, a.vec4, -INFINITY, v);
+      key = umax64(key, first_key(v, largest(v), c * kVerChunk, a.V));
+    }
+    if (threadIdx.x == 0) a.sum[blockIdx.x] = 0.;
+  }
   key = wave_max_u64(key);
-  const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) keys[wave] = key;
   __syncthreads();
-  key = umax64(umax64(keys[0], keys[1]), umax64(keys[2], keys[3]));
-  const float top = key_value(key);
-  double s = 0;
-  if (!GREEDY && fabsf(top) < INFINITY) {
-#pragma unroll
-    for (int k = 0; k < kVerPer; ++k)
-      s += exp_neg((static_cast<double>(v[k]) - static_cast<double>(top)) * a.inv_t);
-    s = wave_sum_d(s);
-    if ((threadIdx.x & 63) == 0) sums[wave] = s;
-    __syncthreads();
-    s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  }
-  if (threadIdx.x == 0) {
-    a.best[blockIdx.x] = key;
-    if (!GREEDY) a.sum[blockIdx.x] = s;
-  }
+  if (threadIdx.x == 0)
+    a.best[blockIdx.x] = umax64(umax64(keys[0], keys[1]), umax64(keys[2], keys[3]));
 }
 
 struct Row {
@@ -141,62 +205,57 @@ struct Row {
   bool sure;      // no finite largest: the id of the key alone
 };
 
-// A row from its chunks, by one wave.
-__device__ __forceinline__ Row whole_row(const VerifyArgs& a, long long row, bool greedy) {
-  const int lane = threadIdx.x & 63;
-  Row r;
-  r.key = 0;
-  for (int c = lane; c < a.chunks; c += kWave) r.key = umax64(r.key, a.best[row * a.chunks + c]);
-  r.key = wave_max_u64(r.key);
-  const float top = key_value(r.key);
-  r.sure = greedy || !(fabsf(top) < INFINITY);
-  r.z = 1.0;
-  if (!r.sure) {
-    double z = 0;
-    for (int c = lane; c < a.chunks; c += kWave) {
-      const float m = key_value(a.best[row * a.chunks + c]);
-      z += a.sum[row * a.chunks + c] *
-           exp_neg((static_cast<double>(m) - static_cast<double>(top)) * a.inv_t);
-    }
-    r.z = wave_sum_d(z);
-  }
-  return r;
-}
-
 struct Decision {
   Row row;        // the row that the new token comes from
   int kept;       // drafts kept before it
   bool rejected;  // a draft was put away there
 };
 
-// Which drafts of sequence b are kept: every row by a wave, their verdicts through LDS.
+// Which drafts of a sequence are kept: every row by 16 lanes, their verdicts through LDS.
 template <bool GREEDY>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, Row* rows, int* keep) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const VerifyArgs a) {
+  __shared__ Row rows[kMaxDrafts + 1];
+  __shared__ int keep[kMaxDrafts + 1];
+  const int b = blockIdx.x;
+  const int sub = threadIdx.x >> 4, lane = threadIdx.x & 15;
   const int count = a.counts ? min(max(a.counts[b], 0), a.K) : a.K;
-  for (int t = wave; t <= count; t += kVerWaves) {
+  for (int t0 = 0; t0 <= count; t0 += kVerThreads / 16) {
+    const int t = min(t0 + sub, count);  // (the last row again by what lanes are left)
     const long long row = static_cast<long long>(b) * (a.K + 1) + t;
-    const Row r = whole_row(a, row, GREEDY);
+    const long long draft = static_cast<long long>(b) * a.K + min(t, a.K - 1);
+    const int id = a.drafts[draft];
+    const bool named = t < count && id >= 0 && id < a.V;
+    float x = 0.f, q = 1.f, u = 0.f;
+    if (!GREEDY && named) {
+      x = a.logits[row * a.V + id];
+      if (a.probs) q = a.probs[draft * a.V + id];
+      u = a.u[row];
+    }
+    Row r;
+    r.key = 0;
+    for (int c = lane; c < a.parts; c += 16) r.key = umax64(r.key, a.best[row * a.parts + c]);
+    r.key = umax64(r.key, dpp_u64<kDppXor1>(r.key));
+    r.key = umax64(r.key, dpp_u64<kDppXor2>(r.key));
+    r.key = umax64(r.key, dpp_u64<kDppHalfMirror>(r.key));
+    r.key = umax64(r.key, dpp_u64<kDppMirror>(r.key));
+    const float top = key_value(r.key);
+    const double shift = -static_cast<double>(top) * a.c;
+    r.sure = GREEDY || !(fabsf(top) < INFINITY);
+    r.z = 1.0;
+    if (!GREEDY) {
+      double z = 0;
+      if (!r.sure)
+        for (int c = lane; c < a.parts; c += 16)
+          z += a.sum[row * a.parts + c] * weight(key_value(a.best[row * a.parts + c]), a.c, shift);
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) z += __shfl_xor(z, d, kWave);
+      if (!r.sure) r.z = z;
+    }
     if (lane == 0) {
       rows[t] = r;
-      bool ok = false;
-      if (t < count) {
-        const int id = a.drafts[static_cast<long long>(b) * a.K + t];
-        if (id >= 0 && id < a.V) {
-          if (GREEDY) {
-            ok = static_cast<uint32_t>(id) == key_index(r.key);
-          } else {
-            const float x = a.logits[row * a.V + id];
-            const double e = r.sure ? (static_cast<uint32_t>(id) == key_index(r.key) ? 1.0 : 0.0)
-                                    : exp_neg((static_cast<double>(x) -
-                                               static_cast<double>(key_value(r.key))) * a.inv_t);
-            const double q =
-                a.probs ? a.probs[(static_cast<long long>(b) * a.K + t) * a.V + id] : 1.0;
-            ok = static_cast<double>(a.u[row]) * q * r.z < e;
-          }
-        }
-      }
-      keep[t] = ok;
+      const bool best = static_cast<uint32_t>(id) == key_index(r.key);
+      const double e = r.sure ? (best ? 1.0 : 0.0) : weight(x, a.c, shift);
+      keep[t] = named && (GREEDY ? best : static_cast<double>(u) * q * r.z < e);
     }
   }
   __syncthreads();
@@ -205,62 +264,51 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, Row* rows
   while (d.kept < count && keep[d.kept]) ++d.kept;
   d.rejected = d.kept < count;
   d.row = rows[d.kept];
-  return d;
+  // the kept drafts, and (greedy) the row's id; a draw writes its own later
+  for (int t = threadIdx.x; t <= a.K; t += kVerThreads) {
+    const int64_t at = static_cast<int64_t>(b) * (a.K + 1) + t;
+    a.tokens[at] = t < d.kept ? a.drafts[static_cast<int64_t>(b) * a.K + t]
+                   : GREEDY && t == d.kept ? static_cast<int>(key_index(d.row.key)) : -1;
+  }
+  if (threadIdx.x == 0) {
+    a.accepted[b] = d.kept;
+    if (!GREEDY) a.decided[b] = d;
+  }
 }
 
-// Weights of the drawn row at this thread's 16 ids of a chunk: e and max(e - q Z, 0).
+// Weights of the drawn row at this thread's PER ids of a chunk, in order: put(k, e, max(e - q Z, 0)).
+template <int PER, class Put>
 __device__ __forceinline__ void draw_weights(const VerifyArgs& a, int b, const Decision& d, int base,
-                                             double* e, double* rest) {
+                                             Put put) {
   const long long row = static_cast<long long>(b) * (a.K + 1) + d.kept;
-  float x[kVerPer], q[kVerPer];
-  load_ids(a.logits + row * a.V, a.V, base, a.vec4, -INFINITY, x);
+  float x[PER], q[PER];
+  load_ids<PER>(a.logits + row * a.V, a.V, base, a.vec4, -INFINITY, x);
   const long long draft = static_cast<long long>(b) * a.K + d.kept;
 #pragma unroll
-  for (int k = 0; k < kVerPer; ++k) q[k] = 0.f;
-  if (d.rejected && a.probs) load_ids(a.probs + draft * a.V, a.V, base, a.vec4, 0.f, q);
+  for (int k = 0; k < PER; ++k) q[k] = 0.f;
+  if (d.rejected && a.probs) load_ids<PER>(a.probs + draft * a.V, a.V, base, a.vec4, 0.f, q);
   const int certain = d.rejected && !a.probs ? a.drafts[draft] : -1;
-  const double top = key_value(d.row.key);
+  const double shift = -static_cast<double>(key_value(d.row.key)) * a.c;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = 4 * i + j, id = base + 1024 * i + 4 * static_cast<int>(threadIdx.x) + j;
-      e[k] = d.row.sure ? (static_cast<uint32_t>(id) == key_index(d.row.key) ? 1.0 : 0.0)
-                        : exp_neg((static_cast<double>(x[k]) - top) * a.inv_t);
-      const double less = id == certain ? d.row.z : static_cast<double>(q[k]) * d.row.z;
-      rest[k] = e[k] > less ? e[k] - less : 0.0;  // (a NaN in q: 0)
-    }
-}
-
-__device__ __forceinline__ void put_tokens(const VerifyArgs& a, int b, int kept, int fresh) {
-  for (int t = threadIdx.x; t <= a.K; t += kVerThreads) {
-    const int id = t < kept ? a.drafts[static_cast<long long>(b) * a.K + t] : t == kept ? fresh : -1;
-    a.tokens[static_cast<long long>(b) * (a.K + 1) + t] = id;
+  for (int k = 0; k < PER; ++k) {
+    const int id = base + 1024 * (k >> 2) + 4 * static_cast<int>(threadIdx.x) + (k & 3);
+    const double e = d.row.sure ? (static_cast<uint32_t>(id) == key_index(d.row.key) ? 1.0 : 0.0)
+                                : weight(x[k], a.c, shift);
+    const double less = id == certain ? d.row.z : static_cast<double>(q[k]) * d.row.z;
+    put(k, e, e > less ? e - less : 0.0);  // (a NaN in q takes nothing off)
   }
-  if (threadIdx.x == 0) a.accepted[b] = kept;
 }
 
-__global__ __launch_bounds__(kVerThreads) void verify_greedy_kernel(const VerifyArgs a) {
-  __shared__ Row rows[kMaxDrafts + 1];
-  __shared__ int keep[kMaxDrafts + 1];
-  const Decision d = decide<true>(a, blockIdx.x, rows, keep);
-  put_tokens(a, blockIdx.x, d.kept, static_cast<int>(key_index(d.row.key)));
-}
-
+template <int PER>
 __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(const VerifyArgs a) {
-  __shared__ Row rows[kMaxDrafts + 1];
-  __shared__ int keep[kMaxDrafts + 1];
   __shared__ double sums[2][kVerWaves];
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const Decision d = decide<false>(a, b, rows, keep);
-  double e[kVerPer], rest[kVerPer];
-  draw_weights(a, b, d, chunk * kVerChunk, e, rest);
+  const Decision d = a.decided[b];
   double se = 0, sr = 0;
-#pragma unroll
-  for (int k = 0; k < kVerPer; ++k) {
-    se += e[k];
-    sr += rest[k];
-  }
+  draw_weights<PER>(a, b, d, chunk * (kVerThreads * PER), [&](int, double e, double rest) {
+    se += e;
+    sr += rest;
+  });
   se = wave_sum_d(se);
   sr = wave_sum_d(sr);
   if ((threadIdx.x & 63) == 0) {
@@ -274,67 +322,82 @@ __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(const VerifyAr
   }
 }
 
+template <int PER>
 __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ Row rows[kMaxDrafts + 1];
-  __shared__ int keep[kMaxDrafts + 1];
-  __shared__ double part[4][kVerWaves];
+  __shared__ double part[PER / 4][kVerWaves];
   __shared__ int first, last;
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Decision d = decide<false>(a, b, rows, keep);
-  // the whole, the chunk that passes the threshold, and the sum before it, by every wave alike
+  const Decision d = a.decided[b];
+  // The chunk in which the running sum passes the threshold, by every wave alike: sums of 64
+  // chunks at a time, each lane's in the chunks' order behind those before them.
   const double* sums = a.rest + static_cast<long long>(b) * a.chunks;
-  double all = 0;
-  for (int c = lane; c < a.chunks; c += kWave) all += sums[c];
-  all = wave_sum_d(all);
-  const bool spare = all > 0;  // else nothing is left beside the draft: from p itself
-  if (!spare) sums = a.plain + static_cast<long long>(b) * a.chunks;
-  // sums in the chunks' order: the total is the last running sum, as a threshold needs
-  double total = 0;
-  for (int c = 0; c < a.chunks; ++c) total += sums[c];
+  const auto upto = [&](int c0, double& mine) {  // inclusive, of the chunks from c0 to this lane's
+    mine = c0 + lane < a.chunks ? sums[c0 + lane] : 0.;
+    double s = mine;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const double x = __shfl_up(s, o, kWave);
+      if (lane >= o) s += x;
+    }
+    return s;
+  };
+  const auto whole = [&]() {
+    double all = 0, mine;
+    for (int c0 = 0; c0 < a.chunks; c0 += kWave) all += __shfl(upto(c0, mine), kWave - 1, kWave);
+    return all;
+  };
+  double total = whole();
+  const bool spare = total > 0;  // else nothing is left beside the draft: from p itself
+  if (!spare) {
+    sums = a.plain + static_cast<long long>(b) * a.chunks;
+    total = whole();
+  }
   const double goal = static_cast<double>(a.u[static_cast<long long>(b) * (a.K + 1) + a.K]) * total;
   int chunk = 0;
   double before = 0, run = 0;
-  bool passed = false;
-  for (int c = 0; c < a.chunks; ++c) {
-    const double s = sums[c];
-    if (s > 0 && !passed) {
-      chunk = c;
-      before = run;
-      passed = run + s > goal;
+  for (int c0 = 0; c0 < a.chunks; c0 += kWave) {
+    double mine;
+    const double s = upto(c0, mine);
+    const uint64_t any = __ballot(mine > 0), past = __ballot(mine > 0 && run + s > goal);
+    // the first chunk past the threshold; none (yet): the last that has any weight
+    const int l = past ? __ffsll(static_cast<unsigned long long>(past)) - 1
+                       : 63 - __clzll(static_cast<long long>(any));
+    if (past | any) {
+      chunk = c0 + l;
+      before = run + __shfl(s, l, kWave) - __shfl(mine, l, kWave);
     }
-    run += s;
+    if (past) break;
+    run += __shfl(s, kWave - 1, kWave);
   }
   if (threadIdx.x == 0) first = a.V, last = -1;
-  double e[kVerPer], rest[kVerPer];
-  const int base = chunk * kVerChunk;
-  draw_weights(a, b, d, base, e, rest);
+  double rest[PER];
+  const int base = chunk * (kVerThreads * PER);
+  draw_weights<PER>(a, b, d, base, [&](int k, double e, double r) { rest[k] = spare ? r : e; });
+  // running sums in the ids' order: blocks of 1024 ids, 4 a thread
+  double part_upto[PER / 4];
 #pragma unroll
-  for (int k = 0; k < kVerPer; ++k)
-    if (!spare) rest[k] = e[k];
-  // running sums in the ids' order: four blocks of 1024 ids, 4 a thread
-  double upto[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < PER / 4; ++i) {
     double s = (rest[4 * i] + rest[4 * i + 1]) + (rest[4 * i + 2] + rest[4 * i + 3]);
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
       const double x = __shfl_up(s, o, kWave);
       if (lane >= o) s += x;
     }
-    upto[i] = s;
+    part_upto[i] = s;
     if (lane == kWave - 1) part[i][wave] = s;
   }
   __syncthreads();
   double start = before;
+  int at_first = a.V, at_last = -1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < PER / 4; ++i) {
     double c = start;
 #pragma unroll
     for (int w = 0; w < kVerWaves; ++w) {
       if (w < wave) c += part[i][w];
       start += part[i][w];
     }
-    const double prev = __shfl_up(upto[i], 1, kWave);
+    const double prev = __shfl_up(part_upto[i], 1, kWave);
     if (lane) c += prev;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -342,17 +405,40 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyAr
       c += w;
       const int id = base + 1024 * i + 4 * static_cast<int>(threadIdx.x) + j;
       if (w > 0) {
-        if (c > goal) atomicMin(&first, id);
-        atomicMax(&last, id);
+        if (c > goal) at_first = min(at_first, id);
+        at_last = max(at_last, id);
       }
     }
   }
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    at_first = min(at_first, __shfl_xor(at_first, o, kWave));
+    at_last = max(at_last, __shfl_xor(at_last, o, kWave));
+  }
+  if (lane == 0) {
+    atomicMin(&first, at_first);
+    atomicMax(&last, at_last);
+  }
   __syncthreads();
   // u at 1, or sums that rounded below the threshold: the last id with any weight
-  put_tokens(a, b, d.kept, first < a.V ? first : last);
+  if (threadIdx.x == 0)
+    a.tokens[static_cast<long long>(b) * (a.K + 1) + d.kept] = first < a.V ? first : last;
 }
 
-inline int verify_chunks(int V) { return (V + kVerChunk - 1) / kVerChunk; }
+inline int verify_chunks(int V, int chunk) { return (V + chunk - 1) / chunk; }
+
+// Ids a thread of a draw: 16, or 4 where that many leave most of the chip idle and the exponentials
+// a thread forms one after the other are what takes long (1 x 32000: the two kernels 14 -> 8 us).
+inline int verify_draw_per(int B, int V) {
+  return static_cast<int64_t>(B) * verify_chunks(V, kVerChunk) < compute_units() ? 4 : 16;
+}
+
+// Chunks of a row that one workgroup of the first kernel takes: as many as leave five a CU, which
+// are resident together (64 x 5 rows of 32 chunks: one each 46 us, eight each 39).
+inline int verify_per_part(int64_t rows, int chunks) {
+  const int64_t n = rows * chunks / (5ll * compute_units());
+  return static_cast<int>(n < 1 ? 1 : n > chunks ? chunks : n);
+}
 
 }  // namespace llmy
 
@@ -360,9 +446,11 @@ using namespace llmy;
 
 extern "C" int64_t llmy_verify_drafts_workspace_bytes(int32_t B, int32_t K, int32_t V) {
   if (B < 0 || K < 1 || K > kMaxDrafts || V < 1 || V > (1 << 30)) return -1;
-  const int64_t chunks = verify_chunks(V), rows = static_cast<int64_t>(B) * (K + 1);
-  if (rows * chunks >= (1ll << 31)) return -1;  // the grid
-  return 16 * chunks * (rows + B);
+  const int64_t rows = static_cast<int64_t>(B) * (K + 1);
+  const int64_t parts = rows * verify_chunks(V, kVerChunk);
+  if (parts >= (1ll << 31)) return -1;  // the grid
+  const int64_t draws = static_cast<int64_t>(B) * verify_chunks(V, kVerThreads * verify_draw_per(B, V));
+  return 16 * (parts + draws) + static_cast<int64_t>(sizeof(Decision)) * B;
 }
 
 extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* draft_tokens,
@@ -388,23 +476,34 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
   VerifyArgs a{};
   a.logits = logits; a.drafts = draft_tokens; a.probs = draft_probs; a.counts = counts; a.u = u;
   a.tokens = tokens; a.accepted = accepted;
-  a.B = B; a.K = K; a.V = V; a.chunks = verify_chunks(V);
-  a.inv_t = greedy ? 0. : fmin(1. / temperature, 0x1p1023);
+  const int per = verify_draw_per(B, V);
+  a.B = B; a.K = K; a.V = V;
+  a.row_chunks = verify_chunks(V, kVerChunk);
+  a.chunks = verify_chunks(V, kVerThreads * per);
+  a.c = greedy ? 0. : fmin(1.4426950408889634 / temperature, 0x1p1023);
   a.vec4 = V % 4 == 0 && aligned(logits, 16) && (!draft_probs || aligned(draft_probs, 16));
-  const int64_t parts = rows * a.chunks;
+  a.per_part = verify_per_part(rows, a.row_chunks);
+  a.parts = (a.row_chunks + a.per_part - 1) / a.per_part;
   a.best = static_cast<uint64_t*>(workspace);
-  a.sum = reinterpret_cast<double*>(a.best + parts);
-  a.rest = a.sum + parts;
+  a.sum = reinterpret_cast<double*>(a.best + rows * a.parts);
+  a.rest = a.sum + rows * a.parts;
   a.plain = a.rest + static_cast<int64_t>(B) * a.chunks;
+  a.decided = reinterpret_cast<Decision*>(a.plain + static_cast<int64_t>(B) * a.chunks);
   const hipStream_t s = as_stream(stream);
-  const dim3 grid(static_cast<unsigned>(parts)), draws(static_cast<unsigned>(B) * a.chunks);
+  const dim3 grid(static_cast<unsigned>(rows * a.parts)), draws(static_cast<unsigned>(B) * a.chunks);
   if (greedy) {
     hipLaunchKernelGGL(verify_rows_kernel<true>, grid, dim3(kVerThreads), 0, s, a);
-    hipLaunchKernelGGL(verify_greedy_kernel, dim3(B), dim3(kVerThreads), 0, s, a);
+    hipLaunchKernelGGL(verify_decide_kernel<true>, dim3(B), dim3(kVerThreads), 0, s, a);
     return launch_status();
   }
   hipLaunchKernelGGL(verify_rows_kernel<false>, grid, dim3(kVerThreads), 0, s, a);
-  hipLaunchKernelGGL(verify_sums_kernel, draws, dim3(kVerThreads), 0, s, a);
-  hipLaunchKernelGGL(verify_draw_kernel, dim3(B), dim3(kVerThreads), 0, s, a);
+  hipLaunchKernelGGL(verify_decide_kernel<false>, dim3(B), dim3(kVerThreads), 0, s, a);
+  if (per == 4) {
+    hipLaunchKernelGGL(verify_sums_kernel<4>, draws, dim3(kVerThreads), 0, s, a);
+    hipLaunchKernelGGL(verify_draw_kernel<4>, dim3(B), dim3(kVerThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(verify_sums_kernel<16>, draws, dim3(kVerThreads), 0, s, a);
+    hipLaunchKernelGGL(verify_draw_kernel<16>, dim3(B), dim3(kVerThreads), 0, s, a);
+  }
   return launch_status();
 }

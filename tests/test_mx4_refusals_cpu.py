@@ -143,7 +143,7 @@ def test_verify_refuses(lib, over):
 
 def test_verify_of_nothing_and_its_workspace(lib):
     assert verify(lib, B=0) == 0
-    assert lib.llmy_verify_drafts_workspace_bytes(2, 3, 1000) == 16 * (2 * 4 + 2)
+    assert lib.llmy_verify_drafts_workspace_bytes(2, 3, 1000) == 16 * (2 * 4 + 2) + 2 * 32
     assert lib.llmy_verify_drafts_workspace_bytes(2, 64, 1000) == -1
 
 
