@@ -23,6 +23,11 @@
 // cover the block's largest magnitude, and each value over it as a 4-bit float, to nearest
 // even.  7 and not 6, the largest code: what lies between is off by no more than half of
 // the code's last step, like the values under 6, and the finer scale serves the other 31.
+// A key next to a border between two codes is a whole step off if its rounding crosses it: of
+// 262144 normed and rotated keys in fp32 one did in a few calls, so 4-bit keys are formed in
+// 64 bits (3.6 -> 4.4 us for one token, 5.1 -> 6.4 for 256 of 8 x 128, 7.0 -> 11.6 for 8191 of
+// 2 x 128) and come to fp32 by rounding to odd, after which a second rounding to fewer bits is
+// as good as the only one.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "paged.hpp"
@@ -86,6 +91,15 @@ __device__ __forceinline__ float mean_square(const float* y) {
   return ss * (1.f / HD);
 }
 
+// To fp32: what is not exact to the neighbour with an odd last bit.
+__device__ __forceinline__ float to_odd(double d) {
+  const float f = static_cast<float>(d);
+  const double back = f;
+  const uint32_t u = __float_as_uint(f);
+  if (back == d || (u & 1u)) return f;
+  return __uint_as_float(fabs(back) > fabs(d) ? u - 1u : u + 1u);  // (NaN stays one)
+}
+
 // Below this mean square the squares may have lost bits to fp32's end; such rows, all under
 // 2^-41, are raised so that bf16's smallest squares to a normal number.  Rows whose
 // squares overflowed reach past 2^60 and are lowered; what that takes below the
@@ -124,6 +138,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
   constexpr int RPI = 64 / LPR; // rows an iteration
   __shared__ __align__(16) float trig[4][2][64];
   __shared__ __align__(16) float turn[M4 ? 4 : 1][M4 ? 512 : 4];
+  __shared__ __align__(16) double trig64[M4 ? 4 : 1][2][M4 ? 64 : 2];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const uint32_t task = blockIdx.x * 4u + wave;
@@ -174,6 +189,12 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
     sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &co);
     trig[wave][0][lane] = co;
     trig[wave][1][lane] = s;
+    if (M4 && first < a.hq + a.hkv && first + IT * RPI > a.hq) {  // this wave has keys
+      double s64, c64;
+      sincospi(2. * (turns - rint(turns)), &s64, &c64);
+      trig64[M4 ? wave : 0][0][M4 ? lane : 0] = c64;
+      trig64[M4 ? wave : 0][1][M4 ? lane : 0] = s64;
+    }
   }
   wave_lds_order();
   if (turned) {
@@ -225,6 +246,52 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const RopeArgs a) {
           y[j + 4] = v * cs[j] + u * sn[j];
         }
       }
+    }
+    if (M4 && (a.w[1] || a.half > 0) && __ballot(kind == 1)) {  // keys again, in 64 bits
+      float x[8];
+      unpack4(x0[i], x);
+      unpack4(x1[i], x + 4);
+      double z[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = x[j];
+      if (a.w[1]) {
+        double ss = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fma(z[j], z[j], ss);
+        ss += __builtin_bit_cast(double, dpp_u64<kDppXor1>(__builtin_bit_cast(uint64_t, ss)));
+        ss += __builtin_bit_cast(double, dpp_u64<kDppXor2>(__builtin_bit_cast(uint64_t, ss)));
+        ss += __builtin_bit_cast(double, dpp_u64<kDppHalfMirror>(__builtin_bit_cast(uint64_t, ss)));
+        if (HD == 128)
+          ss += __builtin_bit_cast(double, dpp_u64<kDppMirror>(__builtin_bit_cast(uint64_t, ss)));
+        const double rs = 1. / sqrt(ss * (1. / HD) + static_cast<double>(a.eps));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          z[j] *= rs * static_cast<double>(a.w[1][d0 + j]);
+          z[j + 4] *= rs * static_cast<double>(a.w[1][d1 + j]);
+        }
+      }
+      if (turned) {
+        const double* c64 = trig64[M4 ? wave : 0][0] + (M4 ? 4 * c : 0);
+        const double* s64 = trig64[M4 ? wave : 0][1] + (M4 ? 4 * c : 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double u = z[j], v = z[j + 4];
+          if (!a.interleaved) {
+            z[j] = u * c64[j] - v * s64[j];
+            z[j + 4] = v * c64[j] + u * s64[j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double u = z[2 * j], v = z[2 * j + 1];
+          if (a.interleaved) {
+            z[2 * j] = u * c64[j] - v * s64[j];
+            z[2 * j + 1] = v * c64[j] + u * s64[j];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = kind == 1 ? to_odd(z[j]) : y[j];
     }
     if (M4) {
       // blocks are of neighbouring dims: each row's values in order through LDS

@@ -530,16 +530,15 @@ def _mx4(k_cache, v_cache, k_scales, v_scales, Hkv: int, hd: int, dev: int) -> t
     """(pages, page) and the addresses of a 4-bit cache's codes [pages, Hkv, page, hd / 2] and
     scales [pages, Hkv, page, hd / 32]."""
     shape = k_cache.shape
-    if len(shape) == 4:
-        scales = (shape[0], Hkv, shape[2], hd // 32)
-        if (k_cache.dtype is _FP4 and v_cache.dtype is _FP4 and k_scales.dtype is _E8M0
-                and v_scales.dtype is _E8M0 and shape[1] == Hkv and shape[3] == hd // 2
-                and v_cache.shape == shape and k_scales.shape == scales
-                and v_scales.shape == scales
-                and all(t.is_contiguous() and t.get_device() == dev
-                        for t in (k_cache, v_cache, k_scales, v_scales))):
-            return (shape[0], shape[2], k_cache.data_ptr(), v_cache.data_ptr(),
-                    k_scales.data_ptr(), v_scales.data_ptr())
+    if (len(shape) == 4 and shape[1] == Hkv and shape[3] * 2 == hd and k_cache.dtype is _FP4
+            and v_cache.dtype is _FP4 and k_scales.dtype is _E8M0 and v_scales.dtype is _E8M0
+            and v_cache.shape == shape and k_scales.shape == (shape[0], Hkv, shape[2], hd // 32)
+            and v_scales.shape == k_scales.shape and k_cache.is_contiguous()
+            and v_cache.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
+            and k_cache.get_device() == dev and v_cache.get_device() == dev
+            and k_scales.get_device() == dev and v_scales.get_device() == dev):
+        return (shape[0], shape[2], k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
+                v_scales.data_ptr())
     raise ValueError(
         f"a 4-bit cache is contiguous codes [pages, {Hkv}, page, {hd // 2}] of {_FP4} and scales "
         f"[pages, {Hkv}, page, {hd // 32}] of {_E8M0} on cuda:{dev}, the current device; got "
@@ -629,7 +628,8 @@ def paged_kv_read_mx4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: to
     if rows is None and N > B:
         raise ValueError(f"{N} tokens and {B} page-table rows: name each token's row")
     pp, pr = _vec(positions, "positions", _I32, N, dev), _vec(rows, "rows", _I32, N, dev)
-    k, v = (torch.empty(N, Hkv, hd, dtype=_BF16, device=k_cache.device) for _ in range(2))
+    k = k_cache.new_empty((N, Hkv, hd), dtype=_BF16)
+    v = torch.empty_like(k)
     _lib.call("llmy_paged_kv_read_mx4", *cache, pt, pr, pp, k.data_ptr(), v.data_ptr(), N, Hkv,
               hd, B, width, page, pages, _stream())
     return k, v
@@ -689,8 +689,9 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, page_table: torc
     p1 = _vec(n_free, "n_free", _I32, 1, dev)
     if tokens < 0:
         raise ValueError(f"tokens must not be negative, got {tokens}")
-    cu = lengths.new_empty(B + 1)
-    rows, positions, out = lengths.new_empty(tokens), lengths.new_empty(tokens), lengths.new_empty(B)
+    # one allocation: rows and positions first, on its 16-byte boundary where tokens % 4 == 0
+    rows, positions, cu, out = lengths.new_empty(2 * tokens + 2 * B + 1).split(
+        (tokens, tokens, B + 1, B))
     nbytes = _lib.load().llmy_paged_plan_workspace_bytes(B, tokens)
     workspace, pw, have = _workspace(workspace, nbytes, lengths, dev)
     _lib.call("llmy_paged_plan", pl, pn, pr, pt, ph, pf, p1, cu.data_ptr(), rows.data_ptr(),
