@@ -65,10 +65,10 @@ __device__ __forceinline__ double exp2_neg(double y) {
   return ldexp(s, static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t))));
 }
 
-// e^((x - top) / T) for x at most top, with shift = -top c: what that has been rounded by
-// is one factor for all weights under it.
-__device__ __forceinline__ double weight(float x, double c, double shift) {
-  return exp2_neg(fma(static_cast<double>(x), c, shift));
+// e^((x - top) / T) for x at most top.  The difference first: where top c passes 2^53 (a
+// temperature near 0), a product's rounding would pass whole powers of two.
+__device__ __forceinline__ double weight(float x, double c, double top) {
+  return exp2_neg((static_cast<double>(x) - top) * c);
 }
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -154,10 +154,10 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(const VerifyAr
       const float old = top;
       top = __builtin_elementwise_maximum(top, most);
       // (under a row's first -inf alone the offset is the lowest number: weights 0)
-      const double shift = -static_cast<double>(fmaxf(top, -3.402823466e38f)) * a.c;
-      s *= weight(old, a.c, shift);
+      const double under = fmaxf(top, -3.402823466e38f);
+      s *= weight(old, a.c, under);
 #pragma unroll
-      for (int k = 0; k < kVerPer; ++k) s += weight(v[k], a.c, shift);
+      for (int k = 0; k < kVerPer; ++k) s += weight(v[k], a.c, under);
     }
 #pragma unroll
     for (int k = 0; k < kVerPer; ++k) v[k] = next[k];
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(const VerifyAr
     all = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[0], tops[1]),
                                         __builtin_elementwise_maximum(tops[2], tops[3]));
     if (fabsf(all) < INFINITY) {
-      s = wave_sum_d(s * weight(top, a.c, -static_cast<double>(all) * a.c));
+      s = wave_sum_d(s * weight(top, a.c, all));
       if ((threadIdx.x & 63) == 0) sums[wave] = s;
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -239,14 +239,13 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const Verify
     r.key = umax64(r.key, dpp_u64<kDppHalfMirror>(r.key));
     r.key = umax64(r.key, dpp_u64<kDppMirror>(r.key));
     const float top = key_value(r.key);
-    const double shift = -static_cast<double>(top) * a.c;
     r.sure = GREEDY || !(fabsf(top) < INFINITY);
     r.z = 1.0;
     if (!GREEDY) {
       double z = 0;
       if (!r.sure)
         for (int c = lane; c < a.parts; c += 16)
-          z += a.sum[row * a.parts + c] * weight(key_value(a.best[row * a.parts + c]), a.c, shift);
+          z += a.sum[row * a.parts + c] * weight(key_value(a.best[row * a.parts + c]), a.c, top);
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) z += __shfl_xor(z, d, kWave);
       if (!r.sure) r.z = z;
@@ -254,7 +253,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const Verify
     if (lane == 0) {
       rows[t] = r;
       const bool best = static_cast<uint32_t>(id) == key_index(r.key);
-      const double e = r.sure ? (best ? 1.0 : 0.0) : weight(x, a.c, shift);
+      const double e = r.sure ? (best ? 1.0 : 0.0) : weight(x, a.c, top);
       keep[t] = named && (GREEDY ? best : static_cast<double>(u) * q * r.z < e);
     }
   }
@@ -288,12 +287,12 @@ __device__ __forceinline__ void draw_weights(const VerifyArgs& a, int b, const D
   for (int k = 0; k < PER; ++k) q[k] = 0.f;
   if (d.rejected && a.probs) load_ids<PER>(a.probs + draft * a.V, a.V, base, a.vec4, 0.f, q);
   const int certain = d.rejected && !a.probs ? a.drafts[draft] : -1;
-  const double shift = -static_cast<double>(key_value(d.row.key)) * a.c;
+  const double top = key_value(d.row.key);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int id = base + 1024 * (k >> 2) + 4 * static_cast<int>(threadIdx.x) + (k & 3);
     const double e = d.row.sure ? (static_cast<uint32_t>(id) == key_index(d.row.key) ? 1.0 : 0.0)
-                                : weight(x[k], a.c, shift);
+                                : weight(x[k], a.c, top);
     const double less = id == certain ? d.row.z : static_cast<double>(q[k]) * d.row.z;
     put(k, e, e > less ? e - less : 0.0);  // (a NaN in q takes nothing off)
   }
@@ -480,7 +479,8 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
   a.B = B; a.K = K; a.V = V;
   a.row_chunks = verify_chunks(V, kVerChunk);
   a.chunks = verify_chunks(V, kVerThreads * per);
-  a.c = greedy ? 0. : fmin(1.4426950408889634 / temperature, 0x1p1023);
+  // (2^800 already takes the least difference of two logits, 2^-149, past every weight)
+  a.c = greedy ? 0. : fmin(1.4426950408889634 / temperature, 0x1p800);
   a.vec4 = V % 4 == 0 && aligned(logits, 16) && (!draft_probs || aligned(draft_probs, 16));
   a.per_part = verify_per_part(rows, a.row_chunks);
   a.parts = (a.row_chunks + a.per_part - 1) / a.per_part;

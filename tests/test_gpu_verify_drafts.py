@@ -167,3 +167,65 @@ def test_captured_and_replayed():
         want, kept, margin = ref.verify(*c)
         assert float(margin.min()) > NEAR
         assert torch.equal(out[0].cpu(), want) and torch.equal(out[1].cpu(), kept)
+
+
+@pytest.mark.parametrize("B,K,V,seed,kw", [
+    # several chunks a workgroup of the first kernel, the last of them short; 16 ids a thread
+    (72, 7, 36000, 20, {}), (65, 5, 57345, 21, {"probs": False}),
+    (90, 5, 45055, 22, {"temperature": 0.0, "probs": False}),
+])
+def test_many_rows(B, K, V, seed, kw):
+    _same(_case(B, K, V, seed, **kw))
+
+
+def test_many_rows_without_a_finite_largest_logit():
+    """Rows of several chunks a workgroup: -inf at first, throughout, infinities and NaN late."""
+    B, K, V = 66, 7, 33000
+    case = list(_case(B, K, V, 30, probs=False, counts=False))
+    x = case[0]
+    x[0::5, :, :20000] = -math.inf
+    x[1::5, 2] = -math.inf
+    x[2::5, 1, [20, 32999]] = math.inf
+    x[3::5, 0, 29000] = math.nan
+    x[3::5, 0, 100] = math.inf
+    case[1] = x[:, :K].nan_to_num(nan=9e9, posinf=8e9, neginf=-9e9).argmax(-1).int()  # often kept
+    case[2] = case[2] * 0.5
+    tokens, accepted = _same(tuple(case))
+    assert 0 < int(accepted.float().mean() * 10) and int(accepted.min()) < K
+    case[3] = 0.0
+    _same(tuple(case))
+
+
+@pytest.mark.parametrize("temperature", [1e-9, 1e-16, 1e-20, 1e-30, 1e-300, 5e-324])
+@pytest.mark.parametrize("scale", [1.0, 1e30])
+def test_temperatures_near_zero(temperature, scale):
+    """Only a row's largest logits have any weight, however far their quotients reach."""
+    B, K, V = 5, 3, 9001
+    logits, ids, u, _, q, n = _case(B, K, V, 3, counts=False)
+    logits *= scale
+    logits[1, :, [7, 8888]] = 50.0 * scale  # two that are largest
+    ids[1] = 7
+    ids[2] = logits[2, :K].argmax(-1).int()
+    u[1, :K], u[1, K] = 0.25, 0.75
+    _, accepted = _same((logits, ids, u, temperature, None, None))
+    assert accepted[1] == K and accepted[2] == K
+    _same((logits, ids, u, temperature, q, None))
+
+
+def test_on_another_stream_and_two_at_once():
+    ops = _ops()
+    cases = [_case(20, 4, 30000, 40), _case(70, 3, 9000, 41)]
+    dev = [[None if t is None or isinstance(t, float) else t.cuda() for t in c] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for d, c, s in zip(dev, cases, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.verify_drafts(d[0], d[1], d[2], temperature=c[3], draft_probs=d[4],
+                                             counts=d[5]))
+        torch.cuda.synchronize()
+        for g, c in zip(got, cases):
+            want, kept, margin = ref.verify(*c)
+            assert float(margin.min()) > NEAR
+            assert torch.equal(g[0].cpu(), want) and torch.equal(g[1].cpu(), kept)
