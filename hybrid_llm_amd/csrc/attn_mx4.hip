@@ -388,7 +388,7 @@ void mx4_attn_kernel(const Mx4Args a) {
       const int c = min(16 * (NT * at.ht + n) + col, TG - 1), t = a.T == 1 ? 0 : c / a.G;
       const int h = at.kvh * a.G + c - t * a.G;
       end[n] = at.len - (a.T - 1 - t);
-      lo[n] = a.window > 0 ? max(0, end[n] - a.window) : 0;
+      lo[n] = a.window > 0 ? max(0, max(0, end[n]) - a.window) : 0;
       const uint16_t* qp = a.q + at.b * a.qb + t * a.qt + h * a.qh + g * (HD / 4);
 #pragma unroll
       for (int x = 0; x < NS; ++x) qf[n][x] = *reinterpret_cast<const uint4*>(qp + 8 * x);
@@ -760,7 +760,8 @@ inline bool mx4_plan(int B, int T, int Hq, int Hkv, int hd, int width, int page,
   // 64 x 1000 22 / 27 / 30, 2000 36 / 41 / 42 (ragged 32 / 37 / 32), 4000 63 / 67 / 65 (ragged
   // 55 / 60 / 44).  Two column tiles a wave (8 tokens): 4 x 64, 64 x 2000 29 / 22 / 33, 4000 51
   // / 37 / 46; 8 x 128, 16 x 2000 35 / 28 / 32, 64 x 2000 51 / 58 / 67.
-  const long long seen = window > 0 && window + T < p->cap_len ? window + T : p->cap_len;
+  const long long span = static_cast<long long>(window) + T;
+  const long long seen = window > 0 && span < p->cap_len ? span : p->cap_len;
   const long long rounds = (seen + 4 * kMxStep - 1) / (4 * kMxStep);
   bool whole;
   if (hd == 128 && units >= cus) {

@@ -399,3 +399,112 @@ def test_repeats_are_equal_to_the_bit():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert torch.equal(want, first)
+
+
+# -------------------------------------------- every form, long caches, other streams
+@pytest.mark.parametrize("B,T,Hq,Hkv,hd,page,longest,window", [
+    (40, 1, 8, 8, 128, 16, 90, 0),        # more head tiles than CUs, short tables: four waves each
+    (36, 3, 16, 8, 128, 32, 700, 50),
+    (70, 1, 8, 4, 64, 16, 500, 0),
+    (70, 5, 16, 4, 64, 64, 500, 0),       # two column tiles
+    (64, 2, 4, 4, 64, 32, 4000, 0),       # long ones: a CU's waves each
+    (34, 1, 8, 8, 128, 64, 5000, 0),      # as many tiles, long tables: runs
+    (3, 64, 4, 1, 64, 16, 4500, 0),       # 256 columns in runs
+    (2, 33, 6, 2, 128, 128, 6000, 2 ** 31 - 1),
+    (300, 2, 2, 1, 64, 16, 2500, 90),     # a window that only some of them pass
+])
+def test_attention_of_many(B, T, Hq, Hkv, hd, page, longest, window):
+    """Lengths from nothing to the longest, some below T: their first tokens see nothing."""
+    g = torch.Generator().manual_seed(B + T + longest)
+    width = -(-longest // page)
+    pages = min(B * width, 600)
+    table = torch.randint(0, pages, (B, width), generator=g).int()  # pages may be shared
+    dev, k, v = _cache(pages, Hkv, page, hd, g)
+    q = torch.randn(B, T, Hq, hd, generator=g).to(BF16)
+    lengths = torch.randint(0, longest + 1, (B,), generator=g).int()
+    lengths[:2] = torch.tensor([longest, T // 2])
+    got = _ops().paged_attn_mx4(q.cuda(), *dev, table.cuda(), lengths.cuda(), window=window).cpu()
+    some = [0, 1, B // 2, B - 1] if B > 4 else list(range(B))
+    want, spread = ref.attend(q[some], k, v, table[some], lengths[some], window=window)
+    _attn_ok(got[some], want, spread)
+    if T > 1:
+        assert not got[1, :T - T // 2].any()  # tokens before the text
+    # and each alone: another split of the work, the same within both calls' errors
+    for b in (B // 2, B - 2):
+        one = _ops().paged_attn_mx4(q[b:b + 1].cuda(), *dev, table[b:b + 1].cuda().contiguous(),
+                                    lengths[b:b + 1].cuda(), window=window).cpu()
+        both = 2.0 ** -7 * got[b].double().abs() + 2 * (2.0 ** -16 + 2.0 ** -10) * 12 + 1e-30
+        assert bool(((one[0].double() - got[b].double()).abs() <= both).all())
+
+
+def test_nothing_to_see_over_long_tables():
+    ops = _ops()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 2, 4, 64, device="cuda").to(BF16)
+    dev, _, _ = _cache(2, 2, 16, 64, torch.Generator().manual_seed(0))
+    lengths = torch.tensor([0, -4, 9000], **i32)
+    empty = torch.zeros(3, 900, **i32)
+    assert not ops.paged_attn_mx4(q, *ops.mx4_cache(0, 2, 16, 64), empty, lengths).any()
+    assert not ops.paged_attn_mx4(q, *dev, empty - 1, lengths).any()
+    assert not ops.paged_attn_mx4(q, *dev, empty, lengths * 0).any()
+
+
+@pytest.mark.parametrize("hd,width", [(128, 3), (128, 200), (64, 200)])
+def test_a_cache_past_32_bit_offsets(hd, width):
+    """Codes of k and of v past 4 GiB each: pages at both ends and around 2^31 and 2^32."""
+    ops, g = _ops(), torch.Generator().manual_seed(width)
+    Hkv, page, Hq, T = 8, 256, 8, 2
+    per = Hkv * page * hd // 2
+    pages = 2 ** 32 // per + 40
+    cache = tuple(torch.empty(s, dtype=torch.uint8, device="cuda").view(t) for s, t in (
+        ((pages, Hkv, page, hd // 2), FP4), ((pages, Hkv, page, hd // 2), FP4),
+        ((pages, Hkv, page, hd // 32), E8M0), ((pages, Hkv, page, hd // 32), E8M0)))
+    B = 2
+    at = 2 ** 31 // per
+    ids = torch.tensor([pages - 1, 0, 2 ** 32 // per, 2 ** 32 // per - 1, at, at - 1])
+    n = 3 * page
+    lengths = torch.tensor([n - 1, n - 40], dtype=torch.int32)
+    table = torch.full((B, width), -1, dtype=torch.int32)
+    table[:, :3] = ids.view(B, 3).int()
+    x = [torch.randn(B * n, Hkv, hd, generator=g).to(BF16) for _ in range(2)]
+    pos = torch.arange(n).repeat(B).int()
+    rows = torch.arange(B).repeat_interleave(n).int()
+    td = table.cuda()
+    ops.paged_kv_append_mx4(x[0].cuda(), x[1].cuda(), *cache, td, pos.cuda(), rows=rows.cuda())
+    vals = [ref.values(*ref.stored(t)) for t in x]
+    for got, want in zip(ops.paged_kv_read_mx4(*cache, td, pos.cuda(), rows=rows.cuda()), vals):
+        assert torch.equal(got.cpu().double(), want)
+    # the oracle's cache: the six pages alone
+    k, v = (t.view(B * 3, page, Hkv, hd).transpose(1, 2) for t in vals)
+    q = torch.randn(B, T, Hq, hd, generator=g).to(BF16)
+    got = ops.paged_attn_mx4(q.cuda(), *cache, td, lengths.cuda())
+    want, spread = ref.attend(q, k, v, torch.arange(6).view(B, 3).int(), lengths)
+    _attn_ok(got.cpu(), want, spread)
+
+
+def test_on_other_streams_and_two_at_once():
+    """Calls that overlap on two streams, over one cache, each with its own workspace."""
+    ops, g = _ops(), torch.Generator().manual_seed(8)
+    Hq, Hkv, hd, page = 8, 2, 64, 32
+    dev, k, v = _cache(300, Hkv, page, hd, g)
+    sets = []
+    for B, T, width in ((3, 2, 250), (5, 4, 200)):
+        table = torch.randint(0, 300, (B, width), generator=g).int()
+        q = torch.randn(B, T, Hq, hd, generator=g).to(BF16)
+        lengths = torch.randint(T, width * page + 1, (B,), generator=g).int()
+        sets.append((q, table, lengths))
+    given = [[t.cuda() for t in s] for s in sets]
+    want = [ops.paged_attn_mx4(q, *dev, t, n).cpu() for q, t, n in given]
+    for (q, table, lengths), w in zip(sets, want):
+        exact, spread = ref.attend(q, k, v, table, lengths)
+        _attn_ok(w, exact, spread)
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for (q, t, n), s in zip(given, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.paged_attn_mx4(q, *dev, t, n))
+        torch.cuda.synchronize()
+        for a, w in zip(got, want):
+            assert torch.equal(a.cpu(), w)
