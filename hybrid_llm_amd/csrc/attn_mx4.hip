@@ -11,18 +11,23 @@
 //     instruction and without rounding.  (The scaled matrix products that take 4-bit operands
 //     themselves align a block's products to its largest and lose what lies 2^-17 under it.)
 //   * S^T = K Q^T: a lane's K operand is its key's 16 bytes (8 for 64 dims) as they lie in
-//     the cache, loaded straight to registers, three steps ahead.  Lane l (g = l / 16)
-//     gets keys 4 g + r of a 16-key tile for column l % 16; two such tiles are, register
+//     the cache, loaded straight to registers, two rounds of the waves ahead.  Lane l (g = l /
+//     16) gets keys 4 g + r of a 16-key tile for column l % 16; two such tiles are, register
 //     by register, the B operand of a 32-key product O^T += V^T P^T under the key order
 //     4 g + j, 16 + 4 g + j.
 //   * V, loaded the same way, is put in bf16 into the wave's own 32 rows of LDS, whose
 //     transposing reads give V^T in that order.  A block scale belongs to a key and 32 dims,
 //     so scaling V costs nothing beyond its conversion, and scaling the weights would
 //     take one set of them per block.
-//   * a wave works alone and waits for no other; waves share a head tile where tables are
-//     short, and otherwise each takes an equal run of the flat list of all (sequence, head
-//     tile, step), found from the lengths on the device: partials of heads that are cut go to
-//     the workspace, and a second kernel joins them.
+//   * the waves of a workgroup take the 32-key steps of a head tile in turn and join their
+//     (m, l, O) in LDS.  Where tables are short a workgroup has a whole tile; otherwise an equal
+//     run of the flat list of all (sequence, head tile, step), found from the lengths on the
+//     device: partials of tiles that are cut go to the workspace, and a second kernel joins
+//     them.  A run of four waves instead of one has a quarter of the parts to store and join.
+// Measured, the call's kernels together (32 heads over 8 x 128): 4 sequences of 131072 tokens,
+// 570 MB, 106 us, 5.4 TB/s; 64 ragged ones of up to 4096 with 4 tokens each and capped scores,
+// 143 MB, 49 us, of which the join takes 6 and the first loads and the changes of tiles most of
+// what is past 28; 16 x 64 over 4, one sequence of 1023, 10 us, a chain of latencies.
 // Masked keys (past the length, before the window, in a page that the table does not name)
 // have their scores set to -inf and their V rows zeroed, so nothing that such a place holds
 // reaches a sum.  A block of V that is NaN counts as zeros in the product, and as NaN
@@ -43,7 +48,7 @@ __device__ __forceinline__ int32_t uniform_at(const int32_t* p, long long i) {
 }
 
 constexpr int kMxStep = 32;      // keys a step
-constexpr int kMxAhead = 2;      // steps in registers
+constexpr int kMxAhead = 2;      // steps of a wave in registers
 constexpr int kMxPad = 8;        // steps that a head tile costs besides
 constexpr int kMxLeast = 16;     // places of a run at the least
 constexpr float kMxLowest = -3.402823466e38f;
@@ -315,8 +320,8 @@ void mx4_attn_kernel(const Mx4Args a) {
   const uint32_t base = lds_addr(mem);
 
   // The round that is loaded next, and its page ids.  Every wave loads something every round,
-  // its tile's last step where it has none of its own, so that the compiler can count the
-  // loads that are in flight: past a branch around them it would wait for all.
+  // the cache's first rows where it has no step, so that the compiler can count the loads that
+  // are in flight: past a branch around them it would wait for all.
   MxPlace to = at;
   bool more = true;
   int ipage[2], istep;
@@ -330,15 +335,17 @@ void mx4_attn_kernel(const Mx4Args a) {
   unsigned holes[kMxAhead];
   MxStage<HD> stage[kMxAhead];
   const auto issue = [&](int d) __attribute__((always_inline)) {
-    holes[d] = !more || to.begin + to.it * W + wave >= to.end ? 3u : 0u;
+    const bool none = !more || to.begin + to.it * W + wave >= to.end;
+    holes[d] = 0u;
     global_u8 kp[2], vp[2], ksp[2], vsp[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int key = istep * kMxStep + 16 * h;
-      const bool ok = ipage[h] >= 0 && ipage[h] < a.pages;
+      const bool ok = !none && ipage[h] >= 0 && ipage[h] < a.pages;
       if (!ok) holes[d] |= 1u << h;
-      const uint64_t off = static_cast<uint64_t>(ok ? ipage[h] : 0) * a.page_bytes +
-                           static_cast<uint32_t>((to.kvh << a.shift) + (key & ((1 << a.shift) - 1))) * CB;
+      const uint64_t off = ok ? static_cast<uint64_t>(ipage[h]) * a.page_bytes +
+                                    static_cast<uint32_t>((to.kvh << a.shift) + (key & ((1 << a.shift) - 1))) * CB
+                              : 0;
       static_assert(CB == 16 * SB, "scales lie as the codes do");
       kp[h] = mx_base(a.kc, off);
       vp[h] = mx_base(a.vc, off);
