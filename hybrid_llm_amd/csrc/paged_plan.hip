@@ -14,7 +14,8 @@
 // 4096 tokens is one workgroup and one launch; a larger one spreads its tokens over many
 // workgroups that each repeat the scan of the sequences (up to 4 a thread, in registers)
 // and stores what the second launch needs to hand the pages out, since a page may be pushed
-// and popped in one call.
+// and popped in one call.  Measured: 64 sequences of a token each 4.3 us; 127 prompts of
+// 262139 tokens 9.6 + 4.0.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "paged.hpp"

@@ -10,13 +10,17 @@
 // more than their distance at large V; so exponentials and sums are in 64 bits, which this
 // chip adds and multiplies at the rate of single 32-bit ones.
 //
-// Bound by the read of the logits (then of one draft row a sequence).  Rows are cut into
-// chunks of 4096 ids, a workgroup each, so that one sequence's rows fill the chip too:
-//   1. each chunk's maximum and sum of exponentials under it;
+// Bound by the read of the logits (then of one draft row a sequence) where there are many rows,
+// by latency where there are few.  Rows are cut into chunks of 4096 ids, so that one sequence's
+// rows fill the chip too:
+//   1. a workgroup's chunks of a row: their maximum and sum of exponentials under it;
 //   2. per sequence: from those, which drafts are kept;
-//   3. per (sequence, chunk): its sum of the distribution to draw from;
+//   3. per sequence and chunk: its sum of the distribution to draw from;
 //   4. per sequence: the chunk in which the sum passes the threshold, and the id in it.
 // Greedy (T = 0): each row's first largest id, then the comparison: two launches.
+// Measured, 64 sequences of 4 drafts, 128256 ids: 40 + 5 + 18 + 8 us, the first at 4.1 TB/s (its
+// exponentials in 64 bits alone take 31 us, under the loads), the third at 3.5; greedy, 64 x 4
+// rows of 32000: 9 + 2 to 3 us, 3.5 TB/s.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "paged.hpp"
