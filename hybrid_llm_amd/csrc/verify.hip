@@ -17,10 +17,11 @@
 //   2. per sequence: from those, which drafts are kept;
 //   3. per sequence and chunk: its sum of the distribution to draw from;
 //   4. per sequence: the chunk in which the sum passes the threshold, and the id in it.
+// 2 to 4 are one launch for few sequences, where launches are what takes long.
 // Greedy (T = 0): each row's first largest id, then the comparison: two launches.
 // Measured, 64 sequences of 4 drafts, 128256 ids: 40 + 5 + 18 + 8 us, the first at 4.1 TB/s (its
 // exponentials in 64 bits alone take 31 us, under the loads), the third at 3.5; greedy, 64 x 4
-// rows of 32000: 9 + 2 to 3 us, 3.5 TB/s.
+// rows of 32000: 9 + 2 to 3 us, 3.5 TB/s; one sequence of 4 drafts, 32000 ids: 4.2 + 9.5.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "paged.hpp"
@@ -43,6 +44,7 @@ struct VerifyArgs {
   double* sum;                  // [B (K + 1), parts]: its sum under that maximum
   double *rest, *plain;         // [B, chunks]: of max(e - q Z, 0) and e of the drawn row
   struct Decision* decided;     // [B]
+  uint32_t* done;               // [B]: chunks whose sums are stored
   double c;                     // log2(e) / T
   int B, K, V;
   int row_chunks, per_part, parts;  // chunks of a row, of a first workgroup, and those of a row
@@ -144,6 +146,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_rows_kernel(const VerifyAr
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   const int c0 = part * a.per_part, c1 = min(a.row_chunks, c0 + a.per_part), wave = threadIdx.x >> 6;
   const float* x = a.logits + static_cast<long long>(row) * a.V;
+  if (!GREEDY && part == 0 && threadIdx.x == 0 && row % (a.K + 1) == 0) a.done[row / (a.K + 1)] = 0u;
   float v[kVerPer], next[kVerPer];
   load_ids<kVerPer>(x, a.V, c0 * kVerChunk, a.vec4, -INFINITY, v);
   float top = -INFINITY;
@@ -215,12 +218,12 @@ struct Decision {
   bool rejected;  // a draft was put away there
 };
 
-// Which drafts of a sequence are kept: every row by 16 lanes, their verdicts through LDS.
+// Which drafts of a sequence are kept: every row by 16 lanes, their verdicts through LDS.  By a
+// workgroup, with the same result in each.
 template <bool GREEDY>
-__global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const VerifyArgs a) {
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, int b) {
   __shared__ Row rows[kMaxDrafts + 1];
   __shared__ int keep[kMaxDrafts + 1];
-  const int b = blockIdx.x;
   const int sub = threadIdx.x >> 4, lane = threadIdx.x & 15;
   const int count = a.counts ? min(max(a.counts[b], 0), a.K) : a.K;
   for (int t0 = 0; t0 <= count; t0 += kVerThreads / 16) {
@@ -267,16 +270,26 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const Verify
   while (d.kept < count && keep[d.kept]) ++d.kept;
   d.rejected = d.kept < count;
   d.row = rows[d.kept];
-  // the kept drafts, and (greedy) the row's id; a draw writes its own later
+  return d;
+}
+
+// A sequence's outputs: the kept drafts, the new token, then -1.
+__device__ __forceinline__ void put_tokens(const VerifyArgs& a, int b, const Decision& d, int id) {
   for (int t = threadIdx.x; t <= a.K; t += kVerThreads) {
     const int64_t at = static_cast<int64_t>(b) * (a.K + 1) + t;
-    a.tokens[at] = t < d.kept ? a.drafts[static_cast<int64_t>(b) * a.K + t]
-                   : GREEDY && t == d.kept ? static_cast<int>(key_index(d.row.key)) : -1;
+    a.tokens[at] = t < d.kept ? a.drafts[static_cast<int64_t>(b) * a.K + t] : t == d.kept ? id : -1;
   }
-  if (threadIdx.x == 0) {
-    a.accepted[b] = d.kept;
-    if (!GREEDY) a.decided[b] = d;
-  }
+  if (threadIdx.x == 0) a.accepted[b] = d.kept;
+}
+
+template <bool GREEDY>
+__global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const VerifyArgs a) {
+  const int b = blockIdx.x;
+  const Decision d = decide<GREEDY>(a, b);
+  if (GREEDY)
+    put_tokens(a, b, d, static_cast<int>(key_index(d.row.key)));
+  else if (threadIdx.x == 0)
+    a.decided[b] = d;
 }
 
 // Weights of the drawn row at this thread's PER ids of a chunk, in order: put(k, e, max(e - q Z, 0)).
@@ -302,11 +315,11 @@ __device__ __forceinline__ void draw_weights(const VerifyArgs& a, int b, const D
   }
 }
 
+// A chunk's sums of the distribution to draw from, stored by thread 0.
 template <int PER>
-__global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(const VerifyArgs a) {
+__device__ __forceinline__ void chunk_sums(const VerifyArgs& a, int b, const Decision& d) {
   __shared__ double sums[2][kVerWaves];
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const Decision d = a.decided[b];
+  const int chunk = blockIdx.x - b * a.chunks;
   double se = 0, sr = 0;
   draw_weights<PER>(a, b, d, chunk * (kVerThreads * PER), [&](int, double e, double rest) {
     se += e;
@@ -326,11 +339,33 @@ __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(const VerifyAr
 }
 
 template <int PER>
+__global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(const VerifyArgs a) {
+  const int b = blockIdx.x / a.chunks;
+  chunk_sums<PER>(a, b, a.decided[b]);
+}
+
+// The draw: a workgroup a sequence, or (JOINED) one a chunk, which decides and sums by itself and
+// draws if it is its sequence's last to come so far.  None waits for another; which one comes
+// last has no effect on what it reads or adds up.
+template <int PER, bool JOINED>
 __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyArgs a) {
   __shared__ double part[PER / 4][kVerWaves];
-  __shared__ int first, last;
-  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Decision d = a.decided[b];
+  __shared__ int first, last, closes;
+  const int b = JOINED ? blockIdx.x / a.chunks : blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Decision d = JOINED ? decide<false>(a, b) : a.decided[b];
+  if (JOINED) {
+    chunk_sums<PER>(a, b, d);
+    if (threadIdx.x == 0) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+      const uint32_t before = __hip_atomic_fetch_add(a.done + b, 1u, __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT);
+      closes = before + 1u == static_cast<uint32_t>(a.chunks);
+    }
+    __syncthreads();
+    if (!closes) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  }
   // The chunk in which the running sum passes the threshold, by every wave alike: sums of 64
   // chunks at a time, each lane's in the chunks' order behind those before them.
   const double* sums = a.rest + static_cast<long long>(b) * a.chunks;
@@ -424,8 +459,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyAr
   }
   __syncthreads();
   // u at 1, or sums that rounded below the threshold: the last id with any weight
-  if (threadIdx.x == 0)
-    a.tokens[static_cast<long long>(b) * (a.K + 1) + d.kept] = first < a.V ? first : last;
+  put_tokens(a, b, d, first < a.V ? first : last);
 }
 
 inline int verify_chunks(int V, int chunk) { return (V + chunk - 1) / chunk; }
@@ -434,6 +468,14 @@ inline int verify_chunks(int V, int chunk) { return (V + chunk - 1) / chunk; }
 // a thread forms one after the other are what takes long (1 x 32000: the two kernels 14 -> 8 us).
 inline int verify_draw_per(int B, int V) {
   return static_cast<int64_t>(B) * verify_chunks(V, kVerChunk) < compute_units() ? 4 : 16;
+}
+
+// Whether decisions, sums and draw are one launch: each workgroup then hands its sums to the other
+// dies' caches, which takes longer the more of them do.  us of a call joined / in three launches,
+// 4 drafts: 1 x 32000 ids 13.2 / 17.8 (in a graph 13.0 / 14.5), 4 x 32000, 128 workgroups, 14.0 /
+// 18.8 (14.1 / 14.9), 8 x 32000 18.4 / 18.8 (18.7 / 15.7), 31 x 32000 34 / 21, 1 x 128256 14.7 / 18.3.
+inline bool verify_joined(int B, int chunks, int per) {
+  return per == 4 && 2ll * B * chunks <= compute_units();
 }
 
 // Chunks of a row that one workgroup of the first kernel takes: as many as leave five a CU, which
@@ -453,7 +495,7 @@ extern "C" int64_t llmy_verify_drafts_workspace_bytes(int32_t B, int32_t K, int3
   const int64_t parts = rows * verify_chunks(V, kVerChunk);
   if (parts >= (1ll << 31)) return -1;  // the grid
   const int64_t draws = static_cast<int64_t>(B) * verify_chunks(V, kVerThreads * verify_draw_per(B, V));
-  return 16 * (parts + draws) + static_cast<int64_t>(sizeof(Decision)) * B;
+  return 16 * (parts + draws) + (static_cast<int64_t>(sizeof(Decision)) + 8) * B;
 }
 
 extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* draft_tokens,
@@ -493,6 +535,7 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
   a.rest = a.sum + rows * a.parts;
   a.plain = a.rest + static_cast<int64_t>(B) * a.chunks;
   a.decided = reinterpret_cast<Decision*>(a.plain + static_cast<int64_t>(B) * a.chunks);
+  a.done = reinterpret_cast<uint32_t*>(a.decided + B);
   const hipStream_t s = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(rows * a.parts)), draws(static_cast<unsigned>(B) * a.chunks);
   if (greedy) {
@@ -501,13 +544,17 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
     return launch_status();
   }
   hipLaunchKernelGGL(verify_rows_kernel<false>, grid, dim3(kVerThreads), 0, s, a);
+  if (verify_joined(B, a.chunks, per)) {
+    hipLaunchKernelGGL((verify_draw_kernel<4, true>), draws, dim3(kVerThreads), 0, s, a);
+    return launch_status();
+  }
   hipLaunchKernelGGL(verify_decide_kernel<false>, dim3(B), dim3(kVerThreads), 0, s, a);
   if (per == 4) {
     hipLaunchKernelGGL(verify_sums_kernel<4>, draws, dim3(kVerThreads), 0, s, a);
-    hipLaunchKernelGGL(verify_draw_kernel<4>, dim3(B), dim3(kVerThreads), 0, s, a);
+    hipLaunchKernelGGL((verify_draw_kernel<4, false>), dim3(B), dim3(kVerThreads), 0, s, a);
   } else {
     hipLaunchKernelGGL(verify_sums_kernel<16>, draws, dim3(kVerThreads), 0, s, a);
-    hipLaunchKernelGGL(verify_draw_kernel<16>, dim3(B), dim3(kVerThreads), 0, s, a);
+    hipLaunchKernelGGL((verify_draw_kernel<16, false>), dim3(B), dim3(kVerThreads), 0, s, a);
   }
   return launch_status();
 }

@@ -229,3 +229,34 @@ def test_on_another_stream_and_two_at_once():
             want, kept, margin = ref.verify(*c)
             assert float(margin.min()) > NEAR
             assert torch.equal(g[0].cpu(), want) and torch.equal(g[1].cpu(), kept)
+
+
+def test_few_rows_and_many_replayed_in_one_graph():
+    """Calls of every form, back to back in one graph, replayed over inputs that change: what a call
+    counts on the GPU starts anew each time."""
+    ops = _ops()
+    sizes = [(1, 4, 32000), (4, 2, 32000), (8, 2, 32000), (1, 63, 9000), (2, 3, 60000), (70, 3, 17000)]
+    sets = [[_case(*n, 50 + i + 10 * r) for i, n in enumerate(sizes)] for r in range(3)]
+    dev = [[None if t is None or isinstance(t, float) else t.cuda() for t in c] for c in sets[0]]
+
+    def calls():
+        return [ops.verify_drafts(d[0], d[1], d[2], temperature=0.8, draft_probs=d[4], counts=d[5])
+                for d in dev]
+
+    calls()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    for r in (0, 1, 2, 0, 0):
+        for d, c in zip(dev, sets[r]):
+            for a, b in zip(d, c):
+                if a is not None:
+                    a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = calls()
+        for c, got, now in zip(sets[r], out, eager):
+            want, kept, margin = ref.verify(*c)
+            assert float(margin.min()) > NEAR
+            for tokens, accepted in (got, now):
+                assert torch.equal(tokens.cpu(), want) and torch.equal(accepted.cpu(), kept)
