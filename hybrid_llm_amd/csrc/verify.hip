@@ -11,15 +11,15 @@
 // chip adds and multiplies at the rate of single 32-bit ones.
 //
 // Bound by the read of the logits (then of one draft row a sequence) where there are many rows,
-// by latency where there are few.  Rows are cut into chunks of 4096 ids, so that one sequence's
-// rows fill the chip too:
+// by latency where there are few.  Rows are cut into chunks, so that one sequence's rows fill
+// the chip too:
 //   1. a workgroup's chunks of a row: their maximum and sum of exponentials under it;
 //   2. per sequence: from those, which drafts are kept;
 //   3. per sequence and chunk: its sum of the distribution to draw from;
 //   4. per sequence: the chunk in which the sum passes the threshold, and the id in it.
 // 2 to 4 are one launch for few sequences, where launches are what takes long.
 // Greedy (T = 0): each row's first largest id, then the comparison: two launches.
-// Measured, 64 sequences of 4 drafts, 128256 ids: 40 + 5 + 18 + 8 us, the first at 4.1 TB/s (its
+// Measured, 64 sequences of 4 drafts, 128256 ids: 40 + 5 + 18 + 6 us, the first at 4.1 TB/s (its
 // exponentials in 64 bits alone take 31 us, under the loads), the third at 3.5; greedy, 64 x 4
 // rows of 32000: 9 + 2 to 3 us, 3.5 TB/s; one sequence of 4 drafts, 32000 ids: 4.2 + 9.5.
 #include "common.hpp"
@@ -31,6 +31,10 @@ namespace llmy {
 constexpr int kVerThreads = 256, kVerPer = 16;
 constexpr int kVerChunk = kVerThreads * kVerPer;
 constexpr int kVerWaves = kVerThreads / kWave;
+// Ids a thread of a draw, few, so that one sequence spreads over the chip and many hide their
+// loads (1 x 32000 ids, 16 a thread against 4: 14 and 8 us; 64 x 128256: 28 and 25).
+constexpr int kVerDraw = 4, kVerDrawChunk = kVerThreads * kVerDraw;
+static_assert(kVerDraw == 4, "sums in the ids' order: a thread's are neighbours");
 constexpr int kMaxDrafts = 63;  // rows of a sequence in LDS
 
 struct VerifyArgs {
@@ -44,7 +48,7 @@ struct VerifyArgs {
   double* sum;                  // [B (K + 1), parts]: its sum under that maximum
   double *rest, *plain;         // [B, chunks]: of max(e - q Z, 0) and e of the drawn row
   struct Decision* decided;     // [B]
-  uint32_t* done;               // [B]: chunks whose sums are stored
+  uint32_t* done;               // [B] in their place: chunks whose sums are stored
   double c;                     // log2(e) / T
   int B, K, V;
   int row_chunks, per_part, parts;  // chunks of a row, of a first workgroup, and those of a row
@@ -292,22 +296,22 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(const Verify
     a.decided[b] = d;
 }
 
-// Weights of the drawn row at this thread's PER ids of a chunk, in order: put(k, e, max(e - q Z, 0)).
-template <int PER, class Put>
+// Weights of the drawn row at this thread's ids of a chunk, in order: put(k, e, max(e - q Z, 0)).
+template <class Put>
 __device__ __forceinline__ void draw_weights(const VerifyArgs& a, int b, const Decision& d, int base,
                                              Put put) {
   const long long row = static_cast<long long>(b) * (a.K + 1) + d.kept;
-  float x[PER], q[PER];
-  load_ids<PER>(a.logits + row * a.V, a.V, base, a.vec4, -INFINITY, x);
+  float x[kVerDraw], q[kVerDraw];
+  load_ids<kVerDraw>(a.logits + row * a.V, a.V, base, a.vec4, -INFINITY, x);
   const long long draft = static_cast<long long>(b) * a.K + d.kept;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) q[k] = 0.f;
-  if (d.rejected && a.probs) load_ids<PER>(a.probs + draft * a.V, a.V, base, a.vec4, 0.f, q);
+  for (int k = 0; k < kVerDraw; ++k) q[k] = 0.f;
+  if (d.rejected && a.probs) load_ids<kVerDraw>(a.probs + draft * a.V, a.V, base, a.vec4, 0.f, q);
   const int certain = d.rejected && !a.probs ? a.drafts[draft] : -1;
   const double top = key_value(d.row.key);
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int id = base + 1024 * (k >> 2) + 4 * static_cast<int>(threadIdx.x) + (k & 3);
+  for (int k = 0; k < kVerDraw; ++k) {
+    const int id = base + kVerDraw * static_cast<int>(threadIdx.x) + k;
     const double e = d.row.sure ? (static_cast<uint32_t>(id) == key_index(d.row.key) ? 1.0 : 0.0)
                                 : weight(x[k], a.c, top);
     const double less = id == certain ? d.row.z : static_cast<double>(q[k]) * d.row.z;
@@ -316,12 +320,11 @@ __device__ __forceinline__ void draw_weights(const VerifyArgs& a, int b, const D
 }
 
 // A chunk's sums of the distribution to draw from, stored by thread 0.
-template <int PER>
 __device__ __forceinline__ void chunk_sums(const VerifyArgs& a, int b, const Decision& d) {
   __shared__ double sums[2][kVerWaves];
   const int chunk = blockIdx.x - b * a.chunks;
   double se = 0, sr = 0;
-  draw_weights<PER>(a, b, d, chunk * (kVerThreads * PER), [&](int, double e, double rest) {
+  draw_weights(a, b, d, chunk * kVerDrawChunk, [&](int, double e, double rest) {
     se += e;
     sr += rest;
   });
@@ -338,24 +341,23 @@ __device__ __forceinline__ void chunk_sums(const VerifyArgs& a, int b, const Dec
   }
 }
 
-template <int PER>
 __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(const VerifyArgs a) {
   const int b = blockIdx.x / a.chunks;
-  chunk_sums<PER>(a, b, a.decided[b]);
+  chunk_sums(a, b, a.decided[b]);
 }
 
 // The draw: a workgroup a sequence, or (JOINED) one a chunk, which decides and sums by itself and
 // draws if it is its sequence's last to come so far.  None waits for another; which one comes
 // last has no effect on what it reads or adds up.
-template <int PER, bool JOINED>
+template <bool JOINED>
 __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ double part[PER / 4][kVerWaves];
+  __shared__ double part[kVerWaves];
   __shared__ int first, last, closes;
   const int b = JOINED ? blockIdx.x / a.chunks : blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Decision d = JOINED ? decide<false>(a, b) : a.decided[b];
   if (JOINED) {
-    chunk_sums<PER>(a, b, d);
+    chunk_sums(a, b, d);
     if (threadIdx.x == 0) {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
       const uint32_t before = __hip_atomic_fetch_add(a.done + b, 1u, __ATOMIC_RELAXED,
@@ -408,44 +410,31 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyAr
     run += __shfl(s, kWave - 1, kWave);
   }
   if (threadIdx.x == 0) first = a.V, last = -1;
-  double rest[PER];
-  const int base = chunk * (kVerThreads * PER);
-  draw_weights<PER>(a, b, d, base, [&](int k, double e, double r) { rest[k] = spare ? r : e; });
-  // running sums in the ids' order: blocks of 1024 ids, 4 a thread
-  double part_upto[PER / 4];
+  double rest[kVerDraw];
+  const int base = chunk * kVerDrawChunk;
+  draw_weights(a, b, d, base, [&](int k, double e, double r) { rest[k] = spare ? r : e; });
+  // running sums in the ids' order
+  double sum = (rest[0] + rest[1]) + (rest[2] + rest[3]);
 #pragma unroll
-  for (int i = 0; i < PER / 4; ++i) {
-    double s = (rest[4 * i] + rest[4 * i + 1]) + (rest[4 * i + 2] + rest[4 * i + 3]);
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const double x = __shfl_up(s, o, kWave);
-      if (lane >= o) s += x;
-    }
-    part_upto[i] = s;
-    if (lane == kWave - 1) part[i][wave] = s;
+  for (int o = 1; o < kWave; o <<= 1) {
+    const double x = __shfl_up(sum, o, kWave);
+    if (lane >= o) sum += x;
   }
+  if (lane == kWave - 1) part[wave] = sum;
   __syncthreads();
-  double start = before;
+#pragma unroll
+  for (int w = 0; w < kVerWaves; ++w)
+    if (w < wave) before += part[w];
+  const double prev = __shfl_up(sum, 1, kWave);
+  if (lane) before += prev;
   int at_first = a.V, at_last = -1;
 #pragma unroll
-  for (int i = 0; i < PER / 4; ++i) {
-    double c = start;
-#pragma unroll
-    for (int w = 0; w < kVerWaves; ++w) {
-      if (w < wave) c += part[i][w];
-      start += part[i][w];
-    }
-    const double prev = __shfl_up(part_upto[i], 1, kWave);
-    if (lane) c += prev;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double w = rest[4 * i + j];
-      c += w;
-      const int id = base + 1024 * i + 4 * static_cast<int>(threadIdx.x) + j;
-      if (w > 0) {
-        if (c > goal) at_first = min(at_first, id);
-        at_last = max(at_last, id);
-      }
+  for (int j = 0; j < kVerDraw; ++j) {
+    before += rest[j];
+    const int id = base + kVerDraw * static_cast<int>(threadIdx.x) + j;
+    if (rest[j] > 0) {
+      if (before > goal) at_first = min(at_first, id);
+      at_last = max(at_last, id);
     }
   }
 #pragma unroll
@@ -464,18 +453,12 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(const VerifyAr
 
 inline int verify_chunks(int V, int chunk) { return (V + chunk - 1) / chunk; }
 
-// Ids a thread of a draw: 16, or 4 where that many leave most of the chip idle and the exponentials
-// a thread forms one after the other are what takes long (1 x 32000: the two kernels 14 -> 8 us).
-inline int verify_draw_per(int B, int V) {
-  return static_cast<int64_t>(B) * verify_chunks(V, kVerChunk) < compute_units() ? 4 : 16;
-}
-
 // Whether decisions, sums and draw are one launch: each workgroup then hands its sums to the other
 // dies' caches, which takes longer the more of them do.  us of a call joined / in three launches,
 // 4 drafts: 1 x 32000 ids 13.2 / 17.8 (in a graph 13.0 / 14.5), 4 x 32000, 128 workgroups, 14.0 /
 // 18.8 (14.1 / 14.9), 8 x 32000 18.4 / 18.8 (18.7 / 15.7), 31 x 32000 34 / 21, 1 x 128256 14.7 / 18.3.
-inline bool verify_joined(int B, int chunks, int per) {
-  return per == 4 && 2ll * B * chunks <= compute_units();
+inline bool verify_joined(int B, int chunks) {
+  return 2ll * B * chunks <= compute_units();
 }
 
 // Chunks of a row that one workgroup of the first kernel takes: as many as leave five a CU, which
@@ -493,9 +476,9 @@ extern "C" int64_t llmy_verify_drafts_workspace_bytes(int32_t B, int32_t K, int3
   if (B < 0 || K < 1 || K > kMaxDrafts || V < 1 || V > (1 << 30)) return -1;
   const int64_t rows = static_cast<int64_t>(B) * (K + 1);
   const int64_t parts = rows * verify_chunks(V, kVerChunk);
-  if (parts >= (1ll << 31)) return -1;  // the grid
-  const int64_t draws = static_cast<int64_t>(B) * verify_chunks(V, kVerThreads * verify_draw_per(B, V));
-  return 16 * (parts + draws) + (static_cast<int64_t>(sizeof(Decision)) + 8) * B;
+  const int64_t draws = static_cast<int64_t>(B) * verify_chunks(V, kVerDrawChunk);
+  if (parts >= (1ll << 31) || draws >= (1ll << 31)) return -1;  // the grids
+  return 16 * (parts + draws) + static_cast<int64_t>(sizeof(Decision)) * B;
 }
 
 extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* draft_tokens,
@@ -521,10 +504,9 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
   VerifyArgs a{};
   a.logits = logits; a.drafts = draft_tokens; a.probs = draft_probs; a.counts = counts; a.u = u;
   a.tokens = tokens; a.accepted = accepted;
-  const int per = verify_draw_per(B, V);
   a.B = B; a.K = K; a.V = V;
   a.row_chunks = verify_chunks(V, kVerChunk);
-  a.chunks = verify_chunks(V, kVerThreads * per);
+  a.chunks = verify_chunks(V, kVerDrawChunk);
   // (2^800 already takes the least difference of two logits, 2^-149, past every weight)
   a.c = greedy ? 0. : fmin(1.4426950408889634 / temperature, 0x1p800);
   a.vec4 = V % 4 == 0 && aligned(logits, 16) && (!draft_probs || aligned(draft_probs, 16));
@@ -535,7 +517,7 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
   a.rest = a.sum + rows * a.parts;
   a.plain = a.rest + static_cast<int64_t>(B) * a.chunks;
   a.decided = reinterpret_cast<Decision*>(a.plain + static_cast<int64_t>(B) * a.chunks);
-  a.done = reinterpret_cast<uint32_t*>(a.decided + B);
+  a.done = reinterpret_cast<uint32_t*>(a.decided);  // (of a joined draw, which stores no decisions)
   const hipStream_t s = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(rows * a.parts)), draws(static_cast<unsigned>(B) * a.chunks);
   if (greedy) {
@@ -544,17 +526,12 @@ extern "C" int32_t llmy_verify_drafts_f32(const float* logits, const int32_t* dr
     return launch_status();
   }
   hipLaunchKernelGGL(verify_rows_kernel<false>, grid, dim3(kVerThreads), 0, s, a);
-  if (verify_joined(B, a.chunks, per)) {
-    hipLaunchKernelGGL((verify_draw_kernel<4, true>), draws, dim3(kVerThreads), 0, s, a);
+  if (verify_joined(B, a.chunks)) {
+    hipLaunchKernelGGL(verify_draw_kernel<true>, draws, dim3(kVerThreads), 0, s, a);
     return launch_status();
   }
   hipLaunchKernelGGL(verify_decide_kernel<false>, dim3(B), dim3(kVerThreads), 0, s, a);
-  if (per == 4) {
-    hipLaunchKernelGGL(verify_sums_kernel<4>, draws, dim3(kVerThreads), 0, s, a);
-    hipLaunchKernelGGL((verify_draw_kernel<4, false>), dim3(B), dim3(kVerThreads), 0, s, a);
-  } else {
-    hipLaunchKernelGGL(verify_sums_kernel<16>, draws, dim3(kVerThreads), 0, s, a);
-    hipLaunchKernelGGL((verify_draw_kernel<16, false>), dim3(B), dim3(kVerThreads), 0, s, a);
-  }
+  hipLaunchKernelGGL(verify_sums_kernel, draws, dim3(kVerThreads), 0, s, a);
+  hipLaunchKernelGGL(verify_draw_kernel<false>, dim3(B), dim3(kVerThreads), 0, s, a);
   return launch_status();
 }
