@@ -585,7 +585,8 @@ def paged_kv_append_mx4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     """paged_kv_append into a cache held in 4 bits (mx4_cache): codes k_cache, v_cache
     [pages,Hkv,page,hd/2] float4_e2m1fn_x2 and scales k_scales, v_scales [pages,Hkv,page,hd/32]
     float8_e8m0fnu, one for each 32 dims of a row (see llmy_paged_kv_append_mx4).  Returns
-    q_out."""
+    q_out, whose rows of tokens at negative positions stay as they were: one made here holds
+    nothing of use there."""
     N, Hkv, hd = k.shape
     dev = _device()
     pk, kr, kh = _heads(k, "k", (N, Hkv, hd), dev)
@@ -679,7 +680,8 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, page_table: torc
     n_free [1] (its height) are updated in place.  Returns (cu_seqlens [B+1], rows [tokens],
     positions [tokens], lengths [B]) for the packed new tokens, of which ``tokens`` bounds the
     number; a token whose sequence got no pages has position -1, entries behind the last row
-    and position -1.  ``workspace``: a buffer of llmy_paged_plan_workspace_bytes that no
+    and position -1.  Lengths are those with the new tokens; of a sequence that got no pages, the
+    one before (0 where reset).  ``workspace``: a buffer of llmy_paged_plan_workspace_bytes that no
     overlapping call uses."""
     dev = _device()
     B, width, pt = _table(page_table, dev)
