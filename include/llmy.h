@@ -828,8 +828,8 @@ int64_t llmy_verify_drafts_workspace_bytes(int32_t B, int32_t K, int32_t V);
  * draft_tokens [B, K]; draft_probs [B, K, V] fp32, the distributions q_t that they were drawn
  * from, or NULL: q_t is 1 at the draft; counts [B] or NULL: drafts there are (0 to K; else K);
  * u [B, K + 1] fp32 in [0, 1).  Draft x_t is kept while u_t q_t(x_t) < p_t(x_t) (one outside
- * [0, V) is not); the first that is not is replaced by a draw from max(p_t - q_t, 0) (where
- * nothing is left, from p_t), and behind the last comes a draw from that row's p: the first
+ * [0, V) is not); the first that is not is replaced by a draw from max(p_t - q_t, 0) (q_t that
+ * is NaN: not kept, 0 in the difference; where nothing is left, from p_t), and behind the last comes a draw from that row's p: the first
  * id, in order, whose running sum passes u[b][K] times the whole.  tokens [B, K + 1]: the
  * kept drafts, the drawn id, then -1; accepted [B]: drafts kept.  temperature <= 0: a draft
  * is kept while it is its row's first largest id, and that id follows; u is not read.  A

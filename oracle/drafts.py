@@ -89,7 +89,7 @@ def verify(logits, draft_tokens, u, temperature=1.0, draft_probs=None, counts=No
                     tokens[b, t] = x
                     t += 1
                     continue
-            rest = torch.where(p > q, p - q, 0)
+            rest = torch.where(q.isnan(), p, torch.where(p > q, p - q, 0))
             rest = rest if temperature > 0 and float(rest.sum()) > 0 else p
             break
         c = rest.cumsum(0)
