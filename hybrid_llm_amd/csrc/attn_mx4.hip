@@ -271,7 +271,8 @@ void mx4_attn_kernel(const Mx4Args a) {
       at.begin = cur.s0 + max(0, p0 - kMxPad);
       at.end = cur.s0 + max(0, p1 - kMxPad);
       at.left = count - (p1 - p0);
-      if (at.end == at.begin) return;  // the pad alone: its steps begin the next run
+      // (at least a step: a run is longer than a tile's pad, and the last one ends with a tile)
+      static_assert(kMxLeast > kMxPad, "a run of a pad alone");
     }
     at.sequence(a, cur.len, cur.lo);
     if (at.begin == at.end) {  // nothing to see (a whole tile): zeros
