@@ -314,8 +314,9 @@ __device__ __forceinline__ void draw_weights(const VerifyArgs& a, int b, const D
     const int id = base + kVerDraw * static_cast<int>(threadIdx.x) + k;
     const double e = d.row.sure ? (static_cast<uint32_t>(id) == key_index(d.row.key) ? 1.0 : 0.0)
                                 : weight(x[k], a.c, top);
-    const double less = id == certain ? d.row.z : static_cast<double>(q[k]) * d.row.z;
-    put(k, e, e > less ? e - less : less != less ? e : 0.0);  // (a NaN in q takes nothing off)
+    const float qk = q[k] == q[k] ? q[k] : 0.f;  // (a NaN in q takes nothing off)
+    const double less = id == certain ? d.row.z : static_cast<double>(qk) * d.row.z;
+    put(k, e, e > less ? e - less : 0.0);
   }
 }
 
