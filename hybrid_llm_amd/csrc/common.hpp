@@ -38,7 +38,8 @@ __device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 
-// 8 codes of a 4-bit cache under their block's scale byte as bf16 (exact).
+// 8 codes of a 4-bit cache under their block's scale byte as bf16: exact, infinite past bf16's end.
+// The conversion takes the scale's exponent alone: 2^-127 under byte 0, NaN under 255.
 __device__ __forceinline__ uint4 mx4_to_bf16(uint32_t w, uint32_t byte) {
   const float step = __uint_as_float(byte << 23);
   uint4 r;

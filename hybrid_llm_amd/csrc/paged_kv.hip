@@ -5,7 +5,8 @@
 //   (y_a, y_b) -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t),  t = pos * inv_freq[i]
 //
 // for the pairs (a, b) = (i, i + half) or (2i, 2i + 1) of the first 2 half dims; the
-// other dims pass.  All in fp32 from the bf16 rows to one rounding at the store.
+// other dims pass.  In fp32 from the bf16 rows to one rounding at the store; keys of a 4-bit
+// cache in fp64.
 //
 // The angle of a far position has more digits than fp32 holds (pos 2^20 at
 // inv_freq 1 leaves 2^-3 of a radian), so pos * inv_freq / 2 pi is formed in fp64,

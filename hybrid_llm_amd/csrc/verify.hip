@@ -19,9 +19,9 @@
 //   4. per sequence: the chunk in which the sum passes the threshold, and the id in it.
 // 2 to 4 are one launch for few sequences, where launches are what takes long.
 // Greedy (T = 0): each row's first largest id, then the comparison: two launches.
-// Measured, 64 sequences of 4 drafts, 128256 ids: 40 + 5 + 18 + 6 us, the first at 4.1 TB/s (its
-// exponentials in 64 bits alone take 31 us, under the loads), the third at 3.5; greedy, 64 x 4
-// rows of 32000: 9 + 2 to 3 us, 3.5 TB/s; one sequence of 4 drafts, 32000 ids: 4.2 + 9.5.
+// Measured, 64 sequences of 4 drafts, 128256 ids: 40 to 42 + 5 + 19 to 20 + 6.5 us, the first at 4 TB/s
+// (its exponentials in 64 bits alone take 31 us, under the loads), the third at 3.0 to 3.2; greedy,
+// 64 x 4 rows of 32000: 9.4 + 2 to 3 us, 3.5 TB/s; one sequence of 4 drafts, 32000 ids: 4.2 + 9.6.
 #include "common.hpp"
 #include "abi_util.hpp"
 #include "paged.hpp"

@@ -331,7 +331,8 @@ int64_t llmy_paged_plan_workspace_bytes(int32_t B, int32_t capacity);
  *     that would need more than are left gets none, nor does any after it that needs some;
  *     nor does one that passes width * page, or whose packed tokens pass `capacity`.
  * held, free_pages, n_free and page_table are updated; entries of page_table from held[b] on
- * and of free_pages from n_free on hold what they held.  Out: cu_seqlens [B + 1], the packed
+ * hold what they held, and those of free_pages from n_free on that or pages pushed and handed
+ * out again by the call.  Out: cu_seqlens [B + 1], the packed
  * tokens' bounds (sums of new_tokens, at most capacity); rows, positions [capacity]: each
  * packed token's sequence and position, both as the append takes them: position -1 where its
  * sequence got no place, row and position -1 behind the last token; lengths_out [B], with
